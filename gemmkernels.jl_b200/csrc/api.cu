@@ -29,7 +29,7 @@ void clear_error() { g_error[0] = 0; }
 // ------------------------------------------------------------------------------------------------
 // descriptor validation shared by every path
 // ------------------------------------------------------------------------------------------------
-static gk_status validate_desc(const gk_gemm_desc* d, const gk_epilogue_desc* epi) {
+gk_status validate_desc(const gk_gemm_desc* d, const gk_epilogue_desc* epi) {
   if (!d) return set_error(GK_ERR_INVALID_ARGUMENT, "descriptor is NULL");
   if (d->struct_size != sizeof(gk_gemm_desc))
     return set_error(GK_ERR_INVALID_ARGUMENT, "gk_gemm_desc.struct_size is %u, this library expects %zu",

@@ -84,6 +84,7 @@ struct gk_handle_s {
   int max_clusters[2][4] = {};     // tc kernel [planes-1][tf32 + 2*rank5] -> co-resident CTA pairs
   bool attr_set[2][2][2][4] = {};  // tc kernel [debug instance][cg-1][planes-1][tf32 + 2*rank5]: smem attribute set
   bool attr_set_generic[2] = {};   // the same for the generic-load instances
+  bool attr_set_fused[3][3] = {};  // layer-level instances [form-1][one CTA, CTA pair, generic loads]
   bool fpu_attr_set[12] = {};      // FFMA kernel instances (3 operand types x 4 transposes): shared-memory limit raised
   bool f64_attr_set[4] = {};       // FP64 kernel instances (4 transposes): shared-memory limit raised
   // staging buffers of gk_gemm_host (grown on demand, freed by gk_destroy)
@@ -97,6 +98,8 @@ struct gk_handle_s {
 };
 
 namespace gk {
+// api.cu: descriptor checks shared by every path
+gk_status validate_desc(const gk_gemm_desc* d, const gk_epilogue_desc* epi);
 // api.cu: grows staging buffer `slot` of the handle to at least `bytes` (never shrinks)
 gk_status stage_reserve(gk_handle h, int slot, size_t bytes);
 // api.cu: creates the two copy streams and at least `n_events` untimed events of the handle

@@ -1,0 +1,157 @@
+// The epilogues of the layer-level products (gk_gemm_fused), shared by the tensor-core kernel, the split-K
+// reduction and the streaming kernel for a few columns, and the column groups of ragged products.
+//
+//   x = alpha * (op(A) op(B))(m, n) + bias            (+ beta * C(m, n) in the STANDARD and GRADIENT forms)
+//   STANDARD   Z = x (kept on request)    D = act(x)
+//   RESIDUAL   Z = x (kept on request)    D = act(x) + beta * C
+//   GRADIENT   Z is read                  D = x * act'(Z)
+//
+// x, act and act' are FP32; D and Z are rounded once, when they are stored (act sees the unrounded x).
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace gk {
+
+enum FusedForm : int32_t { FUSED_STANDARD = 0, FUSED_RESIDUAL = 1, FUSED_GRADIENT = 2 };
+enum FusedAct : int32_t { FUSED_ACT_NONE = 0, FUSED_ACT_RELU = 1, FUSED_ACT_GELU = 2, FUSED_ACT_SILU = 3 };
+
+// What the fused forms of a kernel need beside C, D, alpha, beta, bias and act of the plain ones.
+struct FusedParams {
+  int32_t form;
+  int32_t dtype_z;
+  void* Z;                 // written (STANDARD, RESIDUAL; NULL: not kept) or read (GRADIENT)
+  int64_t z_sn;            // elements between the columns of Z
+  // column groups (ragged products): group g holds the columns offsets[g] .. offsets[g + 1] - 1
+  const void* offsets;     // device, groups + 1 values; NULL: one group of all `total` columns
+  int32_t offsets64;       // 0: 32-bit values, 1: 64-bit values
+  int32_t groups;
+  int32_t total;           // columns there are: offsets are clamped to [0, total]
+  int64_t bias_group;      // elements between the biases of consecutive groups
+};
+
+// FAST: the result is stored in 16 bits, whose half step (2^-12 relative at best) is far above the 2^-21 of
+// the hardware exponential and the approximate quotient; for FP32 results the accurate functions are used.
+template <bool FAST>
+__device__ __forceinline__ float fused_sigmoid(float x) {
+  if constexpr (FAST) return __fdividef(1.0f, 1.0f + __expf(-x));
+  return 1.0f / (1.0f + expf(-x));
+}
+
+// A NaN passes through every activation (ReLU as well: the comparison is false).
+template <bool FAST>
+__device__ __forceinline__ float fused_act(float x, int32_t act) {
+  if (act == FUSED_ACT_RELU) return x < 0.0f ? 0.0f : x;
+  if (act == FUSED_ACT_GELU) return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f));
+  if (act == FUSED_ACT_SILU) return x * fused_sigmoid<FAST>(x);
+  return x;
+}
+
+// act'(z), with ReLU'(0) = 0.  Where z multiplies something that has run out to zero it is clamped first, so
+// that an infinite z (a 16-bit pre-activation that overflowed) gives the limit, 0 or 1, instead of inf * 0.
+template <bool FAST>
+__device__ __forceinline__ float fused_act_gradient(float z, int32_t act) {
+  if (act == FUSED_ACT_RELU) return z > 0.0f ? 1.0f : (z <= 0.0f ? 0.0f : z);
+  if (act == FUSED_ACT_GELU) {   // Phi(z) + z phi(z)
+    const float c = fminf(fmaxf(z, -16.0f), 16.0f);
+    const float e = FAST ? __expf(-0.5f * c * c) : expf(-0.5f * c * c);
+    return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + c * (0.3989422804014327f * e);
+  }
+  if (act == FUSED_ACT_SILU) {
+    const float c = fminf(fmaxf(z, -80.0f), 80.0f);
+    const float s = fused_sigmoid<FAST>(z);
+    return s * (1.0f + c * (1.0f - s));
+  }
+  return 1.0f;
+}
+
+__device__ __forceinline__ float fused_load(const void* p, int64_t i, int dt) {   // dt: 0 F16, 1 BF16, 2 F32
+  if (dt == 2) return static_cast<const float*>(p)[i];
+  if (dt == 0) return __half2float(static_cast<const __half*>(p)[i]);
+  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+
+__device__ __forceinline__ void fused_put(void* p, int64_t i, int dt, float v) {
+  if (dt == 2) static_cast<float*>(p)[i] = v;
+  else if (dt == 0) static_cast<__half*>(p)[i] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+}
+
+// One element (m, n) for the kernels that finish element by element: x = alpha * sum + bias; keeps or reads Z and
+// returns D's value.  C is at element ci.
+__device__ __forceinline__ float fused_finish(const FusedParams& f, float x, float beta, const void* C, int64_t ci, int dtype_c,
+                                              int act, int m, int64_t n) {
+  const float c = beta != 0.0f ? beta * fused_load(C, ci, dtype_c) : 0.0f;
+  const int64_t zi = m + n * f.z_sn;
+  if (f.form != FUSED_RESIDUAL && beta != 0.0f) x += c;
+  if (f.form == FUSED_GRADIENT) return x * fused_act_gradient<false>(fused_load(f.Z, zi, f.dtype_z), act);
+  if (f.Z != nullptr) fused_put(f.Z, zi, f.dtype_z, x);
+  x = fused_act<false>(x, act);
+  return f.form == FUSED_RESIDUAL && beta != 0.0f ? x + c : x;
+}
+
+// Column group boundaries as a warp reads them: lane l of a chunk of 32 groups gets [lo, hi) of group
+// base + l.  Whatever the array holds, every value is clamped to [0, total] and the running maximum is
+// taken, so groups never overlap, never run backwards and never leave the matrix.  `carry` starts as
+// fused_first_offset() and is handed from chunk to chunk; all 32 lanes call.
+__device__ __forceinline__ int fused_offset(const FusedParams& f, int i) {
+  const long long v = f.offsets64 ? static_cast<const long long*>(f.offsets)[i]
+                                  : static_cast<long long>(static_cast<const int32_t*>(f.offsets)[i]);
+  return static_cast<int>(v < 0 ? 0 : (v > f.total ? f.total : v));
+}
+
+__device__ __forceinline__ int fused_first_offset(const FusedParams& f) { return f.offsets ? fused_offset(f, 0) : 0; }
+
+__device__ __forceinline__ void fused_group_chunk(const FusedParams& f, int base, int lane, int& carry, int& lo, int& hi) {
+  const int g = base + lane;
+  int v = g < f.groups ? (f.offsets ? fused_offset(f, g + 1) : f.total) : 0;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int o = __shfl_up_sync(0xffffffffu, v, d);
+    if (lane >= d) v = max(v, o);
+  }
+  hi = max(v, carry);
+  lo = __shfl_up_sync(0xffffffffu, hi, 1);
+  if (lane == 0) lo = carry;
+  carry = __shfl_sync(0xffffffffu, hi, 31);
+}
+
+// Inclusive sum over the lanes of a warp.
+__device__ __forceinline__ int fused_warp_scan(int v, int lane) {
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int o = __shfl_up_sync(0xffffffffu, v, d);
+    if (lane >= d) v += o;
+  }
+  return v;
+}
+
+// The block's work item in a list that deals every group out in chunks of at most `per` columns:
+// item -> group g, first column c0, columns n (n == 0: the list is shorter than `item`).  Called by one
+// whole warp; all lanes get the answer.
+__device__ __forceinline__ void fused_find_item(const FusedParams& f, int item, int per, int lane, int& g, int& c0, int& n) {
+  g = 0; c0 = 0; n = 0;
+  int carry = fused_first_offset(f);
+  int first = 0;   // items before this chunk of groups
+  for (int base = 0; base < f.groups; base += 32) {
+    int lo, hi;
+    fused_group_chunk(f, base, lane, carry, lo, hi);
+    const int items = (hi - lo + per - 1) / per;
+    const int incl = fused_warp_scan(items, lane);
+    const int before = first + incl - items;
+    const unsigned hit = __ballot_sync(0xffffffffu, item >= before && item < before + items);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      g = base + src;
+      const int k = item - __shfl_sync(0xffffffffu, before, src);
+      c0 = __shfl_sync(0xffffffffu, lo, src) + k * per;
+      n = min(per, __shfl_sync(0xffffffffu, hi, src) - c0);
+      return;
+    }
+    first += __shfl_sync(0xffffffffu, incl, 31);
+  }
+}
+
+}  // namespace gk

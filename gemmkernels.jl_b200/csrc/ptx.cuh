@@ -134,6 +134,19 @@ __device__ __forceinline__ void prefetch_tensormap(const void* tmap) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(tmap)) : "memory");
 }
 
+// A tensor map in global memory: its second extent is replaced (generic proxy), the release makes that visible
+// to the acquire of the thread that loads through it.
+__device__ __forceinline__ void tensormap_set_extent1(void* tmap, uint32_t extent) {
+  asm volatile("tensormap.replace.tile.global_dim.global.b1024.b32 [%0], 1, %1;" ::"l"(__cvta_generic_to_global(tmap)), "r"(extent)
+               : "memory");
+}
+__device__ __forceinline__ void fence_tensormap_release() {
+  asm volatile("fence.proxy.tensormap::generic.release.gpu;" ::: "memory");
+}
+__device__ __forceinline__ void fence_tensormap_acquire(const void* tmap) {
+  asm volatile("fence.proxy.tensormap::generic.acquire.gpu [%0], 128;" ::"l"(reinterpret_cast<uint64_t>(tmap)) : "memory");
+}
+
 // 3-D tiled load, completion counted in bytes on `bar` (a barrier of the executing CTA).
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, uint32_t bar, int c0,
                                             int c1, int c2) {

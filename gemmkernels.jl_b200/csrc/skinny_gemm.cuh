@@ -1,0 +1,195 @@
+// Products with a few columns (a few tokens): D[:, J] = epilogue(op(A_g) B[:, J]) for at most NT columns at a time.
+//
+// With one to a few columns every weight is used that often and no more: the product is a stream of A at the rate of
+// HBM, 2 * NT flop per 2 bytes, far below what the FP32 FMA pipe does (NT = 4: 13 TFMA/s at 6.6 TB/s of 36).  The
+// tensor-core kernel reaches its first MMA only after barrier, TMEM and first-copy latencies that are as long as
+// the whole stream of a 4096 x 4096 layer (5.1 us at 6.57 TB/s), so plain 16-byte loads feed FMAs directly.
+//
+// A cluster of S CTAs owns 64 rows of D; its CTA r takes the r-th run of K, so that a layer with few rows still has
+// loads in flight on every SM (S is chosen on the host: two CTAs per SM).  The CTAs' partial sums meet in
+// distributed shared memory, where each CTA adds one slice of the 64 x NT outputs in the order of the ranks (the
+// result does not depend on timing) and applies the epilogue.
+//   K_MAJOR  (A stored with consecutive k): a warp owns 8 rows, its lanes 8 consecutive k each
+//   M_MAJOR  (A stored with consecutive rows): 8 lanes own 8 rows each; the other 32 slots of the CTA (4 per warp)
+//            take 8 consecutive k each
+// Either way a thread has eight 16-byte loads of A in flight and 8 x NT accumulators.
+#pragma once
+#include "fused_epilogue.cuh"
+#include "ptx.cuh"
+
+namespace gk {
+
+constexpr int kSkinnyThreads = 256;
+constexpr int kSkinnyRows = 64;        // rows of D per cluster
+constexpr int kSkinnyStep = 256;       // K consumed per step of a CTA (K runs are multiples of it)
+
+struct SkinnyParams {
+  const void* A; const void* B; const void* C; void* D;
+  int32_t M, K;
+  int64_t lda, ldb, ldc, ldd;
+  int64_t a_group;             // elements between the groups' A
+  float alpha, beta;
+  const float* bias;
+  int32_t bias_axis, act;      // 0 none, 1 per row, 2 per column
+  int32_t dtype_d;             // of C, D and Z: 0 F16, 1 BF16, 2 F32
+  int32_t k_per_rank;          // K run of a CTA, a multiple of kSkinnyStep
+  FusedParams f;
+};
+
+__device__ __forceinline__ uint4 skinny_load_stream(const void* p) {   // weights: used once, not kept in L1
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
+template <typename T> __device__ __forceinline__ void skinny_unpack(const uint4& v, float (&f)[8]);
+template <> __device__ __forceinline__ void skinny_unpack<__nv_bfloat16>(const uint4& v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float(w[i] << 16);
+    f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+template <> __device__ __forceinline__ void skinny_unpack<__half>(const uint4& v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    f[2 * i] = t.x; f[2 * i + 1] = t.y;
+  }
+}
+
+__device__ __forceinline__ float skinny_load_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+  return v;
+}
+
+// Sums v over the lanes that differ in bits `kFrom` .. `kTo` (powers of two, kFrom > kTo), halving the number of
+// values a lane holds at every step while there are several; returns the index of the lane's first value.
+template <int V, int kFrom, int kTo>
+__device__ __forceinline__ int skinny_reduce(float (&v)[V], int lane) {
+  int n = V, first = 0;
+#pragma unroll
+  for (int o = kFrom; o >= kTo; o >>= 1) {
+    if (n > 1) {
+      n >>= 1;
+      const bool up = (lane & o) != 0;
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) {
+        if (i < n) {
+          const float send = up ? v[i] : v[i + n];
+          const float keep = up ? v[i + n] : v[i];
+          v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+        }
+      }
+      if (up) first += n;
+    } else {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+    }
+  }
+  return first;
+}
+
+template <typename T, bool K_MAJOR, int NT>
+__global__ void __launch_bounds__(kSkinnyThreads, 2) skinny_gemm_kernel(const SkinnyParams p) {
+  constexpr int kOut = kSkinnyRows * NT;
+  __shared__ float part[K_MAJOR ? 1 : 8][kOut];   // M_MAJOR: sums of each warp
+  __shared__ float sum[kOut];                     // sums of this CTA's K run, [column][row]
+  __shared__ int item[3];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t ranks;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
+  const uint32_t rank = cluster_cta_rank();
+  const int row0 = static_cast<int>(blockIdx.x / ranks) * kSkinnyRows;
+
+  pdl_launch_dependents();
+  pdl_wait();
+  if (warp == 0) {
+    int g, c0, n;
+    fused_find_item(p.f, blockIdx.y, NT, lane, g, c0, n);
+    if (lane == 0) { item[0] = g; item[1] = c0; item[2] = n; }
+  }
+  __syncthreads();
+  const int g = item[0], c0 = item[1], n = item[2];
+  if (n == 0) return;    // the list is shorter than the grid; the same for every CTA of the cluster
+
+  const T* A = static_cast<const T*>(p.A) + g * p.a_group;
+  const T* B = static_cast<const T*>(p.B) + c0 * p.ldb;
+  const int k_begin = static_cast<int>(rank) * p.k_per_rank;
+  const int k_end = min(k_begin + p.k_per_rank, p.K);
+  float acc[8 * NT];     // [row][column]
+#pragma unroll
+  for (int i = 0; i < 8 * NT; ++i) acc[i] = 0.0f;
+
+  const int slot = K_MAJOR ? lane : warp * 4 + (lane >> 3);
+  const int row = K_MAJOR ? row0 + warp * 8 : row0 + (lane & 7) * 8;    // the thread's first row
+  const bool row_ok = row < p.M;
+  for (int k = k_begin + slot * 8; k < k_end; k += kSkinnyStep) {
+    uint4 w[8], x[NT];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      // rows behind the last one re-read it (their sums are not stored); M_MAJOR has whole runs of 8 rows
+      const T* src = K_MAJOR ? A + static_cast<int64_t>(min(row + i, p.M - 1)) * p.lda + k
+                             : A + static_cast<int64_t>(k + i) * p.lda + (row_ok ? row : 0);
+      w[i] = skinny_load_stream(src);
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      x[t] = make_uint4(0u, 0u, 0u, 0u);
+      if (t < n) x[t] = *reinterpret_cast<const uint4*>(B + t * p.ldb + k);
+    }
+    float xf[NT][8];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) skinny_unpack<T>(x[t], xf[t]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float wf[8];
+      skinny_unpack<T>(w[i], wf);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          if constexpr (K_MAJOR) acc[i * NT + t] = fmaf(wf[j], xf[t][j], acc[i * NT + t]);
+          else acc[j * NT + t] = fmaf(wf[j], xf[t][i], acc[j * NT + t]);
+        }
+    }
+  }
+
+  if constexpr (K_MAJOR) {
+    const int first = skinny_reduce<8 * NT, 16, 1>(acc, lane);
+    constexpr int kCopies = NT >= 4 ? 1 : 4 / NT;     // lanes that end up with the same value
+    if (lane % kCopies == 0) sum[(first % NT) * kSkinnyRows + warp * 8 + first / NT] = acc[0];
+  } else {
+    const int first = skinny_reduce<8 * NT, 16, 8>(acc, lane);
+#pragma unroll
+    for (int i = 0; i < 2 * NT; ++i)
+      part[warp][((first + i) % NT) * kSkinnyRows + (lane & 7) * 8 + (first + i) / NT] = acc[i];
+    __syncthreads();
+    for (int o = threadIdx.x; o < kOut; o += kSkinnyThreads) {
+      float s = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) s += part[w][o];
+      sum[o] = s;
+    }
+  }
+  __syncthreads();
+  if (ranks > 1) cluster_sync_all();
+  const int mine = kOut / static_cast<int>(ranks);
+  const uint32_t sum_addr = smem_u32(sum);
+  for (int o = static_cast<int>(rank) * mine + threadIdx.x; o < static_cast<int>(rank + 1) * mine; o += kSkinnyThreads) {
+    float s = 0.0f;
+    for (uint32_t r = 0; r < ranks; ++r) s += skinny_load_cluster(map_to_cta(sum_addr + 4u * o, r));
+    const int t = o / kSkinnyRows, m = row0 + o % kSkinnyRows;
+    if (t >= n || m >= p.M) continue;
+    const int64_t col = c0 + t;
+    const float bias = p.bias_axis == 1 ? p.bias[m + g * p.f.bias_group] : (p.bias_axis == 2 ? p.bias[col] : 0.0f);
+    fused_put(p.D, m + col * p.ldd, p.dtype_d,
+              fused_finish(p.f, fmaf(p.alpha, s, bias), p.beta, p.C, m + col * p.ldc, p.dtype_d, p.act, m, col));
+  }
+  if (ranks > 1) cluster_sync_all();     // the peers have read this CTA's sums
+}
+
+}  // namespace gk

@@ -12,6 +12,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "fused_epilogue.cuh"
+
 namespace gk {
 
 struct SplitKReduceParams {
@@ -29,6 +31,8 @@ struct SplitKReduceParams {
   int64_t d_sm0, d_sm1, d_sn0, d_sn1, d_plane;
   const float* bias; int bias_axis;          // 0 none, 1 per row, 2 per column
   int act;                                   // 0 none, 1 ReLU, 2 GELU
+  int fused;                                 // 1: the epilogue of `f` (plain one-plane matrices) instead
+  FusedParams f;
 };
 
 __device__ __forceinline__ float splitk_load(const void* p, int64_t i, int dt) {
@@ -44,6 +48,10 @@ __device__ __forceinline__ void splitk_store(void* p, int64_t i, int dt, float v
 }
 
 __device__ __forceinline__ float splitk_finish(const SplitKReduceParams& p, float sum, int m, int n, int pl, int64_t ci) {
+  if (p.fused) {
+    const float bias = p.bias_axis == 1 ? p.bias[m] : (p.bias_axis == 2 ? p.bias[n] : 0.0f);
+    return fused_finish(p.f, p.alpha * sum + bias, p.beta, p.C, ci, p.dtype_c, p.act, m, n);
+  }
   float x = p.alpha * sum;
   if (p.beta != 0.0f) x += p.beta * splitk_load(p.C, p.planes == 2 && p.c_plane == 0 ? 2 * ci + pl : pl * p.c_plane + ci, p.dtype_c);
   if (pl == 0) {

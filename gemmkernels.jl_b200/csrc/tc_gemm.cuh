@@ -20,7 +20,20 @@
 // Every barrier wait is bounded (ptx.cuh: mbar_wait).  When a wait gives up, the CTA raises a
 // shared abort flag, all roles leave their loops, in-flight copies and MMAs are drained with
 // bounded waits, TMEM is released, and an error code is left in *status for the host.
+//
+// FORM selects the layer-level instances (gk_gemm_fused; 16-bit operands, one plane):
+//   kTcFused        one product with the epilogues of fused_epilogue.cuh
+//   kTcRaggedCols   D[:, J_g] = epilogue(op(A_g) B[:, J_g]): the columns J_g of group g are known on the device
+//                   only.  Every CTA turns the offsets into a table of (first tile, first column, last column)
+//                   per group in shared memory; the persistent walk runs over the groups' tiles as one list.  A
+//                   tile may load columns of the next group (they only reach accumulator columns that are not
+//                   stored), so one tensor map serves all groups, wherever they begin.
+//   kTcRaggedDepth  D_g = A[:, J_g] B[:, J_g]^T: the group is a run of K.  Here what lies behind the run must
+//                   not be read (0 * inf), so every group has its own pair of tensor maps, written on the device
+//                   by tc_depth_maps_kernel: the same matrix cut off behind the group's last column, which TMA
+//                   fills with zeros.
 #pragma once
+#include "fused_epilogue.cuh"
 #include "ptx.cuh"
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -40,6 +53,8 @@ constexpr uint64_t kTcWaitLimitNs = 1000ull * 1000ull * 1000ull;  // 1 s per wai
 enum TcDtype : int32_t { TC_F16 = 0, TC_BF16 = 1, TC_F32 = 2 };
 enum TcAct : int32_t { TC_ACT_NONE = 0, TC_ACT_RELU = 1, TC_ACT_GELU = 2 };
 enum TcBias : int32_t { TC_BIAS_NONE = 0, TC_BIAS_ROW = 1, TC_BIAS_COL = 2 };
+
+enum TcForm : int { kTcPlain = 0, kTcFused = 1, kTcRaggedCols = 2, kTcRaggedDepth = 3 };
 
 // status word values (0 = ok)
 enum TcStatus : int32_t {
@@ -130,7 +145,52 @@ struct TcParams {
                   // 8 = per-role cycle counters written to dbg_out[blockIdx.x * 16 + i],
                   // 16 = CTA 0 leaves progress marks in the host-visible diagnostic words
   long long* dbg_out;
+  // FORM != kTcPlain
+  FusedParams f;
+  int32_t col_align;          // kTcRaggedCols: a group's first tile starts at a multiple of this many columns (8
+                              // where TMA needs it: B with consecutive columns; columns before the group are not stored)
+  const CUtensorMap* maps;    // kTcRaggedDepth: maps of A and B for group g at maps[2g], maps[2g + 1]
 };
+
+// Group table of the ragged forms, behind the control block: first tile of each group (groups + 1 values), then
+// first and last + 1 column of each.
+constexpr int kTcCtrlBytes = 256;
+__host__ __device__ constexpr int tc_table_bytes(int groups) { return (3 * groups + 1) * 4; }
+
+template <int FORM>
+__device__ __forceinline__ void tc_build_table(const TcParams& p, int* tab, int lane) {
+  const int G = p.f.groups;
+  const int bn_tile = p.bn * p.n_sub;
+  int carry = fused_first_offset(p.f), tiles = 0;
+  for (int base = 0; base < G; base += 32) {
+    int lo, hi;
+    fused_group_chunk(p.f, base, lane, carry, lo, hi);
+    const int g = base + lane;
+    if constexpr (FORM == kTcRaggedCols) {
+      lo = min(lo, hi);
+      const int first = lo - lo % p.col_align;
+      const int mine = hi > lo ? p.tiles_m * ((hi - first + bn_tile - 1) / bn_tile) : 0;
+      const int incl = fused_warp_scan(mine, lane);
+      if (g < G) tab[g] = tiles + incl - mine;
+      tiles += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (g < G) { tab[G + 1 + g] = lo; tab[2 * G + 1 + g] = hi; }
+  }
+  if (lane == 0) tab[G] = FORM == kTcRaggedCols ? tiles : p.tiles_m * p.tiles_n * G;
+}
+
+// kTcRaggedCols: unit t of the list -> group (the cursor g only moves forward) and tile of it.
+__device__ __forceinline__ void tc_group_tile(const TcParams& p, const int* tab, int t, int& g, int& tm, int& tn) {
+  while (t >= tab[g + 1]) ++g;
+  const int first = tab[g], r = t - first;
+  const int tiles_n = (tab[g + 1] - first) / p.tiles_m;
+  const int band = p.raster_group * tiles_n;       // bands of raster_group tiles down M, stepping along the group's columns
+  const int band_id = r / band, row0 = band_id * p.raster_group;
+  const int rows = min(p.raster_group, p.tiles_m - row0);
+  const int q = r - band_id * band;
+  tm = row0 + q % rows;
+  tn = q / rows;
+}
 
 // The status word may live in host-mapped memory: plain stores, first error wins.
 __device__ __forceinline__ void tc_report(int32_t* status, int32_t code) {
@@ -256,6 +316,69 @@ __device__ __forceinline__ void tc_epilogue_chunk(const TcParams& p, const uint3
   }
 }
 
+// Epilogue of up to 32 columns of one row in the fused forms: bit j of `live` says that column j of the chunk exists.
+// d, c and z point at column 0 of the chunk; C and Z have D's type T.  Sixteen columns at a time: their loads of C
+// and Z are issued before the first use, and what is live fits the 168 registers of a 384-thread CTA.
+template <typename T>
+__device__ __forceinline__ void tc_fused_chunk(const TcParams& p, const uint32_t (&v)[32], T* d, const T* c, T* z, float bias_row,
+                                               int col0, uint32_t live) {
+  constexpr bool kFast = sizeof(T) == 2;
+  constexpr int W = 16;
+  const bool gradient = p.f.form == FUSED_GRADIENT, residual = p.f.form == FUSED_RESIDUAL;
+  const bool has_c = p.beta != 0.0f;
+  // Column pointers advance by additions that the compiler cannot see through: left alone it keeps the 32
+  // multiples of each stride in registers and spills (800 bytes a thread).
+  auto advance = [](auto*& ptr, int64_t step) { ptr += step; asm volatile("" : "+l"(ptr)); };
+#pragma unroll
+  for (int h = 0; h < 32; h += W) {
+    auto in = [&](int j) { return (live >> (h + j)) & 1u; };
+    T cv[W], zv[W];
+    if (has_c) {
+#pragma unroll
+      for (int j = 0; j < W; ++j, advance(c, p.c_sn0))
+        if (in(j)) cv[j] = *c;
+    }
+    if (gradient) {
+#pragma unroll
+      for (int j = 0; j < W; ++j, advance(z, p.f.z_sn))
+        if (in(j)) zv[j] = *z;
+    }
+    float x[W];
+#pragma unroll
+    for (int j = 0; j < W; ++j) x[j] = fmaf(p.alpha, __uint_as_float(v[h + j]), bias_row);
+    if (p.bias_axis == TC_BIAS_COL) {
+#pragma unroll
+      for (int j = 0; j < W; ++j)
+        if (in(j)) x[j] += p.bias[col0 + h + j];
+    }
+    if (has_c && !residual) {
+#pragma unroll
+      for (int j = 0; j < W; ++j)
+        if (in(j)) x[j] += p.beta * tc_to_float(cv[j]);
+    }
+    if (gradient) {
+#define GK_EACH(expr) _Pragma("unroll") for (int j = 0; j < W; ++j) if (in(j)) { expr; }
+      if (p.act == TC_ACT_RELU) { GK_EACH(x[j] *= fused_act_gradient<kFast>(tc_to_float(zv[j]), TC_ACT_RELU)) }
+      else if (p.act == TC_ACT_GELU) { GK_EACH(x[j] *= fused_act_gradient<kFast>(tc_to_float(zv[j]), TC_ACT_GELU)) }
+      else if (p.act == FUSED_ACT_SILU) { GK_EACH(x[j] *= fused_act_gradient<kFast>(tc_to_float(zv[j]), FUSED_ACT_SILU)) }
+    } else {
+      if (p.f.Z != nullptr) {
+#pragma unroll
+        for (int j = 0; j < W; ++j, advance(z, p.f.z_sn))
+          if (in(j)) *z = tc_from_float<T>(x[j]);
+      }
+      if (p.act == TC_ACT_RELU) { GK_EACH(x[j] = fused_act<kFast>(x[j], TC_ACT_RELU)) }
+      else if (p.act == TC_ACT_GELU) { GK_EACH(x[j] = fused_act<kFast>(x[j], TC_ACT_GELU)) }
+      else if (p.act == FUSED_ACT_SILU) { GK_EACH(x[j] = fused_act<kFast>(x[j], FUSED_ACT_SILU)) }
+      if (has_c && residual) { GK_EACH(x[j] += p.beta * tc_to_float(cv[j])) }
+    }
+#undef GK_EACH
+#pragma unroll
+    for (int j = 0; j < W; ++j, advance(d, p.d_sn0))
+      if (in(j)) *d = tc_from_float<T>(x[j]);
+  }
+}
+
 // Even-position bits of x packed together (bit 0, 2, 4, ... -> bit 0, 1, 2, ...).
 __device__ __forceinline__ uint32_t tc_even_bits(uint32_t x) {
   x &= 0x55555555u;
@@ -347,10 +470,11 @@ __device__ __forceinline__ void tc_issue_kblock(uint32_t lo, bool first, uint32_
 // DBG selects the instance that honours TcParams::debug (measurement and test aids); in the production
 // instance every such branch is compiled out, which shortens the per-stage loops of the producer and
 // MMA warps (their cost per pipeline stage is instruction latency, not bandwidth).
-template <int CG, int PLANES, bool TF32, bool RANK5, bool GENERIC = false, bool DBG = false>
+template <int CG, int PLANES, bool TF32, bool RANK5, bool GENERIC = false, bool DBG = false, int FORM = kTcPlain>
 __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __grid_constant__ TcParams p) {
   const int dbg = DBG ? p.debug : 0;
   static_assert(!GENERIC || (CG == 1 && PLANES == 1 && !TF32 && !RANK5), "generic loads: one CTA, one plane, 16-bit types");
+  static_assert(FORM == kTcPlain || (PLANES == 1 && !TF32 && !RANK5 && !DBG), "fused forms: one plane, 16-bit types");
   extern __shared__ uint8_t smem_raw[];
   // 128-byte swizzle atoms are 1024 bytes and the pattern is a function of the address.
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -394,14 +518,23 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
     mbar_init(bar_drain, 1);
     *abort_flag = 0;
     fence_mbar_init();
-    if constexpr (!GENERIC) {
-      prefetch_tensormap(&p.tm_a);
-      prefetch_tensormap(&p.tm_b);
+    if constexpr (!GENERIC && FORM != kTcRaggedDepth) {
+      if (FORM == kTcPlain || p.k_blocks > 0) {   // a product of nothing (K = 0) has no maps
+        prefetch_tensormap(&p.tm_a);
+        prefetch_tensormap(&p.tm_b);
+      }
     }
   }
   if (warp == 2) {
     tmem_alloc<CG>(tmem_slot, p.tmem_cols);
     tmem_relinquish<CG>();
+  }
+  [[maybe_unused]] int* const tab = reinterpret_cast<int*>(ctrl_gen + kTcCtrlBytes);
+  if constexpr (FORM >= kTcRaggedCols) {
+    if (warp == 4) {
+      pdl_wait();             // the offsets may be the previous kernel's output
+      tc_build_table<FORM>(p, tab, lane);
+    }
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -411,7 +544,7 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
   if (threadIdx.x == 0) tc_mark(p.status, dbg, 1, 1);   // set-up done, TMEM allocated
 
   const int units_per_product = p.tiles_m * p.tiles_n * p.k_split;
-  const int num_tiles = units_per_product * p.batch;         // work units
+  const int num_tiles = FORM >= kTcRaggedCols ? tab[p.f.groups] : units_per_product * p.batch;   // work units
   const int cluster_id = blockIdx.x / CG;
   const int num_clusters = gridDim.x / CG;
   const int bn_cta = p.bn / CG;
@@ -419,7 +552,7 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
   const uint32_t sub_cols = PLANES * p.bn;  // TMEM columns per column block
   const uint32_t acc_cols = p.n_sub * sub_cols;  // TMEM columns per accumulator stage
   const bool two_acc = p.acc_stages == 2;
-  const bool skew = !DBG && !GENERIC && PLANES == 1 && p.skew != 0;   // the diagnostic instance keeps the plain schedule
+  const bool skew = !DBG && !GENERIC && PLANES == 1 && FORM <= kTcFused && p.skew != 0;   // the diagnostic instance keeps the plain schedule
 
   if constexpr (GENERIC) {
     if (warp == 0 || warp == 3) {
@@ -438,12 +571,23 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
       uint32_t ph = 0;
       bool ok = true;
       pdl_wait();
+      [[maybe_unused]] int grp = 0;
       for (int t = cluster_id; t < num_tiles && ok && !(dbg & 4); t += num_clusters) {
         int tm, tn;
-        const int bt = t / units_per_product;
-        tc_tile_coords(p, (t - bt * units_per_product) / p.k_split, tm, tn);
-        const int kb0 = (t % p.k_split) * p.kb_per_split, kb1 = min(kb0 + p.kb_per_split, p.k_blocks);
-        const int mn0 = is_a ? tm * kTcTileM : tn * bn_tile;
+        int bt = t / units_per_product;
+        if constexpr (FORM == kTcRaggedCols) { tc_group_tile(p, tab, t, grp, tm, tn); bt = grp; }
+        else tc_tile_coords(p, (t - bt * units_per_product) / p.k_split, tm, tn);
+        const int kb0 = FORM == kTcPlain ? (t % p.k_split) * p.kb_per_split : 0;
+        int kb1 = FORM == kTcPlain ? min(kb0 + p.kb_per_split, p.k_blocks) : p.k_blocks;
+        int mn0 = is_a ? tm * kTcTileM : tn * bn_tile;
+        int k_first = 0, k_ext = p.K;          // K range of the unit
+        if constexpr (FORM == kTcRaggedCols) {
+          if (!is_a) mn0 += tab[p.f.groups + 1 + bt];
+        }
+        if constexpr (FORM == kTcRaggedDepth) {
+          k_first = tab[p.f.groups + 1 + bt]; k_ext = tab[2 * p.f.groups + 1 + bt];
+          kb1 = (k_ext - k_first + p.bk - 1) / p.bk;
+        }
         const uint16_t* g = static_cast<const uint16_t*>(is_a ? p.ga : p.gb) + bt * (is_a ? p.g_a_batch : p.g_b_batch);
         for (int kb = kb0; kb < kb1; kb += p.kps) {
           const bool got = mbar_wait(bar_empty + 8u * s, ph ^ 1u, abort_flag, kTcWaitLimitNs);
@@ -454,12 +598,12 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
           }
           for (int j = 0; j < p.kps; ++j) {
             uint8_t* stage = smem_gen + s * stage_bytes + j * kblock_bytes + part_off;
-            const int k0 = (kb + j) * p.bk;
+            const int k0 = k_first + (kb + j) * p.bk;
             if (mn_major) {
               for (int bx = 0; bx < boxes; ++bx)
-                tc_fill_box_generic(stage + bx * box_bytes, g, ld, mn0 + bx * box_mn, k0, mn_ext, p.K, p.bk, lane);
+                tc_fill_box_generic(stage + bx * box_bytes, g, ld, mn0 + bx * box_mn, k0, mn_ext, k_ext, p.bk, lane);
             } else {
-              tc_fill_box_generic(stage, g, ld, k0, mn0, p.K, mn_ext, rows_k_major, lane);
+              tc_fill_box_generic(stage, g, ld, k0, mn0, k_ext, mn_ext, rows_k_major, lane);
             }
           }
           fence_proxy_async_smem();   // the tensor cores read shared memory through the asynchronous proxy
@@ -508,6 +652,7 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
                 : p.a_planes * p.a_plane_bytes + nb * b_sub_bytes + pl * p.b_plane_bytes + bx * p.b_box_bytes) +
           (RANK5 ? sb * (is_a ? p.a_sub_bytes : p.b_sub_bytes) : 0) + kj * kblock_bytes;
       const void* tmap = is_a ? static_cast<const void*>(&p.tm_a) : static_cast<const void*>(&p.tm_b);
+      [[maybe_unused]] int grp = 0, map_of = -1;      // ragged forms: the unit's group, the group `tmap` belongs to
       const int mn_add = (mn_major ? bx * (is_a ? p.a_box_mn : p.b_box_mn) : sb * sub_step) + nb * p.bn;
       [[maybe_unused]] const int k_add = mn_major ? sb * sub_step : 0;
       [[maybe_unused]] const int perm = is_a ? p.a_perm : p.b_perm;
@@ -526,12 +671,29 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
       pdl_wait();           // operands may be the previous kernel's output
       for (int t = cluster_id; t < num_tiles && ok && !(dbg & 4); t += num_clusters) {
         int tm, tn;
-        const int bt = t / units_per_product;                 // which product of the batch
-        tc_tile_coords(p, (t - bt * units_per_product) / p.k_split, tm, tn);
-        const int kb0 = (t % p.k_split) * p.kb_per_split, kb1 = min(kb0 + p.kb_per_split, p.k_blocks);
+        int bt = t / units_per_product;                       // which product of the batch (or which group)
+        if constexpr (FORM == kTcRaggedCols) { tc_group_tile(p, tab, t, grp, tm, tn); bt = grp; }
+        else tc_tile_coords(p, (t - bt * units_per_product) / p.k_split, tm, tn);
+        const int kb0 = FORM == kTcPlain ? (t % p.k_split) * p.kb_per_split : 0;
+        int kb1 = FORM == kTcPlain ? min(kb0 + p.kb_per_split, p.k_blocks) : p.k_blocks;
         [[maybe_unused]] const int c2 = pl + bt * (is_a ? p.a_batched : p.b_batched);   // plane, or product of a batch
         const int m_cta = (tm * CG + static_cast<int>(rank)) * kTcTileM;
-        const int n_cta = tn * bn_tile + static_cast<int>(rank) * bn_cta;
+        int n_cta = tn * bn_tile + static_cast<int>(rank) * bn_cta;
+        [[maybe_unused]] int k_first = 0;
+        if constexpr (FORM == kTcRaggedCols) {
+          const int lo = tab[p.f.groups + 1 + grp];
+          n_cta += lo - lo % p.col_align;
+        }
+        if constexpr (FORM == kTcRaggedDepth) {
+          k_first = tab[p.f.groups + 1 + bt];
+          kb1 = (tab[2 * p.f.groups + 1 + bt] - k_first + p.bk - 1) / p.bk;
+          if (kb1 > 0 && map_of != bt) {
+            // the maps were written by the kernel before this one, through the generic proxy
+            tmap = p.maps + 2 * bt + (is_a ? 0 : 1);
+            fence_tensormap_acquire(tmap);
+            map_of = bt;
+          }
+        }
         const int mn = (is_a ? m_cta : n_cta) + mn_add;
         // RANK5: the two-mode split of the M/N coordinate is fixed for the tile, and that of the K
         // coordinate advances by one k-block per step: no division inside the k loop.
@@ -558,7 +720,7 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
               // Bytes may be counted on the barrier before they are expected: the phase cannot
               // complete until the arrival that announces them.
               if (lane == 0 && leader) mbar_arrive_expect_tx(bar_full + 8u * s, tx_bytes);
-              const int k0 = (kb + kj) * p.bk;     // a k-block past the end of K (or of this K-run) is loaded too:
+              const int k0 = (FORM == kTcRaggedDepth ? k_first : 0) + (kb + kj) * p.bk;     // a k-block past the end of K (or of this K-run) is loaded too:
                                                    // zeros, or operands the MMA issuer does not use
               const uint32_t dst = smem_base + s * stage_bytes + dst_off;
               if constexpr (RANK5) {
@@ -675,7 +837,8 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
             // k-blocks (F = the ring's depth) go into block 0 as soon as the epilogue has drained it, then -
             // once block 1 is drained too - into block 1, which is what releases their stages.  Tail: the last
             // F k-blocks go into block 0 first, its accumulator is handed to the epilogue, then into block 1.
-            const int kb0 = (t % p.k_split) * p.kb_per_split, kb1 = min(kb0 + p.kb_per_split, p.k_blocks);
+            const int kb0 = FORM == kTcPlain ? (t % p.k_split) * p.kb_per_split : 0;
+            const int kb1 = FORM == kTcPlain ? min(kb0 + p.kb_per_split, p.k_blocks) : p.k_blocks;
             const int nkb = kb1 - kb0, F = p.stages;
             auto await = [&](uint32_t bar, uint32_t par) -> bool {
               const bool g = mbar_wait(bar, par, abort_flag, kTcWaitLimitNs);
@@ -745,7 +908,12 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
         }
         tc_fence_after_sync();
         const uint32_t d_base = tmem_base + as * acc_cols;
-        const int kb0 = (t % p.k_split) * p.kb_per_split, kb1 = min(kb0 + p.kb_per_split, p.k_blocks);
+        const int kb0 = FORM == kTcPlain ? (t % p.k_split) * p.kb_per_split : 0;
+        int kb1 = FORM == kTcPlain ? min(kb0 + p.kb_per_split, p.k_blocks) : p.k_blocks;
+        if constexpr (FORM == kTcRaggedDepth) {
+          const int bt = t / units_per_product;
+          kb1 = (tab[2 * p.f.groups + 1 + bt] - tab[p.f.groups + 1 + bt] + p.bk - 1) / p.bk;
+        }
         bool first_kb = true;   // the first k-block of a tile (or K-run) overwrites the accumulators
         for (int kb = kb0; kb < kb1; kb += p.kps) {
           if (prof) t0 = clock64();
@@ -822,13 +990,22 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
     // plain matrices only (a contraction's C is addressed through two-level strides), planar or real
     pdl_wait();             // D (and C) may still be in use by the previous kernel
     const bool prefetch_c = has_c && p.m_div >= p.M && p.n_div >= p.N && p.c_sm0 == 1 && (PLANES == 1 || p.c_plane != 0);
+    [[maybe_unused]] int grp = 0;
     for (int t = cluster_id; t < num_tiles && ok; t += num_clusters, ++acc_it) {
       int tm, tn;
-      const int bt = t / units_per_product;
-      tc_tile_coords(p, (t - bt * units_per_product) / p.k_split, tm, tn);
-      const int64_t split_off = static_cast<int64_t>(t % p.k_split) * p.split_stride;
+      int bt = t / units_per_product;
+      if constexpr (FORM == kTcRaggedCols) { tc_group_tile(p, tab, t, grp, tm, tn); bt = grp; }
+      else tc_tile_coords(p, (t - bt * units_per_product) / p.k_split, tm, tn);
+      const int64_t split_off = FORM == kTcPlain ? static_cast<int64_t>(t % p.k_split) * p.split_stride : 0;
       const int m = (tm * CG + static_cast<int>(rank)) * kTcTileM + q * 32 + lane;
-      const int n0 = tn * bn_tile;
+      int n0 = tn * bn_tile;
+      [[maybe_unused]] int n_lo = 0, n_hi = p.N;              // columns of the unit's group
+      [[maybe_unused]] bool nothing = FORM != kTcPlain && p.k_blocks == 0;   // no k-block: the accumulators hold nothing
+      if constexpr (FORM == kTcRaggedCols) {
+        n_lo = tab[p.f.groups + 1 + grp]; n_hi = tab[2 * p.f.groups + 1 + grp];
+        n0 += n_lo - n_lo % p.col_align;
+      }
+      if constexpr (FORM == kTcRaggedDepth) nothing = tab[p.f.groups + 1 + bt] == tab[2 * p.f.groups + 1 + bt];
       const uint32_t as = two_acc ? (acc_it & 1u) : 0u;
       const uint32_t aph = (two_acc ? (acc_it >> 1) : acc_it) & 1u;
       if (prefetch_c) {
@@ -838,7 +1015,7 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
         if (m0 < p.M) {
           const size_t es_c = p.dtype_c == TC_F32 ? 4 : 2;
           const char* c_line = static_cast<const char*>(p.C) + (static_cast<size_t>(m0) + static_cast<size_t>(bt) * p.c_batch) * es_c;
-          for (int c = lane + chunk_first; c < bn_tile && n0 + c < p.N; c += chunk_step) {
+          for (int c = lane + chunk_first; c < bn_tile && n0 + c < (FORM == kTcRaggedCols ? n_hi : p.N); c += chunk_step) {
 #pragma unroll
             for (int pl = 0; pl < PLANES; ++pl)
               prefetch_l2(c_line + (static_cast<size_t>(pl) * p.c_plane + static_cast<size_t>(n0 + c) * p.c_sn0) * es_c);
@@ -848,7 +1025,7 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + as * acc_cols;
       const bool m_ok = m < p.M;
       float bias_row = 0.0f;
-      if (p.bias_axis == TC_BIAS_ROW && m_ok) bias_row = p.bias[m];
+      if (p.bias_axis == TC_BIAS_ROW && m_ok) bias_row = p.bias[m + (FORM == kTcRaggedCols ? grp * p.f.bias_group : 0)];
       const int m_in = m % p.m_div, m_out = m / p.m_div;
       const int64_t d_row = m_in * p.d_sm0 + m_out * p.d_sm1 + bt * p.d_batch + split_off;
       const int64_t c_row = m_in * p.c_sm0 + m_out * p.c_sm1 + bt * p.c_batch;
@@ -876,6 +1053,27 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
 #pragma unroll
         for (int pl = 0; pl < PLANES; ++pl) tmem_ld_32x32(t_col + pl * p.bn, v[pl]);
         tmem_ld_wait();
+        if constexpr (FORM != kTcPlain) {
+          const int col0 = n0 + c;
+          const int j_lo = max(n_lo - col0, 0), j_hi = min(n_hi - col0, 32);
+          if (!m_ok || j_hi <= j_lo) continue;
+          if (nothing) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[0][j] = 0u;
+          }
+          const int64_t ci = c_row + static_cast<int64_t>(col0) * p.c_sn0, di = d_row + static_cast<int64_t>(col0) * p.d_sn0;
+          const int64_t zi = m + static_cast<int64_t>(col0) * p.f.z_sn;
+          const uint32_t live = (j_hi == 32 ? 0xffffffffu : (1u << j_hi) - 1u) & (0xffffffffu << j_lo);
+          auto store = [&](auto tag) {
+            using T = decltype(tag);
+            tc_fused_chunk<T>(p, v[0], static_cast<T*>(p.D) + di, static_cast<const T*>(p.C) + ci, static_cast<T*>(p.f.Z) + zi,
+                              bias_row, col0, live);
+          };
+          if (p.dtype_d == TC_F32) store(0.0f);
+          else if (p.dtype_d == TC_F16) store(__half());
+          else store(__nv_bfloat16());
+          continue;
+        }
         const int ncols = p.N - (n0 + c);  // columns of this chunk inside the matrix (may be <= 0)
         if (!m_ok || ncols <= 0) continue;
         const int n_in = (n0 + c) % p.n_div, n_out = (n0 + c) / p.n_div;  // a chunk never straddles n_div
@@ -997,6 +1195,40 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
     p.dbg_out[blockIdx.x * 16 + 13] = static_cast<long long>(t_entry);
     p.dbg_out[blockIdx.x * 16 + 14] = static_cast<long long>(global_timer_ns());
   }
+}
+
+// The tensor maps of kTcRaggedDepth: for every group that has columns, the maps of the whole A and B with the
+// extent of their strided index (the columns, the product's K) set to the group's end.  One warp per block; every
+// block reads all offsets (for the running maximum) and writes the maps of every gridDim.x-th group.
+struct TcDepthMapsParams {
+  CUtensorMap tm_a, tm_b;
+  FusedParams f;
+  CUtensorMap* maps;
+};
+
+static __global__ void __launch_bounds__(32) tc_depth_maps_kernel(const __grid_constant__ TcDepthMapsParams p) {
+  pdl_launch_dependents();
+  pdl_wait();     // the offsets may be the previous kernel's output; the map slots, what an earlier product still reads
+  const int lane = threadIdx.x;
+  int carry = fused_first_offset(p.f);
+  for (int base = 0; base < p.f.groups; base += 32) {
+    int lo, hi;
+    fused_group_chunk(p.f, base, lane, carry, lo, hi);
+    const int g = base + lane;
+    const unsigned live = __ballot_sync(0xffffffffu, g < p.f.groups && hi > lo);
+    for (unsigned rest = live; rest; rest &= rest - 1) {
+      const int src = __ffs(rest) - 1;
+      const int end = __shfl_sync(0xffffffffu, hi, src);
+      if ((base + src) % static_cast<int>(gridDim.x) != static_cast<int>(blockIdx.x)) continue;
+      CUtensorMap* out = p.maps + 2 * (base + src);
+      reinterpret_cast<uint32_t*>(out)[lane] = reinterpret_cast<const uint32_t*>(&p.tm_a)[lane];
+      reinterpret_cast<uint32_t*>(out + 1)[lane] = reinterpret_cast<const uint32_t*>(&p.tm_b)[lane];
+      __syncwarp();
+      if (lane < 2) tensormap_set_extent1(out + lane, static_cast<uint32_t>(end));
+      __syncwarp();
+    }
+  }
+  fence_tensormap_release();
 }
 
 }  // namespace gk

@@ -153,14 +153,15 @@ extern template const void* tc_kernel_select_r<false>(int cg, int planes, bool t
 extern template const void* tc_kernel_select_r<true>(int cg, int planes, bool tf32, bool dbg);
 
 const void* tc_kernel_generic(bool dbg);   // tc_kernels_generic.cu: <1, 1, false, false, GENERIC, dbg>
+const void* tc_kernel_fused(int form, int cg, bool generic);   // tc_kernels_fused.cu: the layer-level forms
 
 // dbg: the instance that honours the descriptor's diagnostic bits (the production instance compiles them out)
 static const void* tc_kernel_select(int cg, int planes, bool tf32, bool rank5, bool dbg) {
   return rank5 ? tc_kernel_select_r<true>(cg, planes, tf32, dbg) : tc_kernel_select_r<false>(cg, planes, tf32, dbg);
 }
 
-static constexpr int kSmemBudget = 232448;  // 227 KiB opt-in limit per CTA on sm_100
-static constexpr int kCtrlBytes = 256;
+static constexpr int kSmemMax = 232448;  // 227 KiB opt-in limit per CTA on sm_100
+static constexpr int kCtrlBytes = kTcCtrlBytes;
 static constexpr double kWideEff = 1.08;   // measured gain of the single-stage 512-column tiles on large products
 
 static int stage_bytes_for(int cg, int bn, int n_sub, int a_planes, int b_planes) {
@@ -181,6 +182,14 @@ static bool box_fits(int64_t ext0, int64_t ext1, int total) {
 // fill all 512 TMEM columns (n_sub * planes * bn == 512) run with one accumulator stage: their
 // epilogue is not overlapped, which the efficiency figure accounts for; they pay off on large
 // problems, where the main loop is limited by the operand feed from L2 rather than by the MMAs.
+// Column tiles of width bn that ragged columns are expected to make: the groups' sizes are known on the device
+// only, so each of the groups that can have columns is given the average and half a tile for its ragged end.
+static double ragged_tiles(const TcProblem& pr, int bn) {
+  const double active = static_cast<double>(std::max<int64_t>(1, std::min<int64_t>(pr.f.groups, pr.N)));
+  const double avg = pr.N / active;
+  return active * std::max(1.0, avg / bn + (pr.f.groups > 1 ? 0.5 : 0.0));
+}
+
 static void choose_tile(const TcProblem& pr, int sm_count, int planes, int* cg_out, int* bn_out, int* nsub_out) {
   // an N-contiguous B is loaded in boxes of 128 bytes of N per CTA
   int n_unit = pr.B.mn_major ? kTcKBytes / dtype_size(pr.B.dtype) : 8;
@@ -192,7 +201,7 @@ static void choose_tile(const TcProblem& pr, int sm_count, int planes, int* cg_o
   int bcg = 1, bbn = 128, bns = 1;
   for (const Cand& c : cands) {
     if (c.n_sub * planes * c.bn > 512) continue;  // accumulators of one tile must fit 512 TMEM columns
-    if (c.n_sub > 1 && pr.rank5) continue;
+    if (c.n_sub > 1 && (pr.rank5 || pr.form >= kTcRaggedCols)) continue;
     if (pr.generic && (c.cg != 1 || c.n_sub != 1)) continue;
     if ((c.bn / c.cg) % n_unit) continue;
     if (pr.cta_group && c.cg != pr.cta_group) continue;
@@ -203,7 +212,10 @@ static void choose_tile(const TcProblem& pr, int sm_count, int planes, int* cg_o
     const int64_t tm = (pr.M + 128 * c.cg - 1) / (128 * c.cg);
     const int64_t tn = (pr.N + c.bn * c.n_sub - 1) / (c.bn * c.n_sub);
     const int64_t slots = std::max(1, sm_count / c.cg);
-    const int64_t waves = (tm * tn * std::max(1, pr.batch) + slots - 1) / slots;
+    int64_t units = tm * tn * std::max(1, pr.batch);
+    if (pr.form == kTcRaggedCols) units = static_cast<int64_t>(std::ceil(tm * ragged_tiles(pr, c.bn)));
+    else if (pr.form == kTcRaggedDepth) units = tm * tn * pr.f.groups;
+    const int64_t waves = (units + slots - 1) / slots;
     // a single accumulator stage exposes the epilogue: worth it only when the main loop is long
     double eff = c.eff;
     if (planes == 2) {
@@ -215,7 +227,7 @@ static void choose_tile(const TcProblem& pr, int sm_count, int planes, int* cg_o
     } else if (c.n_sub * planes * c.bn > 256) {
       // an epilogue that also reads C (or writes through the general path) is several times
       // longer; exposed, it eats the gain
-      const bool light = !pr.has_c;
+      const bool light = !pr.has_c && pr.form == kTcPlain;
       eff = pr.K >= 1024 ? (light ? kWideEff : 0.85) : 0.5;
     }
     const double t = static_cast<double>(waves) * c.bn * c.n_sub / eff;
@@ -239,7 +251,7 @@ static const gk_tuning_entry kBuiltinTuning[] = {
 
 // Nearest measured entry for this problem (see gk_tuning_entry), or nullptr.
 static const gk_tuning_entry* tuning_lookup(gk_handle h, const TcProblem& pr, gk_tuning_entry* copy) {
-  if (pr.rank5 || pr.generic || pr.number != GK_REAL || pr.batch > 1 || pr.k_split > 1) return nullptr;
+  if (pr.rank5 || pr.generic || pr.number != GK_REAL || pr.batch > 1 || pr.k_split > 1 || pr.form != kTcPlain) return nullptr;
   const int has_c = pr.has_c ? 1 : 0;
   const int ta = pr.A.mn_major ? 0 : 1, tb = pr.B.mn_major ? 1 : 0;
   double best = 1e30;
@@ -357,6 +369,15 @@ gk_status tc_plan(gk_handle h, const TcProblem& pr_in, bool encode, TcLaunch* ou
     p.batch = pr.batch;
     p.a_batched = pr.batch_a > 0 ? 1 : 0; p.b_batched = pr.batch_b > 0 ? 1 : 0;
     p.c_batch = pr.batch_c; p.d_batch = pr.batch_d;
+  }
+  if (pr.form != kTcPlain) {
+    if (planes != 1 || pr.rank5 || tf32 || pr.batch > 1 || pr.k_split > 1 || pr.debug != 0 || (pr.form >= kTcRaggedCols && n_sub != 1))
+      return set_error(GK_ERR_INVALID_CONFIG, "fused and ragged products are real products of 16-bit operands with tile_n <= 256 "
+                       "when ragged, without diagnostic bits");
+    p.f = pr.f;
+    p.a_batched = pr.form == kTcRaggedCols && pr.batch_a > 0 && pr.f.groups > 1 ? 1 : 0;
+    p.c_batch = pr.batch_c; p.d_batch = pr.batch_d;
+    p.col_align = pr.form == kTcRaggedCols && pr.B.mn_major && !pr.generic ? 8 : 1;
   }
   p.tiles_m = (p.M + kTcTileM * cg - 1) / (kTcTileM * cg);
   p.tiles_n = (p.N + bn * n_sub - 1) / (bn * n_sub);
@@ -498,6 +519,8 @@ gk_status tc_plan(gk_handle h, const TcProblem& pr_in, bool encode, TcLaunch* ou
   // since that loop became straight-line code the deeper ring of single k-blocks is 1-2 % ahead again
   // (2048^3: 17.2 against 17.5 us, 8192 x 4096 x 8192: 369 against 375 us), and a 256 x 512 tile's MMAs
   // outlast the fixed cost by far.
+  const int table_bytes = pr.form >= kTcRaggedCols ? tc_table_bytes(pr.f.groups) : 0;
+  const int kSmemBudget = kSmemMax - table_bytes;
   const int kblock_bytes = stage_bytes_for(cg, bn, n_sub, planes, planes);
   const int boxes_per_kblock = planes * (p.a_boxes * p.a_sub + n_sub * p.b_boxes * p.b_sub);   // one lane each in a producer warp
   const int mma_cycles_per_kblock = 2 * bn * n_sub * p.n_terms;
@@ -517,7 +540,7 @@ gk_status tc_plan(gk_handle h, const TcProblem& pr_in, bool encode, TcLaunch* ou
   p.stages = stages;
   // Skewed schedule of 512-column tiles (tc_gemm.cuh): every work unit must hold at least two rings of k-blocks.
   p.skew = (n_sub == 2 && acc_stages == 1 && planes == 1 && kps == 1 && !pr.generic && pr.k_split <= 1 &&
-            p.k_blocks >= 2 * stages && !(pr.debug & 32)) ? 1 : 0;
+            pr.form <= kTcFused && p.k_blocks >= 2 * stages && !(pr.debug & 32)) ? 1 : 0;
   uint32_t cols = 32;
   while (cols < static_cast<uint32_t>(acc_stages * n_sub * planes * bn)) cols <<= 1;
   p.tmem_cols = cols;
@@ -558,7 +581,7 @@ gk_status tc_plan(gk_handle h, const TcProblem& pr_in, bool encode, TcLaunch* ou
       if (!pr.epi->bias && encode) return set_error(GK_ERR_INVALID_ARGUMENT, "bias axis set but bias pointer is NULL");
       p.bias = pr.epi->bias; p.bias_axis = pr.epi->bias_axis;
     }
-    if (pr.epi->activation < GK_ACT_NONE || pr.epi->activation > GK_ACT_GELU)
+    if (pr.epi->activation < GK_ACT_NONE || pr.epi->activation > (pr.form == kTcPlain ? GK_ACT_GELU : GK_ACT_SILU))
       return set_error(GK_ERR_UNSUPPORTED, "activation %d is not one of none/ReLU/GELU", pr.epi->activation);
     p.act = pr.epi->activation;
   }
@@ -571,14 +594,17 @@ gk_status tc_plan(gk_handle h, const TcProblem& pr_in, bool encode, TcLaunch* ou
   out->tf32 = tf32;
   out->rank5 = pr.rank5;
   out->generic = pr.generic;
-  out->smem_bytes = stages * stage_bytes + kCtrlBytes + 1024;
+  out->form = pr.form;
+  out->smem_bytes = stages * stage_bytes + kCtrlBytes + table_bytes + 1024;
   // One CTA of this kernel per SM, whatever the stage count: a CTA allocates up to all 512 TMEM columns
   // without a bound on that wait, and with dependent launch the next kernel's CTAs arrive while this one's
   // are still draining.  Asking for more than half of an SM's shared memory makes two tcgen05 CTAs on one
   // SM impossible, so two CTA pairs can never each hold one SM's tensor memory and wait for the other's.
-  out->smem_bytes = std::max(out->smem_bytes, kSmemBudget / 2 + 2048);
+  out->smem_bytes = std::max(out->smem_bytes, kSmemMax / 2 + 2048);
   const bool dbg = pr.debug != 0;
-  out->kernel = pr.generic ? tc_kernel_generic(dbg) : tc_kernel_select(cg, planes, tf32, pr.rank5, dbg);
+  out->kernel = pr.form != kTcPlain ? tc_kernel_fused(pr.form, cg, pr.generic)
+                : pr.generic        ? tc_kernel_generic(dbg)
+                                    : tc_kernel_select(cg, planes, tf32, pr.rank5, dbg);
   if (pr.generic) {
     p.ga = pr.A.ptr; p.gb = pr.B.ptr;
     p.g_lda = pr.A.mn_major ? pr.A.k_str[0] : pr.A.mn_str[0];
@@ -587,16 +613,20 @@ gk_status tc_plan(gk_handle h, const TcProblem& pr_in, bool encode, TcLaunch* ou
   }
 
   // persistent grid
-  const int64_t tiles64 = static_cast<int64_t>(p.tiles_m) * p.tiles_n * p.k_split * p.batch;
+  int64_t tiles64 = static_cast<int64_t>(p.tiles_m) * p.tiles_n * p.k_split * p.batch;
+  if (pr.form == kTcRaggedDepth) tiles64 *= pr.f.groups;
+  if (pr.form == kTcRaggedCols)   // at most: every group with columns ends in a partial tile, and may begin in one
+    tiles64 = p.tiles_m * (pr.N / bn + (p.col_align > 1 ? 2 : 1) * std::min<int64_t>(pr.f.groups, pr.N));
   if (tiles64 > INT32_MAX) return set_error(GK_ERR_INVALID_CONFIG, "too many work units (%lld)", (long long)tiles64);
   const int tiles = static_cast<int>(tiles64);
   int slots;
   {
     std::lock_guard<std::mutex> lock(h->mu);
-    bool& set = pr.generic ? h->attr_set_generic[dbg ? 1 : 0]
+    bool& set = pr.form != kTcPlain ? h->attr_set_fused[pr.form - 1][pr.generic ? 2 : cg - 1]
+                : pr.generic        ? h->attr_set_generic[dbg ? 1 : 0]
                            : h->attr_set[dbg ? 1 : 0][cg - 1][planes - 1][(tf32 ? 1 : 0) + (pr.rank5 ? 2 : 0)];
     if (!set) {
-      GK_CUDA_CHECK(cudaFuncSetAttribute(out->kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBudget));
+      GK_CUDA_CHECK(cudaFuncSetAttribute(out->kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax));
       set = true;
     }
     if (cg == 1) {
@@ -607,7 +637,7 @@ gk_status tc_plan(gk_handle h, const TcProblem& pr_in, bool encode, TcLaunch* ou
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3(2 * (h->sm_count / 2));
         cfg.blockDim = dim3(tc_threads(planes));
-        cfg.dynamicSmemBytes = kSmemBudget;
+        cfg.dynamicSmemBytes = kSmemMax;
         cudaLaunchAttribute at{};
         at.id = cudaLaunchAttributeClusterDimension;
         at.val.clusterDim.x = 2; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
@@ -623,7 +653,7 @@ gk_status tc_plan(gk_handle h, const TcProblem& pr_in, bool encode, TcLaunch* ou
   if (pr.max_ctas > 0) slots = std::max(1, std::min(slots, pr.max_ctas / cg));
   out->grid = cg * std::min(tiles, slots);
 
-  if (encode && !pr.generic) {
+  if (encode && !pr.generic && !(pr.form != kTcPlain && p.k_blocks == 0)) {   // (nothing to multiply: nothing is loaded)
     gk_status s;
     if (pr.rank5) {
       s = encode_modes(h, &p.tm_a, pr.A, planes, a_box, a_tma);
@@ -631,7 +661,7 @@ gk_status tc_plan(gk_handle h, const TcProblem& pr_in, bool encode, TcLaunch* ou
       s = encode_modes(h, &p.tm_b, pr.B, planes, b_box, b_tma);
     } else {
       s = encode_plain(h, &p.tm_a, pr.A, planes, p.a_mn_major ? p.a_box_mn : p.bk, p.a_mn_major ? p.bk : kTcTileM, a_tma,
-                       pr.batch, pr.batch_a);
+                       pr.form == kTcRaggedCols ? pr.f.groups : pr.batch, pr.batch_a);
       if (s != GK_OK) return s;
       s = encode_plain(h, &p.tm_b, pr.B, planes, p.b_mn_major ? p.b_box_mn : p.bk, p.b_mn_major ? p.bk : bn_cta, b_tma,
                        pr.batch, pr.batch_b);
@@ -651,6 +681,20 @@ int tc_choose_k_split(const TcProblem& pr, const TcLaunch& L, int sm_count) {
   const int s = std::min({64, slots / tiles, p.k_blocks / 8});
   (void)pr;
   return s >= 2 ? s : 1;
+}
+
+int64_t tc_depth_maps_bytes(const TcLaunch& L) {
+  if (L.form != kTcRaggedDepth || L.generic || L.params.k_blocks == 0) return 0;
+  return static_cast<int64_t>(L.params.f.groups) * 2 * sizeof(CUtensorMap);
+}
+
+gk_status tc_write_depth_maps(TcLaunch* L, void* workspace, cudaStream_t stream) {
+  TcDepthMapsParams q{};
+  q.tm_a = L->params.tm_a; q.tm_b = L->params.tm_b; q.f = L->params.f;
+  q.maps = static_cast<CUtensorMap*>(workspace);
+  L->params.maps = q.maps;
+  GK_CUDA_CHECK(launch_dependent(tc_depth_maps_kernel, dim3(std::min(q.f.groups, 32)), dim3(32), 0, stream, q));
+  return GK_OK;
 }
 
 gk_status tc_launch(const TcLaunch& L, cudaStream_t stream) {
@@ -732,7 +776,7 @@ gk_status tc_run(gk_handle h, const TcProblem& pr_in, const TcLaunch& L, void* w
   ps.c_sm[0] = 1; ps.c_sm[1] = 0; ps.d_sm[0] = 1; ps.d_sm[1] = 0;
   ps.c_sn[0] = pr.M; ps.c_sn[1] = 0; ps.d_sn[0] = pr.M; ps.d_sn[1] = 0;
   ps.c_plane = ps.d_plane = pr.M * pr.N;
-  ps.alpha = 1.0; ps.beta = 0.0; ps.epi = nullptr;
+  ps.alpha = 1.0; ps.beta = 0.0; ps.epi = nullptr; ps.form = kTcPlain; ps.f = FusedParams{};
   if (pr.tile_n == 0) { ps.tile_n = L.params.bn * L.params.n_sub; ps.cta_group = L.cg; }   // same tile as planned
   ps.k_split = splits; ps.split_stride = set_bytes / 4;
   TcLaunch Ls;
@@ -749,6 +793,7 @@ gk_status tc_run(gk_handle h, const TcProblem& pr_in, const TcLaunch& L, void* w
   r.m_div = clamp_div(pr.m_ext0, pr.m_ext0 < pr.M ? 2 : 1); r.n_div = clamp_div(pr.n_ext0, pr.n_ext0 < pr.N ? 2 : 1);
   r.c_sm0 = pr.c_sm[0]; r.c_sm1 = pr.c_sm[1]; r.c_sn0 = pr.c_sn[0]; r.c_sn1 = pr.c_sn[1]; r.c_plane = pr.c_plane;
   r.d_sm0 = pr.d_sm[0]; r.d_sm1 = pr.d_sm[1]; r.d_sn0 = pr.d_sn[0]; r.d_sn1 = pr.d_sn[1]; r.d_plane = pr.d_plane;
+  r.fused = pr.form == kTcFused ? 1 : 0; r.f = pr.f;
   if (pr.epi) { r.bias = pr.epi->bias; r.bias_axis = pr.epi->bias_axis; r.act = pr.epi->activation; }
   const bool plain = L.planes == 1 && pr.m_ext0 >= pr.M && pr.n_ext0 >= pr.N && pr.d_sm[0] == 1 && (pr.C == nullptr || pr.c_sm[0] == 1);
   const bool vec = plain && pr.M % 4 == 0;

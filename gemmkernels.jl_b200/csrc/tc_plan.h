@@ -44,6 +44,10 @@ struct TcProblem {
   // strided-batched real products (plain matrices only): operand strides in elements, 0 = shared
   int32_t batch = 1;
   int64_t batch_a = 0, batch_b = 0, batch_c = 0, batch_d = 0;
+  // layer-level forms (tc_gemm.cuh): fused epilogue, ragged columns (N = all columns there are, batch_a = elements
+  // between the groups' A), ragged depth (K = all columns there are, batch_c / batch_d = elements between the groups)
+  int form = kTcPlain;
+  FusedParams f{};
 };
 
 // How many runs to cut K into for this problem on this GPU: 1 unless the tiles fill less than half of the
@@ -56,6 +60,7 @@ struct TcLaunch {
   const void* kernel = nullptr;
   int cg = 1, planes = 1;
   bool tf32 = false, rank5 = false, generic = false;
+  int form = kTcPlain;
   int grid = 0;
   int smem_bytes = 0;
 };
@@ -71,6 +76,10 @@ void tc_problem_from_gemm(const gk_gemm_desc& d, const gk_epilogue_desc* epi, co
 // Tile choice, descriptors, grid, epilogue and (when `encode`) the TMA tensor maps.
 gk_status tc_plan(gk_handle h, const TcProblem& pr, bool encode, TcLaunch* out);
 gk_status tc_launch(const TcLaunch& L, cudaStream_t stream);
+// kTcRaggedDepth: bytes of 256-byte aligned workspace for the groups' tensor maps (0: the plan needs none), and the
+// launch that writes them before tc_launch; sets L's map pointer.
+int64_t tc_depth_maps_bytes(const TcLaunch& L);
+gk_status tc_write_depth_maps(TcLaunch* L, void* workspace, cudaStream_t stream);
 // Runs the planned product `L` of `pr`.  Given a 256-byte aligned workspace, a product with few output
 // tiles and a long K is cut into K-runs over the otherwise idle SMs: FP32 partial sums go to the
 // workspace (as many runs as it holds) and a reduction pass applies alpha, beta, bias and activation

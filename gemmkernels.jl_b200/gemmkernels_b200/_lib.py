@@ -20,7 +20,10 @@ GK_F16, GK_BF16, GK_F32, GK_F64, GK_I16, GK_I32, GK_I64, GK_TF32 = range(8)
 GK_OP_AUTO, GK_OP_TCGEN05, GK_OP_FPU, GK_OP_FPU_TROPICAL = range(4)
 GK_REAL, GK_COMPLEX, GK_DUAL = range(3)
 GK_LAYOUT_DENSE, GK_LAYOUT_ZERO, GK_LAYOUT_DIAGONAL = range(3)
-GK_ACT_NONE, GK_ACT_RELU, GK_ACT_GELU = range(3)
+GK_ACT_NONE, GK_ACT_RELU, GK_ACT_GELU, GK_ACT_SILU = range(4)
+GK_FUSED_STANDARD, GK_FUSED_RESIDUAL, GK_FUSED_GRADIENT = range(3)
+GK_RAGGED_COLUMNS, GK_RAGGED_DEPTH = 1, 2
+GK_MAX_GROUPS = 1024
 GK_BIAS_NONE, GK_BIAS_ROW, GK_BIAS_COL = range(3)
 GK_RASTER_AUTO, GK_RASTER_IDENTITY, GK_RASTER_HORIZONTAL, GK_RASTER_VERTICAL, GK_RASTER_LEBESGUE = range(5)
 
@@ -30,6 +33,7 @@ EXPORTS = (
     "gk_contract_static",
     "gk_mgpu_unique_id", "gk_mgpu_init", "gk_mgpu_destroy", "gk_mgpu_gemm_colshard", "gk_mgpu_gemm_colshard_host",
     "gk_mgpu_host_plan", "gk_mgpu_broadcast", "gk_load_tuning",
+    "gk_gemm_fused", "gk_gemm_fused_query", "gk_activation_gradient", "gk_activation_gradient_query",
 )
 GK_MGPU_UNIQUE_ID_BYTES = 128
 GK_MGPU_A_RESIDENT, GK_MGPU_A_BROADCAST = 0, 1
@@ -72,6 +76,42 @@ class EpilogueDesc(C.Structure):
     def __init__(self, **kw):
         super().__init__(**kw)
         self.struct_size = C.sizeof(EpilogueDesc)
+
+
+class FusedDesc(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("form", C.c_int32), ("bias_axis", C.c_int32), ("activation", C.c_int32),
+        ("bias", C.c_void_p), ("z", C.c_void_p), ("ldz", C.c_int64), ("reserved", C.c_int32 * 2),
+    ]
+
+    def __init__(self, **kw):
+        super().__init__(**kw)
+        self.struct_size = C.sizeof(FusedDesc)
+
+
+class GroupDesc(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("ragged", C.c_int32), ("groups", C.c_int32), ("offsets_dtype", C.c_int32),
+        ("offsets", C.c_void_p), ("stride_a", C.c_int64), ("stride_bias", C.c_int64), ("stride_c", C.c_int64),
+        ("stride_d", C.c_int64),
+    ]
+
+    def __init__(self, **kw):
+        super().__init__(**kw)
+        self.struct_size = C.sizeof(GroupDesc)
+
+
+class ActivationGradientDesc(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("dtype", C.c_int32), ("m", C.c_int64), ("n", C.c_int64),
+        ("ld_dd", C.c_int64), ("ld_z", C.c_int64), ("ld_dz", C.c_int64), ("ld_db", C.c_int64),
+        ("activation", C.c_int32), ("groups", C.c_int32), ("offsets_dtype", C.c_int32), ("reserved", C.c_int32),
+        ("offsets", C.c_void_p),
+    ]
+
+    def __init__(self, **kw):
+        super().__init__(**kw)
+        self.struct_size = C.sizeof(ActivationGradientDesc)
 
 
 class GemmPlan(C.Structure):
@@ -174,6 +214,17 @@ def _load() -> C.CDLL:
     lib.gk_mgpu_broadcast.argtypes = [C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p]
     lib.gk_mgpu_host_plan.restype = C.c_int
     lib.gk_mgpu_host_plan.argtypes = [C.POINTER(GemmDesc), C.c_int32, C.POINTER(C.c_int32), C.POINTER(C.c_int64)]
+    lib.gk_gemm_fused_query.restype = C.c_int
+    lib.gk_gemm_fused_query.argtypes = [C.c_void_p, C.POINTER(GemmDesc), C.POINTER(FusedDesc), C.POINTER(GroupDesc),
+                                        C.POINTER(GemmPlan)]
+    lib.gk_gemm_fused.restype = C.c_int
+    lib.gk_gemm_fused.argtypes = [C.c_void_p, C.POINTER(GemmDesc), C.POINTER(FusedDesc), C.POINTER(GroupDesc),
+                                  C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]
+    lib.gk_activation_gradient_query.restype = C.c_int
+    lib.gk_activation_gradient_query.argtypes = [C.c_void_p, C.POINTER(ActivationGradientDesc), C.POINTER(C.c_int64)]
+    lib.gk_activation_gradient.restype = C.c_int
+    lib.gk_activation_gradient.argtypes = [C.c_void_p, C.POINTER(ActivationGradientDesc), C.c_void_p, C.c_void_p,
+                                           C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]
     return lib
 
 

@@ -317,7 +317,8 @@ def matmul(conf: Config, a, b, c, d, *,
            epilogue=None, kernel=Kernel.matmul_singlestage, stream=None, workspace=None):
     """GemmKernels.matmul(conf, a, b, c, d; ...) (src/matmul.jl:7-44): D = epilogue(A*B + C),
     enqueued asynchronously on the current CUDA stream.  Raises ConfigError for combinations the
-    engine cannot run (the reference's tests count that as "skipped")."""
+    engine cannot run (the reference's tests count that as "skipped").  With one of the fused epilogues
+    (Epilogue.BiasActivationResidual, Epilogue.ActivationGradient) D is what that epilogue says."""
     import torch
     hooks = {
         "global_to_shared_a": transform_global_to_shared_a, "global_to_shared_b": transform_global_to_shared_b,
@@ -325,6 +326,9 @@ def matmul(conf: Config, a, b, c, d, *,
         "shared_to_regs_a": transform_shared_to_regs_a, "shared_to_regs_b": transform_shared_to_regs_b,
         "shared_to_regs_c": transform_shared_to_regs_c, "regs_to_shared_d": transform_regs_to_shared_d,
     }
+    if isinstance(epilogue, Epilogue.Fused):
+        from .fused import _run, lower_fused
+        return _run(lower_fused(conf, a, b, c, d, hooks, epilogue, kernel), stream, workspace)
     desc, epi, (pa, pb, pc, pd) = lower(conf, a, b, c, d, hooks, epilogue or Epilogue.Default(), kernel)
     dev = d.device.index if d.device.index is not None else torch.cuda.current_device()
     s = stream if stream is not None else torch.cuda.current_stream(dev).cuda_stream
@@ -418,6 +422,9 @@ class BoundMatmul:
 def bind(conf: Config, a, b, c, d, *, epilogue=None, kernel=Kernel.matmul_singlestage, workspace=None, **transforms):
     """Lower `matmul(conf, a, b, c, d; ...)` once and return a callable that enqueues it."""
     hooks = {k.replace("transform_", ""): v for k, v in transforms.items()}
+    if isinstance(epilogue, Epilogue.Fused):
+        from .fused import BoundFused, lower_fused
+        return BoundFused(lower_fused(conf, a, b, c, d, hooks, epilogue, kernel), workspace)
     return BoundMatmul(conf, a, b, c, d, hooks, epilogue or Epilogue.Default(), kernel, workspace)
 
 
@@ -449,6 +456,10 @@ def query(conf: Config, a, b, c, d, *, epilogue=None, kernel=Kernel.matmul_singl
     limits (src/matmul.jl:24-41)."""
     import torch
     hooks = {k.replace("transform_", ""): v for k, v in hooks.items()}
+    if isinstance(epilogue, Epilogue.Fused):
+        from .fused import lower_fused
+        call = lower_fused(conf, a, b, c, d, hooks, epilogue, kernel)
+        return call.query(handle(call.device.index))
     desc, epi, _ = lower(conf, a, b, c, d, hooks, epilogue or Epilogue.Default(), kernel)
     plan = L.GemmPlan()
     st = L.lib.gk_gemm_query(handle(), C.byref(desc), C.byref(epi), C.byref(plan))

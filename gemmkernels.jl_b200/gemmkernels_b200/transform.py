@@ -40,6 +40,14 @@ class GELU(Functor):
         return "GELU()"
 
 
+class SiLU(Functor):
+    """x -> x * sigmoid(x).  The layer-level epilogues take it (Epilogue.BiasActivationResidual,
+    Epilogue.ActivationGradient, activation_gradient_); it is no transform hook of a plain `matmul`."""
+
+    def __repr__(self):
+        return "SiLU()"
+
+
 class Cast(Functor):
     """Convert to the element type of D; the store already does this, so it folds to nothing."""
 

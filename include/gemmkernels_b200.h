@@ -74,7 +74,12 @@ typedef enum gk_number { GK_REAL = 0, GK_COMPLEX = 1, GK_DUAL = 2 } gk_number;
  * (layout.jl:225-236): A is a length-M vector holding the diagonal of a square matrix. */
 typedef enum gk_layout_kind { GK_LAYOUT_DENSE = 0, GK_LAYOUT_ZERO = 1, GK_LAYOUT_DIAGONAL = 2 } gk_layout_kind;
 
-typedef enum gk_activation { GK_ACT_NONE = 0, GK_ACT_RELU = 1, GK_ACT_GELU = 2 } gk_activation;
+typedef enum gk_activation {
+  GK_ACT_NONE = 0,
+  GK_ACT_RELU = 1,
+  GK_ACT_GELU = 2,
+  GK_ACT_SILU = 3 /* gk_gemm_fused and gk_activation_gradient only */
+} gk_activation;
 
 /* Bias axis.  COL is the reference's Epilogue.Bias (epilogue.jl:44-52: one value per column of D,
  * length N); ROW is one value per row of D (length M). */
@@ -313,6 +318,98 @@ GK_API gk_status gk_gemm_host(gk_handle h, const gk_gemm_desc* desc, const void*
                               const void* b_host, const void* c_host, void* d_host,
                               const gk_epilogue_desc* epi, gk_stream stream);
 
+
+/*
+ * Layer-level products: what a dense or expert layer of a network needs around its matrix product, in
+ * one launch.  No counterpart in the reference.  With op, alpha, beta, C and D as in gk_gemm:
+ *
+ *   x = alpha * op(A) * op(B) + bias                        [+ beta * C in the STANDARD and GRADIENT forms]
+ *   GK_FUSED_STANDARD   D = act(x)                          Z = x is kept when z is not NULL
+ *   GK_FUSED_RESIDUAL   D = act(x) + beta * C               Z = x is kept when z is not NULL
+ *   GK_FUSED_GRADIENT   D = x * act'(Z)                     Z is read; no bias
+ *
+ * GELU is the erf form, ReLU'(0) = 0.  Operands are Float16 or BFloat16 (compute of the same type, op AUTO
+ * or TCGEN05), D is Float16, BFloat16 or Float32, C and Z have D's type.  All of x is FP32; act sees the
+ * unrounded x, Z and D are rounded when they are stored.  D may alias C (any form) and, in the GRADIENT
+ * form, Z; Z that is kept must not share memory with C or D.
+ *
+ * With a gk_group_desc the product is ragged: one of its indices is cut into `groups` runs whose
+ * boundaries are an array on the DEVICE, offsets[0] .. offsets[groups], read by the kernel (so they may be
+ * the output of earlier work on the stream).  Group g owns offsets[g] .. offsets[g + 1] - 1.  The values are
+ * clamped to [0, extent] and made non-decreasing by a running maximum, so no content of the array leads
+ * outside the matrices.
+ *   GK_RAGGED_COLUMNS   D[:, J_g] = epilogue(op(A_g) * op(B)[:, J_g] ...): the columns (n = all there are).
+ *                       A_g = a + g * stride_a (0 shares A), bias + g * stride_bias, per row.  C and Z are
+ *                       M x N like D.  Columns of D and Z outside every group are left as they were.
+ *   GK_RAGGED_DEPTH     D_g = alpha * op(A)[:, J_g] * op(B)[J_g, :] + beta * C_g: the contracted index (k = all
+ *                       there is), e.g. the weight gradient of expert g.  D_g = d + g * stride_d, C_g = c +
+ *                       g * stride_c.  STANDARD form without bias, activation and Z.  A group without columns
+ *                       gives beta * C_g.  Nothing outside a group's run is read into its product.
+ *                       Fast for trans_a = 0, trans_b = 1 (K strided in both operands).
+ */
+typedef enum gk_fused_form { GK_FUSED_STANDARD = 0, GK_FUSED_RESIDUAL = 1, GK_FUSED_GRADIENT = 2 } gk_fused_form;
+
+typedef struct gk_fused_desc {
+  uint32_t struct_size;
+  int32_t form;        /* gk_fused_form */
+  int32_t bias_axis;   /* gk_bias_axis; ROW or NONE when the columns are ragged */
+  int32_t activation;  /* gk_activation */
+  const float* bias;   /* device, FP32 */
+  void* z;             /* device, M x N of D's type, see above; NULL: none */
+  int64_t ldz;
+  int32_t reserved[2];
+} gk_fused_desc;
+
+typedef enum gk_ragged { GK_RAGGED_COLUMNS = 1, GK_RAGGED_DEPTH = 2 } gk_ragged;
+
+#define GK_MAX_GROUPS 1024
+
+typedef struct gk_group_desc {
+  uint32_t struct_size;
+  int32_t ragged;         /* gk_ragged */
+  int32_t groups;         /* 1 .. GK_MAX_GROUPS */
+  int32_t offsets_dtype;  /* GK_I32 or GK_I64 */
+  const void* offsets;    /* device, groups + 1 values */
+  int64_t stride_a, stride_bias;    /* elements; COLUMNS */
+  int64_t stride_c, stride_d;       /* elements; DEPTH */
+} gk_group_desc;
+
+/* What gk_gemm_fused would launch (plan.kernel 1 = tensor cores, 6 = the streaming kernel for a few columns)
+ * and the workspace it can use: REQUIRED for a ragged depth (the groups' tensor maps, 256-byte aligned),
+ * optional for a plain fused product with few output tiles and a long K, none otherwise. */
+GK_API gk_status gk_gemm_fused_query(gk_handle h, const gk_gemm_desc* desc, const gk_fused_desc* fused,
+                                     const gk_group_desc* groups, gk_gemm_plan* plan);
+
+/* Enqueues the product on `stream`.  groups may be NULL (one plain product); c may be NULL when beta == 0.
+ * A workspace belongs to one call at a time: calls that can overlap on the GPU need one each. */
+GK_API gk_status gk_gemm_fused(gk_handle h, const gk_gemm_desc* desc, const gk_fused_desc* fused,
+                               const gk_group_desc* groups, const void* a, const void* b, const void* c,
+                               void* d, void* workspace, int64_t workspace_bytes, gk_stream stream);
+
+/*
+ * The backward pass of an activation behind a bias: dZ = dD * act'(Z), and the bias gradient
+ * db[:, g] = the sum of dZ over the columns of group g (FP32, of the unrounded dZ, in a fixed order).  All
+ * matrices are M x N, column-major, of one element type (Float16, BFloat16 or Float32); dZ may alias dD or Z.
+ * dz may be NULL (only the sums are wanted), db may be NULL (no sums), z may be NULL for GK_ACT_NONE.
+ * offsets as in gk_group_desc; NULL: one group of all columns.  Columns outside every group are not read and
+ * their dZ is left as it was; a group without columns has a bias gradient of zero.
+ */
+typedef struct gk_activation_gradient_desc {
+  uint32_t struct_size;
+  int32_t dtype;          /* gk_dtype of dD, Z and dZ */
+  int64_t m, n;
+  int64_t ld_dd, ld_z, ld_dz, ld_db;
+  int32_t activation;     /* gk_activation */
+  int32_t groups, offsets_dtype, reserved;
+  const void* offsets;    /* device */
+} gk_activation_gradient_desc;
+
+/* Bytes of workspace (partial sums) gk_activation_gradient needs when db is not NULL. */
+GK_API gk_status gk_activation_gradient_query(gk_handle h, const gk_activation_gradient_desc* desc, int64_t* workspace_bytes);
+
+GK_API gk_status gk_activation_gradient(gk_handle h, const gk_activation_gradient_desc* desc, const void* dd,
+                                        const void* z, void* dz, float* db, void* workspace,
+                                        int64_t workspace_bytes, gk_stream stream);
 
 /*
  * Column-sharded GEMM over the GPUs of one box: D[:, J_r] = A * B[:, J_r], rank r owns the column
