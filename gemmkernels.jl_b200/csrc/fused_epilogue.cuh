@@ -30,6 +30,8 @@ struct FusedParams {
   int32_t groups;
   int32_t total;           // columns there are: offsets are clamped to [0, total]
   int64_t bias_group;      // elements between the biases of consecutive groups
+  int32_t wide;            // tensor-core kernel: D, C and Z are 16-bit, M and all leading dimensions are multiples of 8
+                           // and the addresses of 16 bytes: the epilogue moves 8 rows of a column per access
 };
 
 // FAST: the result is stored in 16 bits, whose half step (2^-12 relative at best) is far above the 2^-21 of
@@ -40,11 +42,33 @@ __device__ __forceinline__ float fused_sigmoid(float x) {
   return 1.0f / (1.0f + expf(-x));
 }
 
+// Phi(x), the normal distribution, and e = exp(-x^2 / 2), for results of 16 bits: the rational approximation of
+// the error function by Hastings (Abramowitz and Stegun, 7.1.26; absolute error 1.5e-7) with its exponential at
+// x / sqrt(2) - the one that GELU' needs as well.  The smaller tail is computed, so it keeps its relative accuracy.
+__device__ __forceinline__ float fused_normal(float x, float& e) {
+  const float a = fabsf(x);
+  e = exp2f(-0.72134752044448170f * x * x);                      // log2(e) / 2
+  const float t = __fdividef(1.0f, fmaf(0.23164188700f, a, 1.0f)); // 0.3275911 / sqrt(2)
+  float q = fmaf(1.061405429f, t, -1.453152027f);
+  q = fmaf(q, t, 1.421413741f);
+  q = fmaf(q, t, -0.284496736f);
+  q = fmaf(q, t, 0.254829592f);
+  q *= 0.5f * t * e;                                             // Phi(-|x|)
+  return x < 0.0f ? q : 1.0f - q;
+}
+
 // A NaN passes through every activation (ReLU as well: the comparison is false).
 template <bool FAST>
 __device__ __forceinline__ float fused_act(float x, int32_t act) {
   if (act == FUSED_ACT_RELU) return x < 0.0f ? 0.0f : x;
-  if (act == FUSED_ACT_GELU) return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f));
+  if (act == FUSED_ACT_GELU) {
+    if constexpr (FAST) {
+      float e;
+      return x * fused_normal(x, e);
+    } else {
+      return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f));
+    }
+  }
   if (act == FUSED_ACT_SILU) return x * fused_sigmoid<FAST>(x);
   return x;
 }
@@ -56,8 +80,13 @@ __device__ __forceinline__ float fused_act_gradient(float z, int32_t act) {
   if (act == FUSED_ACT_RELU) return z > 0.0f ? 1.0f : (z <= 0.0f ? 0.0f : z);
   if (act == FUSED_ACT_GELU) {   // Phi(z) + z phi(z)
     const float c = fminf(fmaxf(z, -16.0f), 16.0f);
-    const float e = FAST ? __expf(-0.5f * c * c) : expf(-0.5f * c * c);
-    return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + c * (0.3989422804014327f * e);
+    if constexpr (FAST) {
+      float e;
+      const float phi = fused_normal(z, e);
+      return fmaf(c * 0.3989422804014327f, e, phi);
+    } else {
+      return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + c * (0.3989422804014327f * expf(-0.5f * c * c));
+    }
   }
   if (act == FUSED_ACT_SILU) {
     const float c = fminf(fmaxf(z, -80.0f), 80.0f);

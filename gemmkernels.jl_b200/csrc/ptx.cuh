@@ -317,6 +317,26 @@ __device__ __forceinline__ void tmem_ld_wait() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+// Four 8 x 8 matrices of 16-bit elements between registers and rows of 16 bytes in shared memory, transposed on the
+// way: lane 8q + p names row p of matrix q, and register q of lane i holds elements (2 * (i % 4), i / 4) and
+// (2 * (i % 4) + 1, i / 4) of matrix q.
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint4& v) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, const uint4& v) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};"
+               ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ uint4 shared_load_16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void shared_store_16(uint32_t addr, const uint4& v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
 // Shared-memory matrix descriptor, split in two 32-bit halves so that the issuing thread only
 // adds to the low half while it walks stages and k-steps.
 //   K-major  operand: rows of 128 B (one k-block), 8-row groups `sbo` bytes apart.

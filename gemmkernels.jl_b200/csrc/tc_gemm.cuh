@@ -155,6 +155,7 @@ struct TcParams {
 // Group table of the ragged forms, behind the control block: first tile of each group (groups + 1 values), then
 // first and last + 1 column of each.
 constexpr int kTcCtrlBytes = 256;
+constexpr int kTcStagingBytes = 2048;   // per epilogue warp of the fused forms, behind the table: 32 x 32 16-bit elements
 __host__ __device__ constexpr int tc_table_bytes(int groups) { return (3 * groups + 1) * 4; }
 
 template <int FORM>
@@ -317,15 +318,27 @@ __device__ __forceinline__ void tc_epilogue_chunk(const TcParams& p, const uint3
 }
 
 // Epilogue of up to 32 columns of one row in the fused forms: bit j of `live` says that column j of the chunk exists.
-// d, c and z point at column 0 of the chunk; C and Z have D's type T.  Sixteen columns at a time: their loads of C
+// d, c and z point at column 0 of the chunk; C and Z have D's type T.  Eight columns at a time: their loads of C
 // and Z are issued before the first use, and what is live fits the 168 registers of a 384-thread CTA.
+// A 16-bit element whose type, Float16 or BFloat16, is a run-time choice: one instance of the element-wise code
+// below serves both (two of them cost 300 bytes of spilled registers a thread).
+struct TcHalfWord { uint16_t bits; };
+template <typename T> __device__ __forceinline__ float tc_get(T x, bool) { return x; }
+template <> __device__ __forceinline__ float tc_get<TcHalfWord>(TcHalfWord x, bool f16) {
+  return f16 ? __half2float(__ushort_as_half(x.bits)) : __uint_as_float(static_cast<uint32_t>(x.bits) << 16);
+}
+template <typename T> __device__ __forceinline__ T tc_put(float x, bool) { return x; }
+template <> __device__ __forceinline__ TcHalfWord tc_put<TcHalfWord>(float x, bool f16) {
+  return TcHalfWord{f16 ? __half_as_ushort(__float2half_rn(x)) : __bfloat16_as_ushort(__float2bfloat16_rn(x))};
+}
+
 template <typename T>
 __device__ __forceinline__ void tc_fused_chunk(const TcParams& p, const uint32_t (&v)[32], T* d, const T* c, T* z, float bias_row,
                                                int col0, uint32_t live) {
   constexpr bool kFast = sizeof(T) == 2;
-  constexpr int W = 16;
+  constexpr int W = 8;
   const bool gradient = p.f.form == FUSED_GRADIENT, residual = p.f.form == FUSED_RESIDUAL;
-  const bool has_c = p.beta != 0.0f;
+  const bool has_c = p.beta != 0.0f, f16 = p.dtype_d == TC_F16;
   // Column pointers advance by additions that the compiler cannot see through: left alone it keeps the 32
   // multiples of each stride in registers and spills (800 bytes a thread).
   auto advance = [](auto*& ptr, int64_t step) { ptr += step; asm volatile("" : "+l"(ptr)); };
@@ -354,29 +367,184 @@ __device__ __forceinline__ void tc_fused_chunk(const TcParams& p, const uint32_t
     if (has_c && !residual) {
 #pragma unroll
       for (int j = 0; j < W; ++j)
-        if (in(j)) x[j] += p.beta * tc_to_float(cv[j]);
+        if (in(j)) x[j] += p.beta * tc_get<T>(cv[j], f16);
     }
     if (gradient) {
 #define GK_EACH(expr) _Pragma("unroll") for (int j = 0; j < W; ++j) if (in(j)) { expr; }
-      if (p.act == TC_ACT_RELU) { GK_EACH(x[j] *= fused_act_gradient<kFast>(tc_to_float(zv[j]), TC_ACT_RELU)) }
-      else if (p.act == TC_ACT_GELU) { GK_EACH(x[j] *= fused_act_gradient<kFast>(tc_to_float(zv[j]), TC_ACT_GELU)) }
-      else if (p.act == FUSED_ACT_SILU) { GK_EACH(x[j] *= fused_act_gradient<kFast>(tc_to_float(zv[j]), FUSED_ACT_SILU)) }
+      if (p.act == TC_ACT_RELU) { GK_EACH(x[j] *= fused_act_gradient<kFast>(tc_get<T>(zv[j], f16), TC_ACT_RELU)) }
+      else if (p.act == TC_ACT_GELU) { GK_EACH(x[j] *= fused_act_gradient<kFast>(tc_get<T>(zv[j], f16), TC_ACT_GELU)) }
+      else if (p.act == FUSED_ACT_SILU) { GK_EACH(x[j] *= fused_act_gradient<kFast>(tc_get<T>(zv[j], f16), FUSED_ACT_SILU)) }
     } else {
       if (p.f.Z != nullptr) {
 #pragma unroll
         for (int j = 0; j < W; ++j, advance(z, p.f.z_sn))
-          if (in(j)) *z = tc_from_float<T>(x[j]);
+          if (in(j)) *z = tc_put<T>(x[j], f16);
       }
       if (p.act == TC_ACT_RELU) { GK_EACH(x[j] = fused_act<kFast>(x[j], TC_ACT_RELU)) }
       else if (p.act == TC_ACT_GELU) { GK_EACH(x[j] = fused_act<kFast>(x[j], TC_ACT_GELU)) }
       else if (p.act == FUSED_ACT_SILU) { GK_EACH(x[j] = fused_act<kFast>(x[j], FUSED_ACT_SILU)) }
-      if (has_c && residual) { GK_EACH(x[j] += p.beta * tc_to_float(cv[j])) }
+      if (has_c && residual) { GK_EACH(x[j] += p.beta * tc_get<T>(cv[j], f16)) }
     }
 #undef GK_EACH
 #pragma unroll
     for (int j = 0; j < W; ++j, advance(d, p.d_sn0))
-      if (in(j)) *d = tc_from_float<T>(x[j]);
+      if (in(j)) *d = tc_put<T>(x[j], f16);
   }
+}
+
+// The same for a chunk whose D, C and Z are 16-bit and 16-byte aligned (FusedParams::wide).  A thread owns a row of
+// the accumulator but columns are what is consecutive in memory, so element-wise access moves 64 bytes a request and
+// the 32 requests per array and chunk are what bounds it (8192 x 4096 x 2048 GELU gradient: 207 us).  Here a
+// lane moves 8 rows of a column (16 bytes; a request is 8 columns of 64 bytes) and the warp turns the 32 x 32 block
+// through 2 KiB of its own shared memory with transposing matrix loads and stores: 4 requests instead of 32.
+//   staging: row r holds its 32 columns in four 16-byte slots; slot s lies at s ^ (r >> 1) ^ (r >> 3) (mod 4), which
+//   keeps both the row accesses and the matrix accesses free of bank conflicts.
+//   memory side: lane i has rows 8 * (i % 4) .. + 7 of column 8 * s + i / 4; matrix q of slot s therefore is made of
+//   rows 8 * (p / 2) + 2 * q + p % 2, p = 0 .. 7.
+struct TcStage {
+  uint32_t row;       // shared address of the lane's row
+  uint32_t row_key;
+  uint32_t mat;       // shared address of the row the lane names in matrix accesses
+  uint32_t mat_key;
+  __device__ __forceinline__ TcStage(uint32_t base, int lane) {
+    const int m = 8 * ((lane & 7) >> 1) + 2 * (lane >> 3) + (lane & 1);
+    row = base + lane * 64; row_key = ((lane >> 1) ^ (lane >> 3)) & 3;
+    mat = base + m * 64; mat_key = ((m >> 1) ^ (m >> 3)) & 3;
+  }
+  __device__ __forceinline__ uint32_t row_slot(int s) const { return row + ((s ^ row_key) << 4); }
+  __device__ __forceinline__ uint32_t mat_slot(int s) const { return mat + ((s ^ mat_key) << 4); }
+};
+
+// Loads a chunk's block: `src` is the lane's 8 rows of column i / 4; live as below.
+__device__ __forceinline__ void tc_wide_load(uint4 (&w)[4], const uint16_t* src, int64_t step, uint32_t live_lane) {
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    w[s] = make_uint4(0u, 0u, 0u, 0u);
+    if ((live_lane >> (8 * s)) & 1u) w[s] = *reinterpret_cast<const uint4*>(src + 8 * s * step);
+  }
+}
+
+// Turns what tc_wide_load got so that the lane has the 32 columns of its own row.
+__device__ __forceinline__ void tc_wide_to_row(uint4 (&w)[4], const TcStage& st) {
+#pragma unroll
+  for (int s = 0; s < 4; ++s) stmatrix_x4_trans(st.mat_slot(s), w[s]);
+  __syncwarp();
+#pragma unroll
+  for (int s = 0; s < 4; ++s) w[s] = shared_load_16(st.row_slot(s));
+  __syncwarp();
+}
+
+// Stores the lanes' rows (32 columns each, packed) to memory.
+__device__ __forceinline__ void tc_wide_store(const uint4 (&w)[4], uint16_t* dst, int64_t step, uint32_t live_lane, const TcStage& st) {
+#pragma unroll
+  for (int s = 0; s < 4; ++s) shared_store_16(st.row_slot(s), w[s]);
+  __syncwarp();
+  uint4 t[4];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) ldmatrix_x4_trans(st.mat_slot(s), t[s]);
+  __syncwarp();
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+    if ((live_lane >> (8 * s)) & 1u) *reinterpret_cast<uint4*>(dst + 8 * s * step) = t[s];
+}
+
+template <typename T> __device__ __forceinline__ uint32_t tc_pack(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t tc_pack<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t tc_pack<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T> __device__ __forceinline__ float2 tc_unpack(uint32_t w);
+template <> __device__ __forceinline__ float2 tc_unpack<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+template <> __device__ __forceinline__ float2 tc_unpack<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+// The chunk's arithmetic on the lane's row x (alpha and bias applied): c and z hold the packed columns of C and (read)
+// Z; Z to keep goes to zk, D to d, packed.
+template <typename T, int ACT>
+__device__ __forceinline__ void tc_wide_gradient(float (&x)[32], const uint4 (&z)[4]) {
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    const uint32_t w[4] = {z[s].x, z[s].y, z[s].z, z[s].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 t = tc_unpack<T>(w[i]);
+      x[8 * s + 2 * i] *= fused_act_gradient<true>(t.x, ACT);
+      x[8 * s + 2 * i + 1] *= fused_act_gradient<true>(t.y, ACT);
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void tc_wide_pack(const float (&x)[32], uint4 (&w)[4]) {
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+    w[s] = make_uint4(tc_pack<T>(x[8 * s], x[8 * s + 1]), tc_pack<T>(x[8 * s + 2], x[8 * s + 3]), tc_pack<T>(x[8 * s + 4], x[8 * s + 5]),
+                      tc_pack<T>(x[8 * s + 6], x[8 * s + 7]));
+}
+
+template <typename T>
+__device__ __forceinline__ void tc_wide_add(float (&x)[32], float beta, const uint4 (&c)[4]) {
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    const uint32_t w[4] = {c[s].x, c[s].y, c[s].z, c[s].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 t = tc_unpack<T>(w[i]);
+      x[8 * s + 2 * i] = fmaf(beta, t.x, x[8 * s + 2 * i]);
+      x[8 * s + 2 * i + 1] = fmaf(beta, t.y, x[8 * s + 2 * i + 1]);
+    }
+  }
+}
+
+// One chunk: c and z were loaded with tc_wide_load (c if beta != 0, z in the GRADIENT form); d and zk point at the
+// lane's 8 rows of column i / 4.  All lanes of the warp call.
+template <typename T>
+__device__ __forceinline__ void tc_wide_chunk(const TcParams& p, const uint32_t (&v)[32], uint4 (&c)[4], uint4 (&z)[4], uint16_t* d,
+                                              uint16_t* zk, float bias_row, int col0, uint32_t live, uint32_t live_lane,
+                                              const TcStage& st) {
+  const bool has_c = p.beta != 0.0f, residual = p.f.form == FUSED_RESIDUAL;
+  float x[32];
+#pragma unroll
+  for (int j = 0; j < 32; ++j) x[j] = fmaf(p.alpha, __uint_as_float(v[j]), bias_row);
+  if (p.bias_axis == TC_BIAS_COL) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if ((live >> j) & 1u) x[j] += p.bias[col0 + j];
+  }
+  if (has_c) {
+    tc_wide_to_row(c, st);
+    if (!residual) tc_wide_add<T>(x, p.beta, c);
+  }
+  if (p.f.form == FUSED_GRADIENT) {
+    tc_wide_to_row(z, st);
+    if (p.act == TC_ACT_RELU) tc_wide_gradient<T, TC_ACT_RELU>(x, z);
+    else if (p.act == TC_ACT_GELU) tc_wide_gradient<T, TC_ACT_GELU>(x, z);
+    else if (p.act == FUSED_ACT_SILU) tc_wide_gradient<T, FUSED_ACT_SILU>(x, z);
+  } else {
+    if (p.f.Z != nullptr) {
+      tc_wide_pack<T>(x, z);
+      tc_wide_store(z, zk, p.f.z_sn, live_lane, st);
+    }
+    if (p.act == TC_ACT_RELU) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) x[j] = fused_act<true>(x[j], TC_ACT_RELU);
+    } else if (p.act == TC_ACT_GELU) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) x[j] = fused_act<true>(x[j], TC_ACT_GELU);
+    } else if (p.act == FUSED_ACT_SILU) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) x[j] = fused_act<true>(x[j], FUSED_ACT_SILU);
+    }
+    if (has_c && residual) tc_wide_add<T>(x, p.beta, c);
+  }
+  uint4 w[4];
+  tc_wide_pack<T>(x, w);
+  tc_wide_store(w, d, p.d_sn0, live_lane, st);
 }
 
 // Even-position bits of x packed together (bit 0, 2, 4, ... -> bit 0, 1, 2, ...).
@@ -987,6 +1155,9 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
     const bool fast_store16 = PLANES == 1 && p.dtype_d != TC_F32 && p.beta == 0.0f && p.bias_axis != TC_BIAS_COL &&
                               p.act != TC_ACT_GELU;
     const bool has_c = p.beta != 0.0f;
+    [[maybe_unused]] const TcStage stage(
+        FORM == kTcPlain ? 0u : ((smem_u32(ctrl_gen) + kTcCtrlBytes + (FORM >= kTcRaggedCols ? tc_table_bytes(p.f.groups) : 0) + 15u) & ~15u) +
+                                    (warp - 4) * kTcStagingBytes, lane);
     // plain matrices only (a contraction's C is addressed through two-level strides), planar or real
     pdl_wait();             // D (and C) may still be in use by the previous kernel
     const bool prefetch_c = has_c && p.m_div >= p.M && p.n_div >= p.N && p.c_sm0 == 1 && (PLANES == 1 || p.c_plane != 0);
@@ -1022,6 +1193,14 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
           }
         }
       }
+      if constexpr (FORM != kTcPlain) {
+        if (p.f.form == FUSED_GRADIENT && m - lane < p.M) {      // the same for the tile's part of Z
+          const size_t es = p.dtype_d == TC_F32 ? 4 : 2;
+          const char* z_line = static_cast<const char*>(p.f.Z) + static_cast<size_t>(m - lane) * es;
+          for (int c = lane + chunk_first; c < bn_tile && n0 + c < (FORM == kTcRaggedCols ? n_hi : p.N); c += chunk_step)
+            prefetch_l2(z_line + static_cast<size_t>(n0 + c) * p.f.z_sn * es);
+        }
+      }
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + as * acc_cols;
       const bool m_ok = m < p.M;
       float bias_row = 0.0f;
@@ -1047,33 +1226,59 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
       if (acc_it == 0 && half == 0 && warp == 4 && lane == 0) tc_mark(p.status, dbg, 5, 1);   // first accumulator complete
       const int c_lo = chunk_first + (skew ? half * p.bn : 0), c_hi = skew ? (half + 1) * p.bn : bn_tile;
       for (int c = c_lo; c < c_hi; c += chunk_step) {
+        if constexpr (FORM != kTcPlain) {
+          const int col0 = n0 + c;
+          const int j_lo = max(n_lo - col0, 0), j_hi = min(n_hi - col0, 32);
+          const int m0 = m - lane;
+          if (m0 >= p.M || j_hi <= j_lo) continue;          // the same for the whole warp
+          const uint32_t live = (j_hi == 32 ? 0xffffffffu : (1u << j_hi) - 1u) & (0xffffffffu << j_lo);
+          const uint32_t t_col = t_row + (c >= p.bn ? sub_cols + (c - p.bn) : c);
+          uint32_t v[32];
+          if (p.f.wide) {
+            // the lane's corner on the memory side: rows 8 * (lane % 4) .. + 7 of column lane / 4
+            const int r8 = 8 * (lane & 3), lc = lane >> 2;
+            const uint32_t live_lane = m0 + r8 < p.M ? live >> lc : 0u;
+            const int64_t corner = col0 + lc;
+            const int64_t back = r8 - lane;                  // the row offsets below are those of the lane's own row
+            uint4 cw[4], zw[4];
+            if (has_c) tc_wide_load(cw, static_cast<const uint16_t*>(p.C) + c_row + back + corner * p.c_sn0, p.c_sn0, live_lane);
+            uint16_t* zp = static_cast<uint16_t*>(p.f.Z) + m0 + r8 + corner * p.f.z_sn;
+            if (p.f.form == FUSED_GRADIENT) tc_wide_load(zw, zp, p.f.z_sn, live_lane);
+            uint16_t* dp = static_cast<uint16_t*>(p.D) + d_row + back + corner * p.d_sn0;
+            tmem_ld_32x32(t_col, v);
+            tmem_ld_wait();
+            if (nothing) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = 0u;
+            }
+            if (p.dtype_d == TC_F16) tc_wide_chunk<__half>(p, v, cw, zw, dp, zp, bias_row, col0, live, live_lane, stage);
+            else tc_wide_chunk<__nv_bfloat16>(p, v, cw, zw, dp, zp, bias_row, col0, live, live_lane, stage);
+            continue;
+          }
+          tmem_ld_32x32(t_col, v);
+          tmem_ld_wait();
+          if (!m_ok) continue;
+          if (nothing) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = 0u;
+          }
+          const int64_t ci = c_row + static_cast<int64_t>(col0) * p.c_sn0, di = d_row + static_cast<int64_t>(col0) * p.d_sn0;
+          const int64_t zi = m + static_cast<int64_t>(col0) * p.f.z_sn;
+          auto store = [&](auto tag) {
+            using T = decltype(tag);
+            tc_fused_chunk<T>(p, v, static_cast<T*>(p.D) + di, static_cast<const T*>(p.C) + ci, static_cast<T*>(p.f.Z) + zi,
+                              bias_row, col0, live);
+          };
+          if (p.dtype_d == TC_F32) store(0.0f);
+          else store(TcHalfWord{});
+          continue;
+        }
         uint32_t v[PLANES][32];
         // column c of the tile is column c % bn of block c / bn (bn is a multiple of 32)
         const uint32_t t_col = t_row + (c >= p.bn ? sub_cols + (c - p.bn) : c);
 #pragma unroll
         for (int pl = 0; pl < PLANES; ++pl) tmem_ld_32x32(t_col + pl * p.bn, v[pl]);
         tmem_ld_wait();
-        if constexpr (FORM != kTcPlain) {
-          const int col0 = n0 + c;
-          const int j_lo = max(n_lo - col0, 0), j_hi = min(n_hi - col0, 32);
-          if (!m_ok || j_hi <= j_lo) continue;
-          if (nothing) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[0][j] = 0u;
-          }
-          const int64_t ci = c_row + static_cast<int64_t>(col0) * p.c_sn0, di = d_row + static_cast<int64_t>(col0) * p.d_sn0;
-          const int64_t zi = m + static_cast<int64_t>(col0) * p.f.z_sn;
-          const uint32_t live = (j_hi == 32 ? 0xffffffffu : (1u << j_hi) - 1u) & (0xffffffffu << j_lo);
-          auto store = [&](auto tag) {
-            using T = decltype(tag);
-            tc_fused_chunk<T>(p, v[0], static_cast<T*>(p.D) + di, static_cast<const T*>(p.C) + ci, static_cast<T*>(p.f.Z) + zi,
-                              bias_row, col0, live);
-          };
-          if (p.dtype_d == TC_F32) store(0.0f);
-          else if (p.dtype_d == TC_F16) store(__half());
-          else store(__nv_bfloat16());
-          continue;
-        }
         const int ncols = p.N - (n0 + c);  // columns of this chunk inside the matrix (may be <= 0)
         if (!m_ok || ncols <= 0) continue;
         const int n_in = (n0 + c) % p.n_div, n_out = (n0 + c) / p.n_div;  // a chunk never straddles n_div

@@ -519,7 +519,9 @@ gk_status tc_plan(gk_handle h, const TcProblem& pr_in, bool encode, TcLaunch* ou
   // since that loop became straight-line code the deeper ring of single k-blocks is 1-2 % ahead again
   // (2048^3: 17.2 against 17.5 us, 8192 x 4096 x 8192: 369 against 375 us), and a 256 x 512 tile's MMAs
   // outlast the fixed cost by far.
-  const int table_bytes = pr.form >= kTcRaggedCols ? tc_table_bytes(pr.f.groups) : 0;
+  // group table and the epilogue warps' staging of the layer-level forms
+  const int table_bytes = (pr.form >= kTcRaggedCols ? tc_table_bytes(pr.f.groups) : 0) +
+                          (pr.form != kTcPlain ? 16 + tc_epilogue_warps(1) * kTcStagingBytes : 0);
   const int kSmemBudget = kSmemMax - table_bytes;
   const int kblock_bytes = stage_bytes_for(cg, bn, n_sub, planes, planes);
   const int boxes_per_kblock = planes * (p.a_boxes * p.a_sub + n_sub * p.b_boxes * p.b_sub);   // one lane each in a producer warp
@@ -584,6 +586,11 @@ gk_status tc_plan(gk_handle h, const TcProblem& pr_in, bool encode, TcLaunch* ou
     if (pr.epi->activation < GK_ACT_NONE || pr.epi->activation > (pr.form == kTcPlain ? GK_ACT_GELU : GK_ACT_SILU))
       return set_error(GK_ERR_UNSUPPORTED, "activation %d is not one of none/ReLU/GELU", pr.epi->activation);
     p.act = pr.epi->activation;
+  }
+  if (pr.form != kTcPlain) {
+    auto wide = [](const void* q, int64_t ld) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0 && ld % 8 == 0; };
+    p.f.wide = pr.dtype_d != GK_F32 && p.M % 8 == 0 && wide(p.D, pr.d_sn[0]) && p.d_batch % 8 == 0 &&
+               (p.beta == 0.0f || (wide(p.C, pr.c_sn[0]) && p.c_batch % 8 == 0)) && (!p.f.Z || wide(p.f.Z, p.f.z_sn));
   }
   p.status = h->status_dev;
   p.debug = pr.debug;
