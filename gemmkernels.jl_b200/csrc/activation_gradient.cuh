@@ -42,10 +42,9 @@ template <> __device__ __forceinline__ __half actgrad_round<__half>(float x) { r
 template <> __device__ __forceinline__ __nv_bfloat16 actgrad_round<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
 template <typename T, int VEC, int ACT>
-__global__ void __launch_bounds__(kActGradThreads) activation_gradient_kernel(const ActGradParams p) {
+__global__ void __launch_bounds__(kActGradThreads, 3) activation_gradient_kernel(const ActGradParams p) {
   constexpr int kLanes = kActGradRows / VEC;              // threads along the rows
   constexpr int kSlots = kActGradThreads / kLanes;        // columns in flight
-  constexpr bool kFast = sizeof(T) == 2;
   using V = typename ActGradVec<T, VEC>::type;
   __shared__ float sums[kSlots][kActGradRows + 1];
   __shared__ int item[3];
@@ -78,7 +77,7 @@ __global__ void __launch_bounds__(kActGradThreads) activation_gradient_kernel(co
     const T* dd = static_cast<const T*>(p.dD) + row + static_cast<int64_t>(c0) * p.ldd;
     const T* z = static_cast<const T*>(p.Z) + row + static_cast<int64_t>(c0) * p.ldz;
     T* dz = static_cast<T*>(p.dZ) + row + static_cast<int64_t>(c0) * p.lddz;
-    constexpr int U = 4;                                  // columns per thread whose loads are in flight together
+    constexpr int U = 2;                                  // columns per thread whose loads are in flight together
     for (int c = slot; c < n; c += U * kSlots) {
       V dv[U], zv[U];
 #pragma unroll
@@ -95,12 +94,23 @@ __global__ void __launch_bounds__(kActGradThreads) activation_gradient_kernel(co
         if (col < n) {
           T* de = reinterpret_cast<T*>(&dv[u]);
           const T* ze = reinterpret_cast<const T*>(&zv[u]);
+          if constexpr (sizeof(T) == 2 && VEC > 1) {            // two elements at a time (fused_epilogue.cuh)
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            float v = actgrad_float(de[i]);
-            if (ACT != FUSED_ACT_NONE) v *= fused_act_gradient<kFast>(actgrad_float(ze[i]), ACT);
-            acc[i] += v;
-            de[i] = actgrad_round<T>(v);
+            for (int i = 0; i < VEC; i += 2) {
+              float2 v = make_float2(actgrad_float(de[i]), actgrad_float(de[i + 1]));
+              if (ACT != FUSED_ACT_NONE)
+                v = __fmul2_rn(v, fused_act_gradient2<ACT>(make_float2(actgrad_float(ze[i]), actgrad_float(ze[i + 1]))));
+              acc[i] += v.x; acc[i + 1] += v.y;
+              de[i] = actgrad_round<T>(v.x); de[i + 1] = actgrad_round<T>(v.y);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+              float v = actgrad_float(de[i]);
+              if (ACT != FUSED_ACT_NONE) v *= fused_act_gradient(actgrad_float(ze[i]), ACT);
+              acc[i] += v;
+              de[i] = actgrad_round<T>(v);
+            }
           }
           if (p.dZ != nullptr) *reinterpret_cast<V*>(dz + col * p.lddz) = dv[u];
         }

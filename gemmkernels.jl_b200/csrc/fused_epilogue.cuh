@@ -30,70 +30,116 @@ struct FusedParams {
   int32_t groups;
   int32_t total;           // columns there are: offsets are clamped to [0, total]
   int64_t bias_group;      // elements between the biases of consecutive groups
-  int32_t wide;            // tensor-core kernel: D, C and Z are 16-bit, M and all leading dimensions are multiples of 8
-                           // and the addresses of 16 bytes: the epilogue moves 8 rows of a column per access
+  int32_t wide;            // tensor-core kernel, FusedWide: how the epilogue moves C, D and Z
 };
 
-// FAST: the result is stored in 16 bits, whose half step (2^-12 relative at best) is far above the 2^-21 of
-// the hardware exponential and the approximate quotient; for FP32 results the accurate functions are used.
-template <bool FAST>
-__device__ __forceinline__ float fused_sigmoid(float x) {
-  if constexpr (FAST) return __fdividef(1.0f, 1.0f + __expf(-x));
-  return 1.0f / (1.0f + expf(-x));
+// NONE: element by element.  WORDS: D, C and Z are 16-bit, M and all leading dimensions are multiples of 8 and the
+// addresses of 16 bytes: 8 rows of a column per access.  COPY: D and C are FP32, M and C's leading dimension multiples
+// of 4, C 16-byte aligned and Z not read: C comes through shared memory by asynchronous copies, a chunk ahead.
+enum FusedWide : int32_t { FUSED_WIDE_NONE = 0, FUSED_WIDE_WORDS = 1, FUSED_WIDE_COPY = 2 };
+
+// Activations for results of 32 bits, one element.  A NaN passes through all of them.
+__device__ __forceinline__ float fused_max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float fused_min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 
-// Phi(x), the normal distribution, and e = exp(-x^2 / 2), for results of 16 bits: the rational approximation of
-// the error function by Hastings (Abramowitz and Stegun, 7.1.26; absolute error 1.5e-7) with its exponential at
-// x / sqrt(2) - the one that GELU' needs as well.  The smaller tail is computed, so it keeps its relative accuracy.
-__device__ __forceinline__ float fused_normal(float x, float& e) {
-  const float a = fabsf(x);
-  e = exp2f(-0.72134752044448170f * x * x);                      // log2(e) / 2
-  const float t = __fdividef(1.0f, fmaf(0.23164188700f, a, 1.0f)); // 0.3275911 / sqrt(2)
-  float q = fmaf(1.061405429f, t, -1.453152027f);
-  q = fmaf(q, t, 1.421413741f);
-  q = fmaf(q, t, -0.284496736f);
-  q = fmaf(q, t, 0.254829592f);
-  q *= 0.5f * t * e;                                             // Phi(-|x|)
-  return x < 0.0f ? q : 1.0f - q;
-}
-
-// A NaN passes through every activation (ReLU as well: the comparison is false).
-template <bool FAST>
 __device__ __forceinline__ float fused_act(float x, int32_t act) {
-  if (act == FUSED_ACT_RELU) return x < 0.0f ? 0.0f : x;
-  if (act == FUSED_ACT_GELU) {
-    if constexpr (FAST) {
-      float e;
-      return x * fused_normal(x, e);
-    } else {
-      return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f));
-    }
-  }
-  if (act == FUSED_ACT_SILU) return x * fused_sigmoid<FAST>(x);
+  if (act == FUSED_ACT_RELU) return fused_max_nan(x, 0.0f);
+  if (act == FUSED_ACT_GELU) return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f));
+  if (act == FUSED_ACT_SILU) return x / (1.0f + expf(-x));
   return x;
 }
 
 // act'(z), with ReLU'(0) = 0.  Where z multiplies something that has run out to zero it is clamped first, so
 // that an infinite z (a 16-bit pre-activation that overflowed) gives the limit, 0 or 1, instead of inf * 0.
-template <bool FAST>
 __device__ __forceinline__ float fused_act_gradient(float z, int32_t act) {
   if (act == FUSED_ACT_RELU) return z > 0.0f ? 1.0f : (z <= 0.0f ? 0.0f : z);
   if (act == FUSED_ACT_GELU) {   // Phi(z) + z phi(z)
     const float c = fminf(fmaxf(z, -16.0f), 16.0f);
-    if constexpr (FAST) {
-      float e;
-      const float phi = fused_normal(z, e);
-      return fmaf(c * 0.3989422804014327f, e, phi);
-    } else {
-      return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + c * (0.3989422804014327f * expf(-0.5f * c * c));
-    }
+    return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + c * (0.3989422804014327f * expf(-0.5f * c * c));
   }
   if (act == FUSED_ACT_SILU) {
     const float c = fminf(fmaxf(z, -80.0f), 80.0f);
-    const float s = fused_sigmoid<FAST>(z);
+    const float s = 1.0f / (1.0f + expf(-z));
     return s * (1.0f + c * (1.0f - s));
   }
   return 1.0f;
+}
+
+// The same for results of 16 bits, whose half step (2^-12 relative at best) is far above the 2^-21 of the hardware
+// exponential and reciprocal: two elements at a time, so that the packed FP32 instructions do the arithmetic.
+__device__ __forceinline__ float fused_exp2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float fused_rcp(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float2 fused_2(float x) { return make_float2(x, x); }
+
+// q = Phi(-a), the normal distribution's tail, and e = exp(-a^2 / 2), for a = min(|x|, 16) (beyond it both are
+// zero in FP32).  The rational approximation of the error function by Hastings (Abramowitz and Stegun, 7.1.26;
+// absolute error 1.5e-7) at a / sqrt(2): its exponential is the one that GELU' needs as well, and as it is the tail
+// that is computed, small values keep their relative accuracy.
+__device__ __forceinline__ float2 fused_tail(float2 a, float2& e) {
+  const float2 s = __fmul2_rn(__fmul2_rn(a, a), fused_2(-0.72134752044448170f));        // log2(e) / 2
+  e = make_float2(fused_exp2(s.x), fused_exp2(s.y));
+  const float2 d = __ffma2_rn(a, fused_2(0.23164188700f), fused_2(1.0f));               // 0.3275911 / sqrt(2)
+  const float2 t = make_float2(fused_rcp(d.x), fused_rcp(d.y));
+  float2 q = __ffma2_rn(t, fused_2(0.5f * 1.061405429f), fused_2(0.5f * -1.453152027f));
+  q = __ffma2_rn(q, t, fused_2(0.5f * 1.421413741f));
+  q = __ffma2_rn(q, t, fused_2(0.5f * -0.284496736f));
+  q = __ffma2_rn(q, t, fused_2(0.5f * 0.254829592f));
+  return __fmul2_rn(__fmul2_rn(q, t), e);
+}
+
+__device__ __forceinline__ float2 fused_sigmoid2(float2 x) {
+  const float2 s = __fmul2_rn(x, fused_2(-1.4426950408889634f));
+  const float2 d = __fadd2_rn(make_float2(fused_exp2(s.x), fused_exp2(s.y)), fused_2(1.0f));
+  return make_float2(fused_rcp(d.x), fused_rcp(d.y));
+}
+
+template <int ACT>
+__device__ __forceinline__ float2 fused_act2(float2 x) {
+  if constexpr (ACT == FUSED_ACT_RELU) return make_float2(fused_max_nan(x.x, 0.0f), fused_max_nan(x.y, 0.0f));
+  if constexpr (ACT == FUSED_ACT_GELU) {      // x Phi(x) = max(x, 0) - |x| Phi(-|x|)
+    float2 e;
+    const float2 a = make_float2(fused_min_nan(fabsf(x.x), 16.0f), fused_min_nan(fabsf(x.y), 16.0f));
+    const float2 q = fused_tail(a, e);
+    return __ffma2_rn(make_float2(-a.x, -a.y), q, make_float2(fmaxf(x.x, 0.0f), fmaxf(x.y, 0.0f)));
+  }
+  if constexpr (ACT == FUSED_ACT_SILU) return __fmul2_rn(x, fused_sigmoid2(x));
+  return x;
+}
+
+template <int ACT>
+__device__ __forceinline__ float2 fused_act_gradient2(float2 z) {
+  if constexpr (ACT == FUSED_ACT_RELU) return make_float2(fused_act_gradient(z.x, FUSED_ACT_RELU), fused_act_gradient(z.y, FUSED_ACT_RELU));
+  if constexpr (ACT == FUSED_ACT_GELU) {
+    float2 e;
+    const float2 a = make_float2(fused_min_nan(fabsf(z.x), 16.0f), fused_min_nan(fabsf(z.y), 16.0f));
+    const float2 q = fused_tail(a, e), r = __ffma2_rn(q, fused_2(-1.0f), fused_2(1.0f));
+    const float2 phi = make_float2(z.x > 0.0f ? r.x : q.x, z.y > 0.0f ? r.y : q.y);
+    const float2 c = make_float2(copysignf(a.x, z.x), copysignf(a.y, z.y));
+    return __ffma2_rn(__fmul2_rn(c, fused_2(0.3989422804014327f)), e, phi);
+  }
+  if constexpr (ACT == FUSED_ACT_SILU) {
+    const float2 s = fused_sigmoid2(z);
+    const float2 c = make_float2(fminf(fmaxf(z.x, -80.0f), 80.0f), fminf(fmaxf(z.y, -80.0f), 80.0f));
+    const float2 w = __ffma2_rn(c, __ffma2_rn(s, fused_2(-1.0f), fused_2(1.0f)), fused_2(1.0f));
+    return __fmul2_rn(s, w);
+  }
+  return fused_2(1.0f);
 }
 
 __device__ __forceinline__ float fused_load(const void* p, int64_t i, int dt) {   // dt: 0 F16, 1 BF16, 2 F32
@@ -115,9 +161,9 @@ __device__ __forceinline__ float fused_finish(const FusedParams& f, float x, flo
   const float c = beta != 0.0f ? beta * fused_load(C, ci, dtype_c) : 0.0f;
   const int64_t zi = m + n * f.z_sn;
   if (f.form != FUSED_RESIDUAL && beta != 0.0f) x += c;
-  if (f.form == FUSED_GRADIENT) return x * fused_act_gradient<false>(fused_load(f.Z, zi, f.dtype_z), act);
+  if (f.form == FUSED_GRADIENT) return x * fused_act_gradient(fused_load(f.Z, zi, f.dtype_z), act);
   if (f.Z != nullptr) fused_put(f.Z, zi, f.dtype_z, x);
-  x = fused_act<false>(x, act);
+  x = fused_act(x, act);
   return f.form == FUSED_RESIDUAL && beta != 0.0f ? x + c : x;
 }
 

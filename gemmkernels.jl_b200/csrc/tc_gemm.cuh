@@ -155,7 +155,8 @@ struct TcParams {
 // Group table of the ragged forms, behind the control block: first tile of each group (groups + 1 values), then
 // first and last + 1 column of each.
 constexpr int kTcCtrlBytes = 256;
-constexpr int kTcStagingBytes = 2048;   // per epilogue warp of the fused forms, behind the table: 32 x 32 16-bit elements
+// Per epilogue warp of the fused forms, behind the table: a block of 32 x 32 16-bit elements, or two of FP32 ones.
+__host__ __device__ constexpr int tc_staging_bytes(int wide) { return wide == FUSED_WIDE_COPY ? 2 * 32 * 32 * 4 : 32 * 32 * 2; }
 __host__ __device__ constexpr int tc_table_bytes(int groups) { return (3 * groups + 1) * 4; }
 
 template <int FORM>
@@ -318,7 +319,8 @@ __device__ __forceinline__ void tc_epilogue_chunk(const TcParams& p, const uint3
 }
 
 // Epilogue of up to 32 columns of one row in the fused forms: bit j of `live` says that column j of the chunk exists.
-// d, c and z point at column 0 of the chunk; C and Z have D's type T.  Eight columns at a time: their loads of C
+// d, c and z point at column 0 of the chunk; C and Z have D's type T; c_row_shared != 0: the
+// lane's row of C is in shared memory already (tc_copy_block).  Eight columns at a time: their loads of C
 // and Z are issued before the first use, and what is live fits the 168 registers of a 384-thread CTA.
 // A 16-bit element whose type, Float16 or BFloat16, is a run-time choice: one instance of the element-wise code
 // below serves both (two of them cost 300 bytes of spilled registers a thread).
@@ -334,8 +336,7 @@ template <> __device__ __forceinline__ TcHalfWord tc_put<TcHalfWord>(float x, bo
 
 template <typename T>
 __device__ __forceinline__ void tc_fused_chunk(const TcParams& p, const uint32_t (&v)[32], T* d, const T* c, T* z, float bias_row,
-                                               int col0, uint32_t live) {
-  constexpr bool kFast = sizeof(T) == 2;
+                                               int col0, uint32_t live, uint32_t c_row_shared = 0) {
   constexpr int W = 8;
   const bool gradient = p.f.form == FUSED_GRADIENT, residual = p.f.form == FUSED_RESIDUAL;
   const bool has_c = p.beta != 0.0f, f16 = p.dtype_d == TC_F16;
@@ -347,9 +348,19 @@ __device__ __forceinline__ void tc_fused_chunk(const TcParams& p, const uint32_t
     auto in = [&](int j) { return (live >> (h + j)) & 1u; };
     T cv[W], zv[W];
     if (has_c) {
+      bool copied = false;
+      if constexpr (sizeof(T) == 4) {
+        if (c_row_shared != 0) {
+          copied = true;
 #pragma unroll
-      for (int j = 0; j < W; ++j, advance(c, p.c_sn0))
-        if (in(j)) cv[j] = *c;
+          for (int j = 0; j < W; ++j) cv[j] = shared_load_f32(c_row_shared + (h + j) * 128);
+        }
+      }
+      if (!copied) {
+#pragma unroll
+        for (int j = 0; j < W; ++j, advance(c, p.c_sn0))
+          if (in(j)) cv[j] = *c;
+      }
     }
     if (gradient) {
 #pragma unroll
@@ -371,18 +382,18 @@ __device__ __forceinline__ void tc_fused_chunk(const TcParams& p, const uint32_t
     }
     if (gradient) {
 #define GK_EACH(expr) _Pragma("unroll") for (int j = 0; j < W; ++j) if (in(j)) { expr; }
-      if (p.act == TC_ACT_RELU) { GK_EACH(x[j] *= fused_act_gradient<kFast>(tc_get<T>(zv[j], f16), TC_ACT_RELU)) }
-      else if (p.act == TC_ACT_GELU) { GK_EACH(x[j] *= fused_act_gradient<kFast>(tc_get<T>(zv[j], f16), TC_ACT_GELU)) }
-      else if (p.act == FUSED_ACT_SILU) { GK_EACH(x[j] *= fused_act_gradient<kFast>(tc_get<T>(zv[j], f16), FUSED_ACT_SILU)) }
+      if (p.act == TC_ACT_RELU) { GK_EACH(x[j] *= fused_act_gradient(tc_get<T>(zv[j], f16), TC_ACT_RELU)) }
+      else if (p.act == TC_ACT_GELU) { GK_EACH(x[j] *= fused_act_gradient(tc_get<T>(zv[j], f16), TC_ACT_GELU)) }
+      else if (p.act == FUSED_ACT_SILU) { GK_EACH(x[j] *= fused_act_gradient(tc_get<T>(zv[j], f16), FUSED_ACT_SILU)) }
     } else {
       if (p.f.Z != nullptr) {
 #pragma unroll
         for (int j = 0; j < W; ++j, advance(z, p.f.z_sn))
           if (in(j)) *z = tc_put<T>(x[j], f16);
       }
-      if (p.act == TC_ACT_RELU) { GK_EACH(x[j] = fused_act<kFast>(x[j], TC_ACT_RELU)) }
-      else if (p.act == TC_ACT_GELU) { GK_EACH(x[j] = fused_act<kFast>(x[j], TC_ACT_GELU)) }
-      else if (p.act == FUSED_ACT_SILU) { GK_EACH(x[j] = fused_act<kFast>(x[j], FUSED_ACT_SILU)) }
+      if (p.act == TC_ACT_RELU) { GK_EACH(x[j] = fused_act(x[j], TC_ACT_RELU)) }
+      else if (p.act == TC_ACT_GELU) { GK_EACH(x[j] = fused_act(x[j], TC_ACT_GELU)) }
+      else if (p.act == FUSED_ACT_SILU) { GK_EACH(x[j] = fused_act(x[j], FUSED_ACT_SILU)) }
       if (has_c && residual) { GK_EACH(x[j] += p.beta * tc_get<T>(cv[j], f16)) }
     }
 #undef GK_EACH
@@ -402,11 +413,12 @@ __device__ __forceinline__ void tc_fused_chunk(const TcParams& p, const uint32_t
 //   memory side: lane i has rows 8 * (i % 4) .. + 7 of column 8 * s + i / 4; matrix q of slot s therefore is made of
 //   rows 8 * (p / 2) + 2 * q + p % 2, p = 0 .. 7.
 struct TcStage {
+  uint32_t base;
   uint32_t row;       // shared address of the lane's row
   uint32_t row_key;
   uint32_t mat;       // shared address of the row the lane names in matrix accesses
   uint32_t mat_key;
-  __device__ __forceinline__ TcStage(uint32_t base, int lane) {
+  __device__ __forceinline__ TcStage(uint32_t base, int lane) : base(base) {
     const int m = 8 * ((lane & 7) >> 1) + 2 * (lane >> 3) + (lane & 1);
     row = base + lane * 64; row_key = ((lane >> 1) ^ (lane >> 3)) & 3;
     mat = base + m * 64; mat_key = ((m >> 1) ^ (m >> 3)) & 3;
@@ -414,6 +426,18 @@ struct TcStage {
   __device__ __forceinline__ uint32_t row_slot(int s) const { return row + ((s ^ row_key) << 4); }
   __device__ __forceinline__ uint32_t mat_slot(int s) const { return mat + ((s ^ mat_key) << 4); }
 };
+
+// FUSED_WIDE_COPY: starts the copies of the 32 x 32 block of C at rows m0, columns col0 into `buf` (columns of 128 bytes),
+// eight 16-byte pieces per lane.
+__device__ __forceinline__ void tc_copy_block(const TcParams& p, uint32_t buf, const float* c_col0, int m0, int64_t c_step, uint32_t live,
+                                              int lane) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int piece = lane + 32 * i, col = piece >> 3, part = piece & 7;
+    const bool ok = ((live >> col) & 1u) && m0 + 4 * part < p.M;
+    async_copy_16(buf + piece * 16, ok ? c_col0 + 4 * part + col * c_step : static_cast<const float*>(p.C), ok ? 16u : 0u);
+  }
+}
 
 // Loads a chunk's block: `src` is the lane's 8 rows of column i / 4; live as below.
 __device__ __forceinline__ void tc_wide_load(uint4 (&w)[4], const uint16_t* src, int64_t step, uint32_t live_lane) {
@@ -463,86 +487,83 @@ template <> __device__ __forceinline__ float2 tc_unpack<__nv_bfloat16>(uint32_t 
   return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 
-// The chunk's arithmetic on the lane's row x (alpha and bias applied): c and z hold the packed columns of C and (read)
-// Z; Z to keep goes to zk, D to d, packed.
-template <typename T, int ACT>
-__device__ __forceinline__ void tc_wide_gradient(float (&x)[32], const uint4 (&z)[4]) {
-#pragma unroll
-  for (int s = 0; s < 4; ++s) {
-    const uint32_t w[4] = {z[s].x, z[s].y, z[s].z, z[s].w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 t = tc_unpack<T>(w[i]);
-      x[8 * s + 2 * i] *= fused_act_gradient<true>(t.x, ACT);
-      x[8 * s + 2 * i + 1] *= fused_act_gradient<true>(t.y, ACT);
-    }
-  }
-}
-
+// The lane's row as 16 pairs of columns.  A packed 16-byte slot s holds the pairs 4 * s .. 4 * s + 3.
 template <typename T>
-__device__ __forceinline__ void tc_wide_pack(const float (&x)[32], uint4 (&w)[4]) {
+__device__ __forceinline__ void tc_wide_pack(const float2 (&x)[16], uint4 (&w)[4]) {
 #pragma unroll
   for (int s = 0; s < 4; ++s)
-    w[s] = make_uint4(tc_pack<T>(x[8 * s], x[8 * s + 1]), tc_pack<T>(x[8 * s + 2], x[8 * s + 3]), tc_pack<T>(x[8 * s + 4], x[8 * s + 5]),
-                      tc_pack<T>(x[8 * s + 6], x[8 * s + 7]));
+    w[s] = make_uint4(tc_pack<T>(x[4 * s].x, x[4 * s].y), tc_pack<T>(x[4 * s + 1].x, x[4 * s + 1].y),
+                      tc_pack<T>(x[4 * s + 2].x, x[4 * s + 2].y), tc_pack<T>(x[4 * s + 3].x, x[4 * s + 3].y));
+}
+
+__device__ __forceinline__ uint32_t tc_word(const uint4 (&w)[4], int i) {      // pair i of the row (i is a constant)
+  const uint4& q = w[i >> 2];
+  return (i & 3) == 0 ? q.x : (i & 3) == 1 ? q.y : (i & 3) == 2 ? q.z : q.w;
+}
+
+template <typename T, int ACT>
+__device__ __forceinline__ void tc_wide_gradient(float2 (&x)[16], const uint4 (&z)[4]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = __fmul2_rn(x[i], fused_act_gradient2<ACT>(tc_unpack<T>(tc_word(z, i))));
 }
 
 template <typename T>
-__device__ __forceinline__ void tc_wide_add(float (&x)[32], float beta, const uint4 (&c)[4]) {
+__device__ __forceinline__ void tc_wide_add(float2 (&x)[16], float beta, const uint4 (&c)[4]) {
 #pragma unroll
-  for (int s = 0; s < 4; ++s) {
-    const uint32_t w[4] = {c[s].x, c[s].y, c[s].z, c[s].w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 t = tc_unpack<T>(w[i]);
-      x[8 * s + 2 * i] = fmaf(beta, t.x, x[8 * s + 2 * i]);
-      x[8 * s + 2 * i + 1] = fmaf(beta, t.y, x[8 * s + 2 * i + 1]);
-    }
-  }
+  for (int i = 0; i < 16; ++i) x[i] = __ffma2_rn(fused_2(beta), tc_unpack<T>(tc_word(c, i)), x[i]);
 }
 
-// One chunk: c and z were loaded with tc_wide_load (c if beta != 0, z in the GRADIENT form); d and zk point at the
-// lane's 8 rows of column i / 4.  All lanes of the warp call.
+template <int ACT>
+__device__ __forceinline__ void tc_wide_act(float2 (&x)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = fused_act2<ACT>(x[i]);
+}
+
+// One chunk: `w` was loaded with tc_wide_load from Z (GRADIENT form) or else from C; c, d and z point at the lane's 8
+// rows of column i / 4.  All lanes of the warp call.
 template <typename T>
-__device__ __forceinline__ void tc_wide_chunk(const TcParams& p, const uint32_t (&v)[32], uint4 (&c)[4], uint4 (&z)[4], uint16_t* d,
-                                              uint16_t* zk, float bias_row, int col0, uint32_t live, uint32_t live_lane,
+__device__ __forceinline__ void tc_wide_chunk(const TcParams& p, const uint32_t (&v)[32], uint4 (&w)[4], const uint16_t* c, uint16_t* d,
+                                              uint16_t* z, float bias_row, int col0, uint32_t live, uint32_t live_lane,
                                               const TcStage& st) {
-  const bool has_c = p.beta != 0.0f, residual = p.f.form == FUSED_RESIDUAL;
-  float x[32];
+  const bool has_c = p.beta != 0.0f;
+  float2 x[16];
 #pragma unroll
-  for (int j = 0; j < 32; ++j) x[j] = fmaf(p.alpha, __uint_as_float(v[j]), bias_row);
+  for (int i = 0; i < 16; ++i)
+    x[i] = __ffma2_rn(fused_2(p.alpha), make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), fused_2(bias_row));
   if (p.bias_axis == TC_BIAS_COL) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if ((live >> j) & 1u) x[j] += p.bias[col0 + j];
-  }
-  if (has_c) {
-    tc_wide_to_row(c, st);
-    if (!residual) tc_wide_add<T>(x, p.beta, c);
+    for (int i = 0; i < 16; ++i) {
+      if ((live >> (2 * i)) & 1u) x[i].x += p.bias[col0 + 2 * i];
+      if ((live >> (2 * i + 1)) & 1u) x[i].y += p.bias[col0 + 2 * i + 1];
+    }
   }
   if (p.f.form == FUSED_GRADIENT) {
-    tc_wide_to_row(z, st);
-    if (p.act == TC_ACT_RELU) tc_wide_gradient<T, TC_ACT_RELU>(x, z);
-    else if (p.act == TC_ACT_GELU) tc_wide_gradient<T, TC_ACT_GELU>(x, z);
-    else if (p.act == FUSED_ACT_SILU) tc_wide_gradient<T, FUSED_ACT_SILU>(x, z);
+    if (has_c) {
+      uint4 cw[4];
+      tc_wide_load(cw, c, p.c_sn0, live_lane);
+      tc_wide_to_row(cw, st);
+      tc_wide_add<T>(x, p.beta, cw);
+    }
+    tc_wide_to_row(w, st);
+    if (p.act == TC_ACT_RELU) tc_wide_gradient<T, FUSED_ACT_RELU>(x, w);
+    else if (p.act == TC_ACT_GELU) tc_wide_gradient<T, FUSED_ACT_GELU>(x, w);
+    else if (p.act == FUSED_ACT_SILU) tc_wide_gradient<T, FUSED_ACT_SILU>(x, w);
   } else {
+    const bool residual = p.f.form == FUSED_RESIDUAL;
+    if (has_c) {
+      tc_wide_to_row(w, st);
+      if (!residual) tc_wide_add<T>(x, p.beta, w);
+    }
     if (p.f.Z != nullptr) {
-      tc_wide_pack<T>(x, z);
-      tc_wide_store(z, zk, p.f.z_sn, live_lane, st);
+      uint4 t[4];
+      tc_wide_pack<T>(x, t);
+      tc_wide_store(t, z, p.f.z_sn, live_lane, st);
     }
-    if (p.act == TC_ACT_RELU) {
-#pragma unroll
-      for (int j = 0; j < 32; ++j) x[j] = fused_act<true>(x[j], TC_ACT_RELU);
-    } else if (p.act == TC_ACT_GELU) {
-#pragma unroll
-      for (int j = 0; j < 32; ++j) x[j] = fused_act<true>(x[j], TC_ACT_GELU);
-    } else if (p.act == FUSED_ACT_SILU) {
-#pragma unroll
-      for (int j = 0; j < 32; ++j) x[j] = fused_act<true>(x[j], FUSED_ACT_SILU);
-    }
-    if (has_c && residual) tc_wide_add<T>(x, p.beta, c);
+    if (p.act == TC_ACT_RELU) tc_wide_act<FUSED_ACT_RELU>(x);
+    else if (p.act == TC_ACT_GELU) tc_wide_act<FUSED_ACT_GELU>(x);
+    else if (p.act == FUSED_ACT_SILU) tc_wide_act<FUSED_ACT_SILU>(x);
+    if (has_c && residual) tc_wide_add<T>(x, p.beta, w);
   }
-  uint4 w[4];
   tc_wide_pack<T>(x, w);
   tc_wide_store(w, d, p.d_sn0, live_lane, st);
 }
@@ -1157,7 +1178,7 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
     const bool has_c = p.beta != 0.0f;
     [[maybe_unused]] const TcStage stage(
         FORM == kTcPlain ? 0u : ((smem_u32(ctrl_gen) + kTcCtrlBytes + (FORM >= kTcRaggedCols ? tc_table_bytes(p.f.groups) : 0) + 15u) & ~15u) +
-                                    (warp - 4) * kTcStagingBytes, lane);
+                                    (warp - 4) * tc_staging_bytes(p.f.wide), lane);
     // plain matrices only (a contraction's C is addressed through two-level strides), planar or real
     pdl_wait();             // D (and C) may still be in use by the previous kernel
     const bool prefetch_c = has_c && p.m_div >= p.M && p.n_div >= p.N && p.c_sm0 == 1 && (PLANES == 1 || p.c_plane != 0);
@@ -1213,6 +1234,38 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
       long long e0 = 0, e1 = 0;
       for (int half = 0; half < (skew ? 2 : 1); ++half) {
       const uint32_t hb = skew ? static_cast<uint32_t>(half) : as;
+      [[maybe_unused]] const int c_lo = chunk_first + (skew ? half * p.bn : 0), c_hi = skew ? (half + 1) * p.bn : bn_tile;
+      // Fused forms.  live_of(c): which columns of the chunk at c belong to this warp's part of the matrix (bit j:
+      // column n0 + c + j).  fetch(c): starts loading the chunk's C, or the Z of the gradient form, into `buf` or into
+      // registers; the first chunk's goes out before the accumulators are waited for.
+      [[maybe_unused]] const int m0 = m - lane, r8 = 8 * (lane & 3), lc = lane >> 2;   // the lane's corner on the memory side
+      [[maybe_unused]] const int64_t back = r8 - lane;       // c_row and d_row are those of the lane's own row
+      [[maybe_unused]] const uint16_t* c_word = static_cast<const uint16_t*>(p.C) + c_row + back;
+      [[maybe_unused]] auto live_of = [&](int c) -> uint32_t {
+        const int col0 = n0 + c, j_lo = max(n_lo - col0, 0), j_hi = min(n_hi - col0, 32);
+        if (m0 >= p.M || j_hi <= j_lo) return 0u;
+        return (j_hi == 32 ? 0xffffffffu : (1u << j_hi) - 1u) & (0xffffffffu << j_lo);
+      };
+      [[maybe_unused]] uint32_t buf = 0;
+      [[maybe_unused]] uint4 fetched[4];
+      [[maybe_unused]] auto fetch = [&](int c, uint32_t into, uint4 (&w)[4]) {
+        const uint32_t live = live_of(c);
+        if (p.f.wide == FUSED_WIDE_COPY) {
+          tc_copy_block(p, stage.base + into, static_cast<const float*>(p.C) + c_row - lane + static_cast<int64_t>(n0 + c) * p.c_sn0, m0,
+                        p.c_sn0, live, lane);
+        } else {
+          const uint32_t live_lane = m0 + r8 < p.M ? live >> lc : 0u;
+          const int64_t corner = n0 + c + lc;
+          if (p.f.form == FUSED_GRADIENT) tc_wide_load(w, static_cast<const uint16_t*>(p.f.Z) + m0 + r8 + corner * p.f.z_sn, p.f.z_sn, live_lane);
+          else if (has_c) tc_wide_load(w, c_word + corner * p.c_sn0, p.c_sn0, live_lane);
+        }
+      };
+      if constexpr (FORM != kTcPlain) {
+        if (p.f.wide != FUSED_WIDE_NONE && c_lo < c_hi) {
+          fetch(c_lo, 0u, fetched);
+          if (p.f.wide == FUSED_WIDE_COPY) async_copy_commit();
+        }
+      }
       // all-or-nothing per warp: the TMEM loads below are warp-collective
       e0 = (dbg & 8) ? clock64() : 0;
       const bool got = mbar_wait(bar_tfull + 8u * hb, aph, abort_flag, kTcWaitLimitNs);
@@ -1224,53 +1277,57 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
       }
       tc_fence_after_sync();
       if (acc_it == 0 && half == 0 && warp == 4 && lane == 0) tc_mark(p.status, dbg, 5, 1);   // first accumulator complete
-      const int c_lo = chunk_first + (skew ? half * p.bn : 0), c_hi = skew ? (half + 1) * p.bn : bn_tile;
       for (int c = c_lo; c < c_hi; c += chunk_step) {
         if constexpr (FORM != kTcPlain) {
+          // C (or the Z of the gradient form) of the next chunk is fetched before this one is finished
+          const uint32_t live = live_of(c);
           const int col0 = n0 + c;
-          const int j_lo = max(n_lo - col0, 0), j_hi = min(n_hi - col0, 32);
-          const int m0 = m - lane;
-          if (m0 >= p.M || j_hi <= j_lo) continue;          // the same for the whole warp
-          const uint32_t live = (j_hi == 32 ? 0xffffffffu : (1u << j_hi) - 1u) & (0xffffffffu << j_lo);
-          const uint32_t t_col = t_row + (c >= p.bn ? sub_cols + (c - p.bn) : c);
-          uint32_t v[32];
-          if (p.f.wide) {
-            // the lane's corner on the memory side: rows 8 * (lane % 4) .. + 7 of column lane / 4
-            const int r8 = 8 * (lane & 3), lc = lane >> 2;
-            const uint32_t live_lane = m0 + r8 < p.M ? live >> lc : 0u;
-            const int64_t corner = col0 + lc;
-            const int64_t back = r8 - lane;                  // the row offsets below are those of the lane's own row
-            uint4 cw[4], zw[4];
-            if (has_c) tc_wide_load(cw, static_cast<const uint16_t*>(p.C) + c_row + back + corner * p.c_sn0, p.c_sn0, live_lane);
-            uint16_t* zp = static_cast<uint16_t*>(p.f.Z) + m0 + r8 + corner * p.f.z_sn;
-            if (p.f.form == FUSED_GRADIENT) tc_wide_load(zw, zp, p.f.z_sn, live_lane);
-            uint16_t* dp = static_cast<uint16_t*>(p.D) + d_row + back + corner * p.d_sn0;
+          [[maybe_unused]] uint4 ahead[4];
+          if (p.f.wide == FUSED_WIDE_COPY) {
+            if (c + chunk_step < c_hi) fetch(c + chunk_step, buf ^ 4096u, ahead);
+            async_copy_commit();
+          } else if (p.f.wide == FUSED_WIDE_WORDS && c + chunk_step < c_hi) {
+            fetch(c + chunk_step, 0u, ahead);
+          }
+          if (live != 0u) {                                  // the same for the whole warp
+            const uint32_t t_col = t_row + (c >= p.bn ? sub_cols + (c - p.bn) : c);
+            uint32_t v[32];
             tmem_ld_32x32(t_col, v);
             tmem_ld_wait();
             if (nothing) {
 #pragma unroll
               for (int j = 0; j < 32; ++j) v[j] = 0u;
             }
-            if (p.dtype_d == TC_F16) tc_wide_chunk<__half>(p, v, cw, zw, dp, zp, bias_row, col0, live, live_lane, stage);
-            else tc_wide_chunk<__nv_bfloat16>(p, v, cw, zw, dp, zp, bias_row, col0, live, live_lane, stage);
-            continue;
+            if (p.f.wide == FUSED_WIDE_WORDS) {
+              const uint32_t live_lane = m0 + r8 < p.M ? live >> lc : 0u;
+              const int64_t corner = col0 + lc;
+              uint16_t* zp = static_cast<uint16_t*>(p.f.Z) + m0 + r8 + corner * p.f.z_sn;
+              uint16_t* dp = static_cast<uint16_t*>(p.D) + d_row + back + corner * p.d_sn0;
+              if (p.dtype_d == TC_F16) tc_wide_chunk<__half>(p, v, fetched, c_word + corner * p.c_sn0, dp, zp, bias_row, col0, live, live_lane, stage);
+              else tc_wide_chunk<__nv_bfloat16>(p, v, fetched, c_word + corner * p.c_sn0, dp, zp, bias_row, col0, live, live_lane, stage);
+            } else {
+              uint32_t c_row_shared = 0;
+              if (p.f.wide == FUSED_WIDE_COPY) {
+                async_copy_wait<1>();
+                __syncwarp();
+                c_row_shared = stage.base + buf + 4 * lane;
+              }
+              if (m_ok) {
+                const int64_t ci = c_row + static_cast<int64_t>(col0) * p.c_sn0, di = d_row + static_cast<int64_t>(col0) * p.d_sn0;
+                const int64_t zi = m + static_cast<int64_t>(col0) * p.f.z_sn;
+                if (p.dtype_d == TC_F32)
+                  tc_fused_chunk<float>(p, v, static_cast<float*>(p.D) + di, static_cast<const float*>(p.C) + ci, static_cast<float*>(p.f.Z) + zi,
+                                        bias_row, col0, live, c_row_shared);
+                else
+                  tc_fused_chunk<TcHalfWord>(p, v, static_cast<TcHalfWord*>(p.D) + di, static_cast<const TcHalfWord*>(p.C) + ci,
+                                             static_cast<TcHalfWord*>(p.f.Z) + zi, bias_row, col0, live);
+              }
+            }
           }
-          tmem_ld_32x32(t_col, v);
-          tmem_ld_wait();
-          if (!m_ok) continue;
-          if (nothing) {
+          __syncwarp();                                      // the buffer just read is filled again in the next round
+          buf ^= 4096u;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = 0u;
-          }
-          const int64_t ci = c_row + static_cast<int64_t>(col0) * p.c_sn0, di = d_row + static_cast<int64_t>(col0) * p.d_sn0;
-          const int64_t zi = m + static_cast<int64_t>(col0) * p.f.z_sn;
-          auto store = [&](auto tag) {
-            using T = decltype(tag);
-            tc_fused_chunk<T>(p, v, static_cast<T*>(p.D) + di, static_cast<const T*>(p.C) + ci, static_cast<T*>(p.f.Z) + zi,
-                              bias_row, col0, live);
-          };
-          if (p.dtype_d == TC_F32) store(0.0f);
-          else store(TcHalfWord{});
+          for (int i = 0; i < 4; ++i) fetched[i] = ahead[i];
           continue;
         }
         uint32_t v[PLANES][32];
@@ -1386,6 +1443,7 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
         p.dbg_out[blockIdx.x * 16 + 15] = static_cast<long long>(global_timer_ns());   // last tile stored
       }
     }
+    if constexpr (FORM != kTcPlain) async_copy_wait<0>();   // (only a loop that was left early has copies in flight)
   }
 
   // ------------------------------------------------------------------ teardown

@@ -520,8 +520,22 @@ gk_status tc_plan(gk_handle h, const TcProblem& pr_in, bool encode, TcLaunch* ou
   // (2048^3: 17.2 against 17.5 us, 8192 x 4096 x 8192: 369 against 375 us), and a 256 x 512 tile's MMAs
   // outlast the fixed cost by far.
   // group table and the epilogue warps' staging of the layer-level forms
-  const int table_bytes = (pr.form >= kTcRaggedCols ? tc_table_bytes(pr.f.groups) : 0) +
-                          (pr.form != kTcPlain ? 16 + tc_epilogue_warps(1) * kTcStagingBytes : 0);
+  int table_bytes = 0;
+  if (pr.form != kTcPlain) {
+    auto wide = [](const void* q, int64_t ld, int64_t batch, int unit) {
+      return (reinterpret_cast<uintptr_t>(q) & 15) == 0 && ld % unit == 0 && batch % unit == 0;
+    };
+    const bool reads_c = pr.C != nullptr && pr.beta != 0.0;
+    p.f.wide = FUSED_WIDE_NONE;
+    if (pr.dtype_d != GK_F32) {
+      if (p.M % 8 == 0 && wide(pr.D, pr.d_sn[0], pr.batch_d, 8) && (!reads_c || wide(pr.C, pr.c_sn[0], pr.batch_c, 8)) &&
+          (!p.f.Z || wide(p.f.Z, p.f.z_sn, 0, 8)))
+        p.f.wide = FUSED_WIDE_WORDS;
+    } else if (reads_c && p.f.form != FUSED_GRADIENT && p.M % 4 == 0 && wide(pr.C, pr.c_sn[0], pr.batch_c, 4)) {
+      p.f.wide = FUSED_WIDE_COPY;
+    }
+    table_bytes = (pr.form >= kTcRaggedCols ? tc_table_bytes(pr.f.groups) : 0) + 16 + tc_epilogue_warps(1) * tc_staging_bytes(p.f.wide);
+  }
   const int kSmemBudget = kSmemMax - table_bytes;
   const int kblock_bytes = stage_bytes_for(cg, bn, n_sub, planes, planes);
   const int boxes_per_kblock = planes * (p.a_boxes * p.a_sub + n_sub * p.b_boxes * p.b_sub);   // one lane each in a producer warp
@@ -586,11 +600,6 @@ gk_status tc_plan(gk_handle h, const TcProblem& pr_in, bool encode, TcLaunch* ou
     if (pr.epi->activation < GK_ACT_NONE || pr.epi->activation > (pr.form == kTcPlain ? GK_ACT_GELU : GK_ACT_SILU))
       return set_error(GK_ERR_UNSUPPORTED, "activation %d is not one of none/ReLU/GELU", pr.epi->activation);
     p.act = pr.epi->activation;
-  }
-  if (pr.form != kTcPlain) {
-    auto wide = [](const void* q, int64_t ld) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0 && ld % 8 == 0; };
-    p.f.wide = pr.dtype_d != GK_F32 && p.M % 8 == 0 && wide(p.D, pr.d_sn[0]) && p.d_batch % 8 == 0 &&
-               (p.beta == 0.0f || (wide(p.C, pr.c_sn[0]) && p.c_batch % 8 == 0)) && (!p.f.Z || wide(p.f.Z, p.f.z_sn));
   }
   p.status = h->status_dev;
   p.debug = pr.debug;
