@@ -403,6 +403,29 @@ __device__ __forceinline__ void tc_fused_chunk(const TcParams& p, const uint32_t
   }
 }
 
+// FP32 results without activation and Z - weight gradients: D = alpha * AB + bias (+ beta * C, from shared memory).
+// Every warp-uniform decision costs a branch and, behind it, an instruction fetch (about 40 cycles); taken once per
+// chunk instead of once per eight columns they made 537 MB of weight gradients 266 -> 160 us of stores alone.
+__device__ __forceinline__ void tc_plain_chunk(const TcParams& p, const uint32_t (&v)[32], float* d, float bias_row, uint32_t live,
+                                               uint32_t c_row_shared) {
+  const int64_t step = p.d_sn0;
+  float x[32];
+  if (c_row_shared != 0) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) x[j] = fmaf(p.beta, shared_load_f32(c_row_shared + j * 128), fmaf(p.alpha, __uint_as_float(v[j]), bias_row));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) x[j] = fmaf(p.alpha, __uint_as_float(v[j]), bias_row);
+  }
+  if (live == 0xffffffffu) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) { *d = x[j]; d += step; }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) { if ((live >> j) & 1u) *d = x[j]; d += step; }
+  }
+}
+
 // The same for a chunk whose D, C and Z are 16-bit and 16-byte aligned (FusedParams::wide).  A thread owns a row of
 // the accumulator but columns are what is consecutive in memory, so element-wise access moves 64 bytes a request and
 // the 32 requests per array and chunk are what bounds it (8192 x 4096 x 2048 GELU gradient: 207 us).  Here a
@@ -1179,6 +1202,8 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
     [[maybe_unused]] const TcStage stage(
         FORM == kTcPlain ? 0u : ((smem_u32(ctrl_gen) + kTcCtrlBytes + (FORM >= kTcRaggedCols ? tc_table_bytes(p.f.groups) : 0) + 15u) & ~15u) +
                                     (warp - 4) * tc_staging_bytes(p.f.wide), lane);
+    [[maybe_unused]] const bool plain_f32 = FORM != kTcPlain && p.dtype_d == TC_F32 && p.f.form != FUSED_GRADIENT && p.f.Z == nullptr &&
+                                            p.act == TC_ACT_NONE && p.bias_axis != TC_BIAS_COL && (!has_c || p.f.wide == FUSED_WIDE_COPY);
     // plain matrices only (a contraction's C is addressed through two-level strides), planar or real
     pdl_wait();             // D (and C) may still be in use by the previous kernel
     const bool prefetch_c = has_c && p.m_div >= p.M && p.n_div >= p.N && p.c_sm0 == 1 && (PLANES == 1 || p.c_plane != 0);
@@ -1315,7 +1340,9 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
               if (m_ok) {
                 const int64_t ci = c_row + static_cast<int64_t>(col0) * p.c_sn0, di = d_row + static_cast<int64_t>(col0) * p.d_sn0;
                 const int64_t zi = m + static_cast<int64_t>(col0) * p.f.z_sn;
-                if (p.dtype_d == TC_F32)
+                if (plain_f32)
+                  tc_plain_chunk(p, v, static_cast<float*>(p.D) + di, bias_row, live, c_row_shared);
+                else if (p.dtype_d == TC_F32)
                   tc_fused_chunk<float>(p, v, static_cast<float*>(p.D) + di, static_cast<const float*>(p.C) + ci, static_cast<float*>(p.f.Z) + zi,
                                         bias_row, col0, live, c_row_shared);
                 else
@@ -1431,7 +1458,9 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) {
-        if constexpr (CG == 2) mbar_arrive_cluster(tempty_leader + 8u * hb);
+        // (fused forms: the release's wait for this tile's stores cost 18 % of a store-bound product)
+        if constexpr (CG == 2 && FORM != kTcPlain) mbar_arrive_cluster_relaxed(tempty_leader + 8u * hb);
+        else if constexpr (CG == 2) mbar_arrive_cluster(tempty_leader + 8u * hb);
         else mbar_arrive(bar_tempty + 8u * hb);
       }
       }
