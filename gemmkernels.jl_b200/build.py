@@ -21,7 +21,7 @@ LIB_DIR = HERE / "lib"
 LIB_PATH = LIB_DIR / "libgemmkernels_b200.so"
 
 SOURCES = ["tc_kernels_rank3.cu", "tc_kernels_rank5.cu", "api.cu", "tc_plan.cu", "contract.cu", "mgpu.cu", "tc_kernels_generic.cu",
-           "tc_kernels_fused.cu", "fused.cu"]
+           "tc_kernels_fused.cu", "tc_kernels_ragged_cols.cu", "tc_kernels_ragged_depth.cu", "fused.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

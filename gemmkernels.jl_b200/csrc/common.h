@@ -84,7 +84,7 @@ struct gk_handle_s {
   int max_clusters[2][4] = {};     // tc kernel [planes-1][tf32 + 2*rank5] -> co-resident CTA pairs
   bool attr_set[2][2][2][4] = {};  // tc kernel [debug instance][cg-1][planes-1][tf32 + 2*rank5]: smem attribute set
   bool attr_set_generic[2] = {};   // the same for the generic-load instances
-  bool attr_set_fused[3][3] = {};  // layer-level instances [form-1][one CTA, CTA pair, generic loads]
+  bool attr_set_fused[3][3][3] = {};  // layer-level instances [form-1][epilogue][one CTA, CTA pair, generic loads]
   bool fpu_attr_set[12] = {};      // FFMA kernel instances (3 operand types x 4 transposes): shared-memory limit raised
   bool f64_attr_set[4] = {};       // FP64 kernel instances (4 transposes): shared-memory limit raised
   // staging buffers of gk_gemm_host (grown on demand, freed by gk_destroy)

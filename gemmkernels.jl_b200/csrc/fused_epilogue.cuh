@@ -30,13 +30,7 @@ struct FusedParams {
   int32_t groups;
   int32_t total;           // columns there are: offsets are clamped to [0, total]
   int64_t bias_group;      // elements between the biases of consecutive groups
-  int32_t wide;            // tensor-core kernel, FusedWide: how the epilogue moves C, D and Z
 };
-
-// NONE: element by element.  WORDS: D, C and Z are 16-bit, M and all leading dimensions are multiples of 8 and the
-// addresses of 16 bytes: 8 rows of a column per access.  COPY: D and C are FP32, M and C's leading dimension multiples
-// of 4, C 16-byte aligned and Z not read: C comes through shared memory by asynchronous copies, a chunk ahead.
-enum FusedWide : int32_t { FUSED_WIDE_NONE = 0, FUSED_WIDE_WORDS = 1, FUSED_WIDE_COPY = 2 };
 
 // Activations for results of 32 bits, one element.  A NaN passes through all of them.
 __device__ __forceinline__ float fused_max_nan(float a, float b) {

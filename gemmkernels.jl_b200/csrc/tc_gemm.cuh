@@ -54,6 +54,15 @@ enum TcDtype : int32_t { TC_F16 = 0, TC_BF16 = 1, TC_F32 = 2 };
 enum TcAct : int32_t { TC_ACT_NONE = 0, TC_ACT_RELU = 1, TC_ACT_GELU = 2 };
 enum TcBias : int32_t { TC_BIAS_NONE = 0, TC_BIAS_ROW = 1, TC_BIAS_COL = 2 };
 
+// How the epilogue of a layer-level form moves C, D and Z (chosen on the host from types, alignment and epilogue):
+//   kTcWords     16-bit D, C and Z, M and all leading dimensions multiples of 8, addresses of 16 bytes: 8 rows of a
+//                column per access, blocks of 32 x 32 turned in shared memory.  Long per chunk (activations): 16 warps.
+//   kTcFloats    FP32 D without activation and Z; C (M and its leading dimension multiples of 4, 16-byte aligned) comes
+//                through shared memory by asynchronous copies, a chunk ahead
+//   kTcElements  everything else, element by element
+enum TcEpi : int { kTcElements = 0, kTcWords = 1, kTcFloats = 2 };
+__host__ __device__ constexpr int tc_fused_warps(int epi) { return 8; }
+
 enum TcForm : int { kTcPlain = 0, kTcFused = 1, kTcRaggedCols = 2, kTcRaggedDepth = 3 };
 
 // status word values (0 = ok)
@@ -155,8 +164,10 @@ struct TcParams {
 // Group table of the ragged forms, behind the control block: first tile of each group (groups + 1 values), then
 // first and last + 1 column of each.
 constexpr int kTcCtrlBytes = 256;
-// Per epilogue warp of the fused forms, behind the table: a block of 32 x 32 16-bit elements, or two of FP32 ones.
-__host__ __device__ constexpr int tc_staging_bytes(int wide) { return wide == FUSED_WIDE_COPY ? 2 * 32 * 32 * 4 : 32 * 32 * 2; }
+// Per epilogue warp of the layer-level forms, behind the table: a block of 32 x 32 16-bit elements, or two of FP32 ones.
+__host__ __device__ constexpr int tc_staging_bytes(int epi) {
+  return epi == kTcFloats ? 2 * 32 * 32 * 4 : (epi == kTcWords ? 32 * 32 * 2 : 0);
+}
 __host__ __device__ constexpr int tc_table_bytes(int groups) { return (3 * groups + 1) * 4; }
 
 template <int FORM>
@@ -319,8 +330,7 @@ __device__ __forceinline__ void tc_epilogue_chunk(const TcParams& p, const uint3
 }
 
 // Epilogue of up to 32 columns of one row in the fused forms: bit j of `live` says that column j of the chunk exists.
-// d, c and z point at column 0 of the chunk; C and Z have D's type T; c_row_shared != 0: the
-// lane's row of C is in shared memory already (tc_copy_block).  Eight columns at a time: their loads of C
+// d, c and z point at column 0 of the chunk; C and Z have D's type T.  Eight columns at a time: their loads of C
 // and Z are issued before the first use, and what is live fits the 168 registers of a 384-thread CTA.
 // A 16-bit element whose type, Float16 or BFloat16, is a run-time choice: one instance of the element-wise code
 // below serves both (two of them cost 300 bytes of spilled registers a thread).
@@ -335,8 +345,8 @@ template <> __device__ __forceinline__ TcHalfWord tc_put<TcHalfWord>(float x, bo
 }
 
 template <typename T>
-__device__ __forceinline__ void tc_fused_chunk(const TcParams& p, const uint32_t (&v)[32], T* d, const T* c, T* z, float bias_row,
-                                               int col0, uint32_t live, uint32_t c_row_shared = 0) {
+__device__ __forceinline__ void tc_elements_chunk(const TcParams& p, const uint32_t (&v)[32], T* d, const T* c, T* z, float bias_row,
+                                               int col0, uint32_t live) {
   constexpr int W = 8;
   const bool gradient = p.f.form == FUSED_GRADIENT, residual = p.f.form == FUSED_RESIDUAL;
   const bool has_c = p.beta != 0.0f, f16 = p.dtype_d == TC_F16;
@@ -348,19 +358,9 @@ __device__ __forceinline__ void tc_fused_chunk(const TcParams& p, const uint32_t
     auto in = [&](int j) { return (live >> (h + j)) & 1u; };
     T cv[W], zv[W];
     if (has_c) {
-      bool copied = false;
-      if constexpr (sizeof(T) == 4) {
-        if (c_row_shared != 0) {
-          copied = true;
 #pragma unroll
-          for (int j = 0; j < W; ++j) cv[j] = shared_load_f32(c_row_shared + (h + j) * 128);
-        }
-      }
-      if (!copied) {
-#pragma unroll
-        for (int j = 0; j < W; ++j, advance(c, p.c_sn0))
-          if (in(j)) cv[j] = *c;
-      }
+      for (int j = 0; j < W; ++j, advance(c, p.c_sn0))
+        if (in(j)) cv[j] = *c;
     }
     if (gradient) {
 #pragma unroll
@@ -405,8 +405,8 @@ __device__ __forceinline__ void tc_fused_chunk(const TcParams& p, const uint32_t
 
 // FP32 results without activation and Z - weight gradients: D = alpha * AB + bias (+ beta * C, from shared memory).
 // Every warp-uniform decision costs a branch and, behind it, an instruction fetch (about 40 cycles); taken once per
-// chunk instead of once per eight columns they made 537 MB of weight gradients 266 -> 160 us of stores alone.
-__device__ __forceinline__ void tc_plain_chunk(const TcParams& p, const uint32_t (&v)[32], float* d, float bias_row, uint32_t live,
+// chunk instead of once per eight columns they made the stores of 537 MB of weight gradients 266 -> 131 us.
+__device__ __forceinline__ void tc_floats_chunk(const TcParams& p, const uint32_t (&v)[32], float* d, float bias_row, uint32_t live,
                                                uint32_t c_row_shared) {
   const int64_t step = p.d_sn0;
   float x[32];
@@ -426,7 +426,7 @@ __device__ __forceinline__ void tc_plain_chunk(const TcParams& p, const uint32_t
   }
 }
 
-// The same for a chunk whose D, C and Z are 16-bit and 16-byte aligned (FusedParams::wide).  A thread owns a row of
+// The same for a chunk whose D, C and Z are 16-bit and 16-byte aligned (kTcWords).  A thread owns a row of
 // the accumulator but columns are what is consecutive in memory, so element-wise access moves 64 bytes a request and
 // the 32 requests per array and chunk are what bounds it (8192 x 4096 x 2048 GELU gradient: 207 us).  Here a
 // lane moves 8 rows of a column (16 bytes; a request is 8 columns of 64 bytes) and the warp turns the 32 x 32 block
@@ -450,7 +450,7 @@ struct TcStage {
   __device__ __forceinline__ uint32_t mat_slot(int s) const { return mat + ((s ^ mat_key) << 4); }
 };
 
-// FUSED_WIDE_COPY: starts the copies of the 32 x 32 block of C at rows m0, columns col0 into `buf` (columns of 128 bytes),
+// kTcFloats: starts the copies of the 32 x 32 block of C at rows m0, columns col0 into `buf` (columns of 128 bytes),
 // eight 16-byte pieces per lane.
 __device__ __forceinline__ void tc_copy_block(const TcParams& p, uint32_t buf, const float* c_col0, int m0, int64_t c_step, uint32_t live,
                                               int lane) {
@@ -544,8 +544,8 @@ __device__ __forceinline__ void tc_wide_act(float2 (&x)[16]) {
 
 // One chunk: `w` was loaded with tc_wide_load from Z (GRADIENT form) or else from C; c, d and z point at the lane's 8
 // rows of column i / 4.  All lanes of the warp call.
-template <typename T>
-__device__ __forceinline__ void tc_wide_chunk(const TcParams& p, const uint32_t (&v)[32], uint4 (&w)[4], const uint16_t* c, uint16_t* d,
+template <typename T, int FORM>
+__device__ __forceinline__ void tc_words_chunk(const TcParams& p, const uint32_t (&v)[32], uint4 (&w)[4], const uint16_t* c, uint16_t* d,
                                               uint16_t* z, float bias_row, int col0, uint32_t live, uint32_t live_lane,
                                               const TcStage& st) {
   const bool has_c = p.beta != 0.0f;
@@ -553,14 +553,19 @@ __device__ __forceinline__ void tc_wide_chunk(const TcParams& p, const uint32_t 
 #pragma unroll
   for (int i = 0; i < 16; ++i)
     x[i] = __ffma2_rn(fused_2(p.alpha), make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), fused_2(bias_row));
-  if (p.bias_axis == TC_BIAS_COL) {
+  if (FORM == kTcFused && p.bias_axis == TC_BIAS_COL) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       if ((live >> (2 * i)) & 1u) x[i].x += p.bias[col0 + 2 * i];
       if ((live >> (2 * i + 1)) & 1u) x[i].y += p.bias[col0 + 2 * i + 1];
     }
   }
-  if (p.f.form == FUSED_GRADIENT) {
+  if constexpr (FORM == kTcRaggedDepth) {      // alpha, beta and C only
+    if (has_c) {
+      tc_wide_to_row(w, st);
+      tc_wide_add<T>(x, p.beta, w);
+    }
+  } else if (p.f.form == FUSED_GRADIENT) {
     if (has_c) {
       uint4 cw[4];
       tc_wide_load(cw, c, p.c_sn0, live_lane);
@@ -682,11 +687,13 @@ __device__ __forceinline__ void tc_issue_kblock(uint32_t lo, bool first, uint32_
 // DBG selects the instance that honours TcParams::debug (measurement and test aids); in the production
 // instance every such branch is compiled out, which shortens the per-stage loops of the producer and
 // MMA warps (their cost per pipeline stage is instruction latency, not bandwidth).
-template <int CG, int PLANES, bool TF32, bool RANK5, bool GENERIC = false, bool DBG = false, int FORM = kTcPlain>
-__global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __grid_constant__ TcParams p) {
+template <int CG, int PLANES, bool TF32, bool RANK5, bool GENERIC = false, bool DBG = false, int FORM = kTcPlain, int EPI = kTcElements>
+__global__ void __launch_bounds__(FORM == kTcPlain ? tc_threads(PLANES) : 128 + 32 * tc_fused_warps(EPI), 1)
+    tc_gemm_kernel(const __grid_constant__ TcParams p) {
   const int dbg = DBG ? p.debug : 0;
   static_assert(!GENERIC || (CG == 1 && PLANES == 1 && !TF32 && !RANK5), "generic loads: one CTA, one plane, 16-bit types");
   static_assert(FORM == kTcPlain || (PLANES == 1 && !TF32 && !RANK5 && !DBG), "fused forms: one plane, 16-bit types");
+  constexpr int kEpiWarps = FORM == kTcPlain ? tc_epilogue_warps(PLANES) : tc_fused_warps(EPI);
   extern __shared__ uint8_t smem_raw[];
   // 128-byte swizzle atoms are 1024 bytes and the pattern is a function of the address.
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -725,7 +732,7 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(bar_tfull + 8u * a, 1);
-      mbar_init(bar_tempty + 8u * a, tc_epilogue_warps(PLANES) * CG);  // one arrival per epilogue warp per CTA
+      mbar_init(bar_tempty + 8u * a, kEpiWarps * CG);  // one arrival per epilogue warp per CTA
     }
     mbar_init(bar_drain, 1);
     *abort_flag = 0;
@@ -1189,7 +1196,7 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
   } else if (warp >= 4) {
     // ------------------------------------------------------------------ epilogue
     const int q = warp & 3;                 // TMEM lane quarter this warp may read
-    const int chunk_step = 32 * (tc_epilogue_warps(PLANES) / 4);
+    const int chunk_step = 32 * (kEpiWarps / 4);
     const int chunk_first = 32 * ((warp - 4) >> 2);
     const uint32_t tempty_leader = (CG == 2) ? map_to_cta(bar_tempty, 0) : bar_tempty;
     uint32_t acc_it = 0;
@@ -1201,9 +1208,7 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
     const bool has_c = p.beta != 0.0f;
     [[maybe_unused]] const TcStage stage(
         FORM == kTcPlain ? 0u : ((smem_u32(ctrl_gen) + kTcCtrlBytes + (FORM >= kTcRaggedCols ? tc_table_bytes(p.f.groups) : 0) + 15u) & ~15u) +
-                                    (warp - 4) * tc_staging_bytes(p.f.wide), lane);
-    [[maybe_unused]] const bool plain_f32 = FORM != kTcPlain && p.dtype_d == TC_F32 && p.f.form != FUSED_GRADIENT && p.f.Z == nullptr &&
-                                            p.act == TC_ACT_NONE && p.bias_axis != TC_BIAS_COL && (!has_c || p.f.wide == FUSED_WIDE_COPY);
+                                    (warp - 4) * tc_staging_bytes(EPI), lane);
     // plain matrices only (a contraction's C is addressed through two-level strides), planar or real
     pdl_wait();             // D (and C) may still be in use by the previous kernel
     const bool prefetch_c = has_c && p.m_div >= p.M && p.n_div >= p.N && p.c_sm0 == 1 && (PLANES == 1 || p.c_plane != 0);
@@ -1275,20 +1280,20 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
       [[maybe_unused]] uint4 fetched[4];
       [[maybe_unused]] auto fetch = [&](int c, uint32_t into, uint4 (&w)[4]) {
         const uint32_t live = live_of(c);
-        if (p.f.wide == FUSED_WIDE_COPY) {
-          tc_copy_block(p, stage.base + into, static_cast<const float*>(p.C) + c_row - lane + static_cast<int64_t>(n0 + c) * p.c_sn0, m0,
+        if constexpr (EPI == kTcFloats) {
+          if (has_c) tc_copy_block(p, stage.base + into, static_cast<const float*>(p.C) + c_row - lane + static_cast<int64_t>(n0 + c) * p.c_sn0, m0,
                         p.c_sn0, live, lane);
-        } else {
+        } else if constexpr (EPI == kTcWords) {
           const uint32_t live_lane = m0 + r8 < p.M ? live >> lc : 0u;
           const int64_t corner = n0 + c + lc;
-          if (p.f.form == FUSED_GRADIENT) tc_wide_load(w, static_cast<const uint16_t*>(p.f.Z) + m0 + r8 + corner * p.f.z_sn, p.f.z_sn, live_lane);
+          if (FORM != kTcRaggedDepth && p.f.form == FUSED_GRADIENT) tc_wide_load(w, static_cast<const uint16_t*>(p.f.Z) + m0 + r8 + corner * p.f.z_sn, p.f.z_sn, live_lane);
           else if (has_c) tc_wide_load(w, c_word + corner * p.c_sn0, p.c_sn0, live_lane);
         }
       };
       if constexpr (FORM != kTcPlain) {
-        if (p.f.wide != FUSED_WIDE_NONE && c_lo < c_hi) {
+        if (EPI != kTcElements && c_lo < c_hi) {
           fetch(c_lo, 0u, fetched);
-          if (p.f.wide == FUSED_WIDE_COPY) async_copy_commit();
+          if (EPI == kTcFloats) async_copy_commit();
         }
       }
       // all-or-nothing per warp: the TMEM loads below are warp-collective
@@ -1308,12 +1313,8 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
           const uint32_t live = live_of(c);
           const int col0 = n0 + c;
           [[maybe_unused]] uint4 ahead[4];
-          if (p.f.wide == FUSED_WIDE_COPY) {
-            if (c + chunk_step < c_hi) fetch(c + chunk_step, buf ^ 4096u, ahead);
-            async_copy_commit();
-          } else if (p.f.wide == FUSED_WIDE_WORDS && c + chunk_step < c_hi) {
-            fetch(c + chunk_step, 0u, ahead);
-          }
+          if (EPI != kTcElements && c + chunk_step < c_hi) fetch(c + chunk_step, buf ^ 4096u, ahead);
+          if (EPI == kTcFloats) async_copy_commit();
           if (live != 0u) {                                  // the same for the whole warp
             const uint32_t t_col = t_row + (c >= p.bn ? sub_cols + (c - p.bn) : c);
             uint32_t v[32];
@@ -1323,38 +1324,34 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
 #pragma unroll
               for (int j = 0; j < 32; ++j) v[j] = 0u;
             }
-            if (p.f.wide == FUSED_WIDE_WORDS) {
+            const int64_t di = d_row + static_cast<int64_t>(col0) * p.d_sn0;
+            if constexpr (EPI == kTcWords) {
               const uint32_t live_lane = m0 + r8 < p.M ? live >> lc : 0u;
-              const int64_t corner = col0 + lc;
-              uint16_t* zp = static_cast<uint16_t*>(p.f.Z) + m0 + r8 + corner * p.f.z_sn;
-              uint16_t* dp = static_cast<uint16_t*>(p.D) + d_row + back + corner * p.d_sn0;
-              if (p.dtype_d == TC_F16) tc_wide_chunk<__half>(p, v, fetched, c_word + corner * p.c_sn0, dp, zp, bias_row, col0, live, live_lane, stage);
-              else tc_wide_chunk<__nv_bfloat16>(p, v, fetched, c_word + corner * p.c_sn0, dp, zp, bias_row, col0, live, live_lane, stage);
-            } else {
-              uint32_t c_row_shared = 0;
-              if (p.f.wide == FUSED_WIDE_COPY) {
-                async_copy_wait<1>();
-                __syncwarp();
-                c_row_shared = stage.base + buf + 4 * lane;
-              }
-              if (m_ok) {
-                const int64_t ci = c_row + static_cast<int64_t>(col0) * p.c_sn0, di = d_row + static_cast<int64_t>(col0) * p.d_sn0;
-                const int64_t zi = m + static_cast<int64_t>(col0) * p.f.z_sn;
-                if (plain_f32)
-                  tc_plain_chunk(p, v, static_cast<float*>(p.D) + di, bias_row, live, c_row_shared);
-                else if (p.dtype_d == TC_F32)
-                  tc_fused_chunk<float>(p, v, static_cast<float*>(p.D) + di, static_cast<const float*>(p.C) + ci, static_cast<float*>(p.f.Z) + zi,
-                                        bias_row, col0, live, c_row_shared);
-                else
-                  tc_fused_chunk<TcHalfWord>(p, v, static_cast<TcHalfWord*>(p.D) + di, static_cast<const TcHalfWord*>(p.C) + ci,
-                                             static_cast<TcHalfWord*>(p.f.Z) + zi, bias_row, col0, live);
-              }
+              uint16_t* zp = static_cast<uint16_t*>(p.f.Z) + m0 + r8 + (col0 + lc) * p.f.z_sn;
+              uint16_t* dp = static_cast<uint16_t*>(p.D) + di + back + lc * p.d_sn0;
+              const uint16_t* cp = c_word + (col0 + lc) * p.c_sn0;
+              if (p.dtype_d == TC_F16) tc_words_chunk<__half, FORM>(p, v, fetched, cp, dp, zp, bias_row, col0, live, live_lane, stage);
+              else tc_words_chunk<__nv_bfloat16, FORM>(p, v, fetched, cp, dp, zp, bias_row, col0, live, live_lane, stage);
+            } else if constexpr (EPI == kTcFloats) {
+              async_copy_wait<1>();
+              __syncwarp();
+              if (m_ok) tc_floats_chunk(p, v, static_cast<float*>(p.D) + di, bias_row, live, has_c ? stage.base + buf + 4 * lane : 0u);
+            } else if (m_ok) {
+              const int64_t ci = c_row + static_cast<int64_t>(col0) * p.c_sn0, zi = m + static_cast<int64_t>(col0) * p.f.z_sn;
+              if (p.dtype_d == TC_F32)
+                tc_elements_chunk<float>(p, v, static_cast<float*>(p.D) + di, static_cast<const float*>(p.C) + ci,
+                                         static_cast<float*>(p.f.Z) + zi, bias_row, col0, live);
+              else
+                tc_elements_chunk<TcHalfWord>(p, v, static_cast<TcHalfWord*>(p.D) + di, static_cast<const TcHalfWord*>(p.C) + ci,
+                                              static_cast<TcHalfWord*>(p.f.Z) + zi, bias_row, col0, live);
             }
           }
-          __syncwarp();                                      // the buffer just read is filled again in the next round
+          if (EPI == kTcFloats) __syncwarp();                // the buffer just read is filled again in the next round
           buf ^= 4096u;
+          if constexpr (EPI == kTcWords) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) fetched[i] = ahead[i];
+            for (int i = 0; i < 4; ++i) fetched[i] = ahead[i];
+          }
           continue;
         }
         uint32_t v[PLANES][32];
@@ -1472,7 +1469,7 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
         p.dbg_out[blockIdx.x * 16 + 15] = static_cast<long long>(global_timer_ns());   // last tile stored
       }
     }
-    if constexpr (FORM != kTcPlain) async_copy_wait<0>();   // (only a loop that was left early has copies in flight)
+    if constexpr (FORM != kTcPlain && EPI == kTcFloats) async_copy_wait<0>();   // (only a loop that was left early has copies in flight)
   }
 
   // ------------------------------------------------------------------ teardown

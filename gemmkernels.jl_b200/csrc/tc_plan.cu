@@ -153,7 +153,16 @@ extern template const void* tc_kernel_select_r<false>(int cg, int planes, bool t
 extern template const void* tc_kernel_select_r<true>(int cg, int planes, bool tf32, bool dbg);
 
 const void* tc_kernel_generic(bool dbg);   // tc_kernels_generic.cu: <1, 1, false, false, GENERIC, dbg>
-const void* tc_kernel_fused(int form, int cg, bool generic);   // tc_kernels_fused.cu: the layer-level forms
+// the layer-level forms, one translation unit each (tc_kernels_fused.cu, _ragged_cols.cu, _ragged_depth.cu)
+template <int FORM> const void* tc_kernel_form(int epi, int cg, bool generic);
+extern template const void* tc_kernel_form<kTcFused>(int epi, int cg, bool generic);
+extern template const void* tc_kernel_form<kTcRaggedCols>(int epi, int cg, bool generic);
+extern template const void* tc_kernel_form<kTcRaggedDepth>(int epi, int cg, bool generic);
+static const void* tc_kernel_fused(int form, int epi, int cg, bool generic) {
+  return form == kTcFused        ? tc_kernel_form<kTcFused>(epi, cg, generic)
+         : form == kTcRaggedCols ? tc_kernel_form<kTcRaggedCols>(epi, cg, generic)
+                                 : tc_kernel_form<kTcRaggedDepth>(epi, cg, generic);
+}
 
 // dbg: the instance that honours the descriptor's diagnostic bits (the production instance compiles them out)
 static const void* tc_kernel_select(int cg, int planes, bool tf32, bool rank5, bool dbg) {
@@ -526,15 +535,17 @@ gk_status tc_plan(gk_handle h, const TcProblem& pr_in, bool encode, TcLaunch* ou
       return (reinterpret_cast<uintptr_t>(q) & 15) == 0 && ld % unit == 0 && batch % unit == 0;
     };
     const bool reads_c = pr.C != nullptr && pr.beta != 0.0;
-    p.f.wide = FUSED_WIDE_NONE;
+    const gk_epilogue_desc* e = pr.epi;
+    out->epi = kTcElements;
     if (pr.dtype_d != GK_F32) {
       if (p.M % 8 == 0 && wide(pr.D, pr.d_sn[0], pr.batch_d, 8) && (!reads_c || wide(pr.C, pr.c_sn[0], pr.batch_c, 8)) &&
           (!p.f.Z || wide(p.f.Z, p.f.z_sn, 0, 8)))
-        p.f.wide = FUSED_WIDE_WORDS;
-    } else if (reads_c && p.f.form != FUSED_GRADIENT && p.M % 4 == 0 && wide(pr.C, pr.c_sn[0], pr.batch_c, 4)) {
-      p.f.wide = FUSED_WIDE_COPY;
+        out->epi = kTcWords;
+    } else if (!p.f.Z && !(e && (e->activation != GK_ACT_NONE || e->bias_axis == GK_BIAS_COL)) &&
+               (!reads_c || (p.M % 4 == 0 && wide(pr.C, pr.c_sn[0], pr.batch_c, 4)))) {
+      out->epi = kTcFloats;
     }
-    table_bytes = (pr.form >= kTcRaggedCols ? tc_table_bytes(pr.f.groups) : 0) + 16 + tc_epilogue_warps(1) * tc_staging_bytes(p.f.wide);
+    table_bytes = (pr.form >= kTcRaggedCols ? tc_table_bytes(pr.f.groups) : 0) + 16 + tc_fused_warps(out->epi) * tc_staging_bytes(out->epi);
   }
   const int kSmemBudget = kSmemMax - table_bytes;
   const int kblock_bytes = stage_bytes_for(cg, bn, n_sub, planes, planes);
@@ -618,7 +629,7 @@ gk_status tc_plan(gk_handle h, const TcProblem& pr_in, bool encode, TcLaunch* ou
   // SM impossible, so two CTA pairs can never each hold one SM's tensor memory and wait for the other's.
   out->smem_bytes = std::max(out->smem_bytes, kSmemMax / 2 + 2048);
   const bool dbg = pr.debug != 0;
-  out->kernel = pr.form != kTcPlain ? tc_kernel_fused(pr.form, cg, pr.generic)
+  out->kernel = pr.form != kTcPlain ? tc_kernel_fused(pr.form, out->epi, cg, pr.generic)
                 : pr.generic        ? tc_kernel_generic(dbg)
                                     : tc_kernel_select(cg, planes, tf32, pr.rank5, dbg);
   if (pr.generic) {
@@ -638,7 +649,7 @@ gk_status tc_plan(gk_handle h, const TcProblem& pr_in, bool encode, TcLaunch* ou
   int slots;
   {
     std::lock_guard<std::mutex> lock(h->mu);
-    bool& set = pr.form != kTcPlain ? h->attr_set_fused[pr.form - 1][pr.generic ? 2 : cg - 1]
+    bool& set = pr.form != kTcPlain ? h->attr_set_fused[pr.form - 1][out->epi][pr.generic ? 2 : cg - 1]
                 : pr.generic        ? h->attr_set_generic[dbg ? 1 : 0]
                            : h->attr_set[dbg ? 1 : 0][cg - 1][planes - 1][(tf32 ? 1 : 0) + (pr.rank5 ? 2 : 0)];
     if (!set) {
@@ -648,11 +659,12 @@ gk_status tc_plan(gk_handle h, const TcProblem& pr_in, bool encode, TcLaunch* ou
     if (cg == 1) {
       slots = h->sm_count;
     } else {
+      // (the layer-level forms, like every tcgen05 kernel, run one CTA per SM: the same pairs fit)
       int& cached = h->max_clusters[planes - 1][(tf32 ? 1 : 0) + (pr.rank5 ? 2 : 0)];
       if (cached == 0) {
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3(2 * (h->sm_count / 2));
-        cfg.blockDim = dim3(tc_threads(planes));
+        cfg.blockDim = dim3(tc_launch_threads(*out));
         cfg.dynamicSmemBytes = kSmemMax;
         cudaLaunchAttribute at{};
         at.id = cudaLaunchAttributeClusterDimension;
@@ -716,7 +728,7 @@ gk_status tc_write_depth_maps(TcLaunch* L, void* workspace, cudaStream_t stream)
 gk_status tc_launch(const TcLaunch& L, cudaStream_t stream) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(L.grid);
-  cfg.blockDim = dim3(tc_threads(L.planes));
+  cfg.blockDim = dim3(tc_launch_threads(L));
   cfg.dynamicSmemBytes = L.smem_bytes;
   cfg.stream = stream;
   cudaLaunchAttribute at[2]{};

@@ -60,10 +60,12 @@ struct TcLaunch {
   const void* kernel = nullptr;
   int cg = 1, planes = 1;
   bool tf32 = false, rank5 = false, generic = false;
-  int form = kTcPlain;
+  int form = kTcPlain, epi = kTcElements;
   int grid = 0;
   int smem_bytes = 0;
 };
+
+inline int tc_launch_threads(const TcLaunch& L) { return L.form == kTcPlain ? tc_threads(L.planes) : 128 + 32 * tc_fused_warps(L.epi); }
 
 // True when the descriptor (and, if given, the operand addresses) can go through TMA + tcgen05.
 bool tc_eligible(const gk_gemm_desc& d, const void* a, const void* b, std::string* why);
