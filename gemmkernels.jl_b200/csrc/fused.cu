@@ -6,6 +6,7 @@
 #include <cstring>
 
 #include "activation_gradient.cuh"
+#include "align_operand.cuh"
 #include "common.h"
 #include "skinny_gemm.cuh"
 #include "tc_plan.h"
@@ -107,34 +108,67 @@ static void fused_problem(const gk_gemm_desc& d, const gk_fused_desc& fu, const 
   }
 }
 
-// TMA, or the bounds-checked loads of the generic instances.
-static bool fused_tma(const gk_gemm_desc& d, const gk_group_desc* gr, const void* a, const void* b) {
-  gk_gemm_desc e = d;
-  e.k = std::max<int64_t>(e.k, 1);
-  if (!tc_eligible(e, a, b, nullptr)) return false;
-  if (!gr) return true;
-  if (gr->ragged == GK_RAGGED_COLUMNS) return gr->groups <= 1 || (gr->stride_a * dtype_size(d.dtype_a)) % 16 == 0;
-  // The run of K of a group may start anywhere: TMA takes any start along the strided index only.
-  return d.trans_a == 0 && d.trans_b != 0;
+// How a tensor-core product gets at its operands.  TMA takes 16-byte aligned columns (and, along a ragged depth, only
+// operands whose K is the strided index: a group's run may start anywhere); an operand that is not aligned is copied
+// with padded columns into the workspace first.  Without the room for that, or with the wrong order along a ragged depth,
+// the generic instances read the operands with bounds-checked loads.
+struct OperandCopy { bool copy = false; int64_t rows = 0, cols = 0, ld = 0, group = 0, bytes = 0; int32_t groups = 1; };
+struct FusedFeed {
+  bool possible = true;            // TMA can be used once the copies are made
+  OperandCopy a, b;
+  int64_t bytes() const { return a.bytes + b.bytes; }
+};
+
+static FusedFeed fused_feed(const gk_gemm_desc& d, const gk_group_desc* gr, const void* a, const void* b) {
+  FusedFeed f;
+  if (gr && gr->ragged == GK_RAGGED_DEPTH && (d.trans_a || !d.trans_b)) { f.possible = false; return f; }
+  if (d.k < 1 || d.alpha == 0.0) return f;      // nothing is loaded
+  const bool cols = gr && gr->ragged == GK_RAGGED_COLUMNS;
+  auto plan = [&](OperandCopy& c, const void* p, int64_t ld, bool trans, int64_t mn, bool is_a) {
+    const int64_t stride = is_a && cols && gr->groups > 1 ? gr->stride_a : 0;
+    c.copy = (reinterpret_cast<uintptr_t>(p) & 15) || ld % 8 || stride % 8;
+    if (!c.copy) return;
+    // stored rows x columns: op(A) is M x K, op(B) is K x N
+    c.rows = trans == is_a ? d.k : mn; c.cols = trans == is_a ? mn : d.k;
+    c.ld = (c.rows + 7) / 8 * 8; c.groups = stride > 0 ? gr->groups : 1; c.group = c.ld * c.cols;
+    c.bytes = (c.group * c.groups * 2 + 255) / 256 * 256;
+  };
+  plan(f.a, a, d.lda, d.trans_a != 0, d.m, true);
+  plan(f.b, b, d.ldb, d.trans_b != 0, d.n, false);
+  return f;
+}
+
+static gk_status launch_copy(gk_handle h, const OperandCopy& c, const void* src, int64_t ld, int64_t stride, void* dst, const FusedParams& f,
+                             bool skip_empty, cudaStream_t stream) {
+  AlignParams p{};
+  p.src = static_cast<const uint16_t*>(src); p.dst = static_cast<uint16_t*>(dst);
+  p.ld = ld; p.group = c.groups > 1 ? stride : 0; p.ld_dst = c.ld; p.group_dst = c.group;
+  p.rows = static_cast<int32_t>(c.rows); p.cols = static_cast<int32_t>(c.cols);
+  p.skip_empty = skip_empty ? 1 : 0;
+  p.f = f;
+  const int per_block = kAlignThreads / 32;
+  const int64_t want = std::max<int64_t>(1, 16 * static_cast<int64_t>(h->sm_count) / c.groups);
+  const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((c.cols + per_block - 1) / per_block, want));
+  GK_CUDA_CHECK(launch_dependent(&align_operand_kernel, dim3(blocks, static_cast<unsigned>(c.groups)), dim3(kAlignThreads), 0, stream, p));
+  return GK_OK;
 }
 
 // ------------------------------------------------------------------------------------------------
 // a few columns: the streaming kernel
 // ------------------------------------------------------------------------------------------------
-struct SkinnyPlan { int nt = 0, ranks = 1, items = 0, rows = 0, k_per_rank = 0; };
+struct SkinnyPlan { int nt = 0, ranks = 1, items = 0, rows = 0, k_per_rank = 0; bool any = false; };
 
 static bool skinny_plan(gk_handle h, const gk_gemm_desc& d, const gk_group_desc* gr, const void* a, const void* b, SkinnyPlan* out) {
   if (gr && gr->ragged != GK_RAGGED_COLUMNS) return false;
   if (d.tile_n || d.cta_group || d.stages || d.max_ctas) return false;      // a tensor-core tile was asked for
-  if (d.trans_b || d.k < 1 || d.alpha == 0.0 || d.n < 1 || d.m < 1) return false;
-  const int es = 2;
-  auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
-  if (!al(a) || !al(b) || (d.lda * es) % 16 || (d.ldb * es) % 16 || d.k % 8 || (!d.trans_a && d.m % 8)) return false;
+  if (d.k < 1 || d.alpha == 0.0 || d.n < 1 || d.m < 1) return false;
   const int64_t groups = gr ? gr->groups : 1;
-  if (gr && groups > 1 && (gr->stride_a * es) % 16) return false;
   const int64_t active = std::min<int64_t>(groups, d.n);
   if (d.n > 4 * active || d.n > 4096) return false;
   SkinnyPlan p;
+  auto al = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
+  p.any = !al(a) || !al(b) || d.lda % 8 || d.ldb % 8 || d.k % 8 || (!d.trans_a && d.m % 8) || d.trans_b ||
+          (gr && groups > 1 && gr->stride_a % 8);
   p.nt = d.n <= 1 ? 1 : (d.n <= 2 * active ? 2 : 4);
   p.items = static_cast<int>(std::min<int64_t>(d.n, d.n / p.nt + active));
   if (groups == 1) p.items = static_cast<int>((d.n + p.nt - 1) / p.nt);
@@ -147,14 +181,17 @@ static bool skinny_plan(gk_handle h, const gk_gemm_desc& d, const gk_group_desc*
   return true;
 }
 
+template <typename T, bool K_MAJOR, bool ANY>
+static const void* skinny_kernel_nt(int nt) {
+  return nt == 1   ? reinterpret_cast<const void*>(&skinny_gemm_kernel<T, K_MAJOR, 1, ANY>)
+         : nt == 2 ? reinterpret_cast<const void*>(&skinny_gemm_kernel<T, K_MAJOR, 2, ANY>)
+                   : reinterpret_cast<const void*>(&skinny_gemm_kernel<T, K_MAJOR, 4, ANY>);
+}
+
 template <typename T>
-static const void* skinny_kernel(bool k_major, int nt) {
-  if (k_major) return nt == 1 ? reinterpret_cast<const void*>(&skinny_gemm_kernel<T, true, 1>)
-                      : nt == 2 ? reinterpret_cast<const void*>(&skinny_gemm_kernel<T, true, 2>)
-                                : reinterpret_cast<const void*>(&skinny_gemm_kernel<T, true, 4>);
-  return nt == 1 ? reinterpret_cast<const void*>(&skinny_gemm_kernel<T, false, 1>)
-         : nt == 2 ? reinterpret_cast<const void*>(&skinny_gemm_kernel<T, false, 2>)
-                   : reinterpret_cast<const void*>(&skinny_gemm_kernel<T, false, 4>);
+static const void* skinny_kernel(bool k_major, bool any, int nt) {
+  if (k_major) return any ? skinny_kernel_nt<T, true, true>(nt) : skinny_kernel_nt<T, true, false>(nt);
+  return any ? skinny_kernel_nt<T, false, true>(nt) : skinny_kernel_nt<T, false, false>(nt);
 }
 
 static gk_status launch_skinny(const SkinnyPlan& sp, const gk_gemm_desc& d, const gk_fused_desc& fu, const gk_group_desc* gr,
@@ -162,7 +199,8 @@ static gk_status launch_skinny(const SkinnyPlan& sp, const gk_gemm_desc& d, cons
   SkinnyParams p{};
   p.A = a; p.B = b; p.C = c; p.D = dd;
   p.M = static_cast<int32_t>(d.m); p.K = static_cast<int32_t>(d.k);
-  p.lda = d.lda; p.ldb = d.ldb; p.ldc = d.ldc; p.ldd = d.ldd;
+  p.lda = d.lda; p.ldc = d.ldc; p.ldd = d.ldd;
+  p.b_sk = d.trans_b ? d.ldb : 1; p.b_sn = d.trans_b ? 1 : d.ldb;
   p.a_group = gr ? gr->stride_a : 0;
   p.alpha = static_cast<float>(d.alpha);
   p.beta = d.layout_c == GK_LAYOUT_DENSE ? static_cast<float>(d.beta) : 0.0f;
@@ -181,7 +219,8 @@ static gk_status launch_skinny(const SkinnyPlan& sp, const gk_gemm_desc& d, cons
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at; cfg.numAttrs = 2;
   void* args[1] = {&p};
-  const void* kernel = d.dtype_a == GK_F16 ? skinny_kernel<__half>(d.trans_a != 0, sp.nt) : skinny_kernel<__nv_bfloat16>(d.trans_a != 0, sp.nt);
+  const void* kernel = d.dtype_a == GK_F16 ? skinny_kernel<__half>(d.trans_a != 0, sp.any, sp.nt)
+                                            : skinny_kernel<__nv_bfloat16>(d.trans_a != 0, sp.any, sp.nt);
   GK_CUDA_CHECK(cudaLaunchKernelExC(&cfg, kernel, args));
   return GK_OK;
 }
@@ -261,7 +300,8 @@ gk_status gk_gemm_fused_query(gk_handle h, const gk_gemm_desc* desc, const gk_fu
   gk_epilogue_desc epi{sizeof(gk_epilogue_desc), fused->bias_axis, fused->bias, fused->activation, {0, 0, 0}};
   TcProblem pr;
   fused_problem(*desc, *fused, groups, &epi, nullptr, nullptr, nullptr, nullptr, &pr);
-  pr.generic = !fused_tma(*desc, groups, nullptr, nullptr);
+  const FusedFeed feed = fused_feed(*desc, groups, nullptr, nullptr);
+  pr.generic = !feed.possible;
   TcLaunch L;
   if ((s = tc_plan(h, pr, false, &L)) != GK_OK) return s;
   if (plan->kernel == 0) {
@@ -269,7 +309,7 @@ gk_status gk_gemm_fused_query(gk_handle h, const gk_gemm_desc* desc, const gk_fu
     plan->smem_bytes = L.smem_bytes; plan->tmem_columns = static_cast<int32_t>(L.params.tmem_cols);
     plan->tile_m = kTcTileM * L.cg; plan->tile_n = L.params.bn * L.params.n_sub; plan->tile_k = L.params.bk * L.params.kps;
     plan->stages = L.params.stages;
-    plan->workspace_bytes = pr.form == kTcFused && pr.K > 0 ? tc_split_workspace_bytes(h, pr, L) : tc_depth_maps_bytes(L);
+    plan->workspace_bytes = feed.bytes() + (pr.form == kTcFused && pr.K > 0 ? tc_split_workspace_bytes(h, pr, L) : tc_depth_maps_bytes(L));
   }
   return GK_OK;
 }
@@ -292,7 +332,25 @@ gk_status gk_gemm_fused(gk_handle h, const gk_gemm_desc* desc, const gk_fused_de
   fused_problem(*desc, *fused, groups, &epi, a, b, desc->beta != 0.0 ? c : nullptr, d, &pr);
   SkinnyPlan sp;
   if (skinny_plan(h, *desc, groups, a, b, &sp)) return launch_skinny(sp, *desc, *fused, groups, pr, a, b, c, d, st);
-  pr.generic = !fused_tma(*desc, groups, a, b);
+  const FusedFeed feed = fused_feed(*desc, groups, a, b);
+  const int64_t copies = feed.bytes();
+  pr.generic = !feed.possible || (copies > 0 && (workspace_bytes < copies || (reinterpret_cast<uintptr_t>(workspace) & 255)));
+  if (!pr.generic && copies > 0) {
+    char* ws = static_cast<char*>(workspace);
+    gk_gemm_desc e = *desc;
+    gk_group_desc eg;
+    if (groups) eg = *groups;
+    if (feed.a.copy) {
+      if ((s = launch_copy(h, feed.a, a, desc->lda, groups ? groups->stride_a : 0, ws, pr.f, feed.a.groups > 1, st)) != GK_OK) return s;
+      a = ws; e.lda = feed.a.ld; eg.stride_a = feed.a.groups > 1 ? feed.a.group : 0;
+    }
+    if (feed.b.copy) {
+      if ((s = launch_copy(h, feed.b, b, desc->ldb, 0, ws + feed.a.bytes, pr.f, false, st)) != GK_OK) return s;
+      b = ws + feed.a.bytes; e.ldb = feed.b.ld;
+    }
+    workspace = ws + copies; workspace_bytes -= copies;
+    fused_problem(e, *fused, groups ? &eg : nullptr, &epi, a, b, desc->beta != 0.0 ? c : nullptr, d, &pr);
+  }
   TcLaunch L;
   if ((s = tc_plan(h, pr, true, &L)) != GK_OK) return s;
   if (pr.form == kTcFused) return pr.K > 0 ? tc_run(h, pr, L, workspace, workspace_bytes, st) : tc_launch(L, st);

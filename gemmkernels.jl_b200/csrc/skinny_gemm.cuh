@@ -13,7 +13,11 @@
 //   M_MAJOR  (A stored with consecutive rows): 8 lanes own 8 rows each; the other 32 slots of the CTA (4 per warp)
 //            take 8 consecutive k each
 // Either way a thread has eight 16-byte loads of A in flight and 8 x NT accumulators.
+//
+// ANY drops the conditions of the plain form (K, and for M_MAJOR also M, a multiple of 8; every address 16-byte aligned; B
+// with consecutive k): eight elements are cut from two 16-byte granules, what lies behind K is zeroed.
 #pragma once
+#include "any_load.cuh"
 #include "fused_epilogue.cuh"
 #include "ptx.cuh"
 
@@ -26,7 +30,7 @@ constexpr int kSkinnyStep = 256;       // K consumed per step of a CTA (K runs a
 struct SkinnyParams {
   const void* A; const void* B; const void* C; void* D;
   int32_t M, K;
-  int64_t lda, ldb, ldc, ldd;
+  int64_t lda, b_sk, b_sn, ldc, ldd;   // B(k, n) at k * b_sk + n * b_sn
   int64_t a_group;             // elements between the groups' A
   float alpha, beta;
   const float* bias;
@@ -93,7 +97,7 @@ __device__ __forceinline__ int skinny_reduce(float (&v)[V], int lane) {
   return first;
 }
 
-template <typename T, bool K_MAJOR, int NT>
+template <typename T, bool K_MAJOR, int NT, bool ANY>
 __global__ void __launch_bounds__(kSkinnyThreads, 2) skinny_gemm_kernel(const SkinnyParams p) {
   constexpr int kOut = kSkinnyRows * NT;
   __shared__ float part[K_MAJOR ? 1 : 8][kOut];   // M_MAJOR: sums of each warp
@@ -117,7 +121,10 @@ __global__ void __launch_bounds__(kSkinnyThreads, 2) skinny_gemm_kernel(const Sk
   if (n == 0) return;    // the list is shorter than the grid; the same for every CTA of the cluster
 
   const T* A = static_cast<const T*>(p.A) + g * p.a_group;
-  const T* B = static_cast<const T*>(p.B) + c0 * p.ldb;
+  const T* B = static_cast<const T*>(p.B) + c0 * p.b_sn;
+  // ANY: where this group's A and the columns of B end
+  const uint16_t* a_first = reinterpret_cast<const uint16_t*>(A);
+  const uint16_t* a_last = a_first + (K_MAJOR ? static_cast<int64_t>(p.M - 1) * p.lda + p.K : static_cast<int64_t>(p.K - 1) * p.lda + p.M);
   const int k_begin = static_cast<int>(rank) * p.k_per_rank;
   const int k_end = min(k_begin + p.k_per_rank, p.K);
   float acc[8 * NT];     // [row][column]
@@ -134,12 +141,29 @@ __global__ void __launch_bounds__(kSkinnyThreads, 2) skinny_gemm_kernel(const Sk
       // rows behind the last one re-read it (their sums are not stored); M_MAJOR has whole runs of 8 rows
       const T* src = K_MAJOR ? A + static_cast<int64_t>(min(row + i, p.M - 1)) * p.lda + k
                              : A + static_cast<int64_t>(k + i) * p.lda + (row_ok ? row : 0);
-      w[i] = skinny_load_stream(src);
+      if constexpr (!ANY) {
+        w[i] = skinny_load_stream(src);
+      } else if constexpr (K_MAJOR) {
+        w[i] = any_keep(any_load_8(reinterpret_cast<const uint16_t*>(src), a_first, a_last), min(8, p.K - k));
+      } else {
+        w[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (k + i < k_end) w[i] = any_load_8(reinterpret_cast<const uint16_t*>(src), a_first, a_last);
+      }
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       x[t] = make_uint4(0u, 0u, 0u, 0u);
-      if (t < n) x[t] = *reinterpret_cast<const uint4*>(B + t * p.ldb + k);
+      if (t < n) {
+        if constexpr (!ANY) {
+          x[t] = *reinterpret_cast<const uint4*>(B + t * p.b_sn + k);
+        } else {
+          const uint16_t* src = reinterpret_cast<const uint16_t*>(B) + t * p.b_sn + k * p.b_sk;
+          uint32_t e[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) e[j] = k + j < k_end ? src[j * p.b_sk] : 0u;
+          x[t] = make_uint4(e[0] | (e[1] << 16), e[2] | (e[3] << 16), e[4] | (e[5] << 16), e[6] | (e[7] << 16));
+        }
+      }
     }
     float xf[NT][8];
 #pragma unroll

@@ -89,10 +89,12 @@ class _Call:
         return plan
 
     def workspace_bytes(self, h) -> int:
-        ragged = self.groups.ragged if self.groups is not None else 0
-        if ragged == L.GK_RAGGED_COLUMNS:
+        d, gr = self.desc, self.groups
+        ragged = gr.ragged if gr is not None else 0
+        aligned = d.lda % 8 == 0 and d.ldb % 8 == 0 and (gr is None or gr.stride_a % 8 == 0)
+        if aligned and ragged == L.GK_RAGGED_COLUMNS:
             return 0
-        if ragged == 0 and not (self.desc.m * self.desc.n <= (1 << 22) and self.desc.k >= 2048):
+        if aligned and ragged == 0 and not (d.m * d.n <= (1 << 22) and d.k >= 2048):
             return 0          # many output tiles, or a short K: nothing is cut along K
         return self.query(h).workspace_bytes
 
@@ -277,20 +279,23 @@ def _hooks(transforms: dict) -> dict:
 # products grouped by expert
 # ------------------------------------------------------------------------------------------------
 def matmul_grouped(conf: Config, a, b, c, d, offsets, *, epilogue=None, kernel=Kernel.matmul_singlestage, stream=None,
-                   **transforms):
+                   workspace=None, **transforms):
     """D[:, J_g] = epilogue(A[:, :, g] * B[:, J_g] + C[:, J_g]) for every group g, in one launch.
 
     `a` is (M, K, groups) - or (K, M, groups) with a RowMajor layout, which makes this the input gradient of the same
     layer; its groups may lie any distance apart.  `b`, `c` and `d` are as for `matmul` with N = all columns there are
     (`conf.matmul_shape`); `offsets` is a device array of groups + 1 Int32 or Int64 values, of which group g takes the
     columns offsets[g] .. offsets[g + 1] - 1.  `epilogue` is Epilogue.Default, Epilogue.Bias with a bias of (M, groups)
-    and axis="row", or one of the fused ones.  Columns outside every group are left as they were."""
-    _run(lower_grouped(conf, a, b, c, d, offsets, _hooks(transforms), epilogue or Epilogue.Default(), kernel), stream)
+    and axis="row", or one of the fused ones.  Columns outside every group are left as they were.  Operands
+    whose columns are not 16-byte aligned are copied into the workspace first (`grouped_query` reports its size; the
+    package lends one when it is None); when it is too small, slower bounds-checked loads read them."""
+    _run(lower_grouped(conf, a, b, c, d, offsets, _hooks(transforms), epilogue or Epilogue.Default(), kernel), stream, workspace)
 
 
-def bind_grouped(conf: Config, a, b, c, d, offsets, *, epilogue=None, kernel=Kernel.matmul_singlestage, **transforms) -> BoundFused:
-    """`matmul_grouped` with its arguments lowered once."""
-    return BoundFused(lower_grouped(conf, a, b, c, d, offsets, _hooks(transforms), epilogue or Epilogue.Default(), kernel))
+def bind_grouped(conf: Config, a, b, c, d, offsets, *, epilogue=None, kernel=Kernel.matmul_singlestage, workspace=None,
+                 **transforms) -> BoundFused:
+    """`matmul_grouped` with its arguments lowered once (and a workspace of its own, where it uses one)."""
+    return BoundFused(lower_grouped(conf, a, b, c, d, offsets, _hooks(transforms), epilogue or Epilogue.Default(), kernel), workspace)
 
 
 def matmul_grouped_outer(conf: Config, a, b, c, d, offsets, *, kernel=Kernel.matmul_singlestage, stream=None, workspace=None,

@@ -375,8 +375,10 @@ typedef struct gk_group_desc {
 } gk_group_desc;
 
 /* What gk_gemm_fused would launch (plan.kernel 1 = tensor cores, 6 = the streaming kernel for a few columns)
- * and the workspace it can use: REQUIRED for a ragged depth (the groups' tensor maps, 256-byte aligned),
- * optional for a plain fused product with few output tiles and a long K, none otherwise. */
+ * and the 256-byte aligned workspace it can use: REQUIRED for a ragged depth with K strided in both operands (the
+ * groups' tensor maps); optional for operands whose columns are not 16-byte aligned (they are copied with padded
+ * columns; without the room, bounds-checked loads read them, several times slower) and for a plain fused product
+ * with few output tiles and a long K (cut along K); none otherwise. */
 GK_API gk_status gk_gemm_fused_query(gk_handle h, const gk_gemm_desc* desc, const gk_fused_desc* fused,
                                      const gk_group_desc* groups, gk_gemm_plan* plan);
 

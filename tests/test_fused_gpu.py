@@ -264,18 +264,59 @@ def test_fused_tile_shapes(tile_n, cg, m):
     a, b, r = ints(g, m, k), ints(g, k, n), ints(g, m, n, dtype=torch.float32)
     d, z = torch.zeros_like(r), torch.zeros_like(r)
 
-    def run():
-        GK.matmul(conf(m, n, k, torch.float16, torch.float32, residual=True, tile_n=tile_n, cta_group=cg), a, b, r, d,
-                  epilogue=Epilogue.BiasActivationResidual(None, "row", ACT["relu"], z))
-
-    if tile_n == 512 and m % 8:      # columns of A that are not 16-byte aligned: one CTA per tile, 256 columns at most
-        with pytest.raises(GK.ConfigError, match="16-byte"):
-            run()
-        return
-    run()
+    GK.matmul(conf(m, n, k, torch.float16, torch.float32, residual=True, tile_n=tile_n, cta_group=cg), a, b, r, d,
+              epilogue=Epilogue.BiasActivationResidual(None, "row", ACT["relu"], z))
     done()
     x = a.double() @ b.double()
     assert torch.equal(z.double(), x) and torch.equal(d.double(), x.clamp(min=0) + r.double())
+
+
+@pytest.mark.parametrize("ta,tb", [(False, False), (True, True)])
+@pytest.mark.parametrize("m,n,k", [(77, 45, 33), (300, 257, 1111), (130, 70, 6)])
+def test_unaligned_operands_with_and_without_room_for_their_copies(m, n, k, ta, tb):
+    g = gen(m)
+    a, b, r = ints(g, m, k), ints(g, k, n), ints(g, m, n, dtype=torch.float32)
+    aw, bw = cm(a.T) if ta else a, cm(b.T) if tb else b
+    cf = conf(m, n, k, torch.float16, torch.float32, ta, tb, True)
+    epi = Epilogue.BiasActivationResidual(activation=ACT["relu"])
+    want = (a.double() @ b.double()).clamp(min=0) + r.double()
+    need = GK.query(cf, aw, bw, r, torch.zeros_like(r), epilogue=epi).workspace_bytes
+    assert need > 0
+    for room in (need, 256):
+        ws = torch.full((need + 256,), 5, dtype=torch.uint8, device="cuda")
+        d = torch.zeros_like(r)
+        GK.matmul(cf, aw, bw, r, d, epilogue=epi, workspace=ws[:room])
+        done()
+        assert torch.equal(d.double(), want) and (ws[room:] == 5).all()
+    # operands that start in the middle of an allocation, two bytes past a 16-byte boundary
+    big = torch.zeros(a.numel() + 64, dtype=torch.float16, device="cuda")
+    shifted = big[1: 1 + a.numel()].view(aw.shape[1], aw.shape[0]).T
+    shifted.copy_(aw)
+    d = torch.zeros_like(r)
+    GK.matmul(cf, shifted, bw, r, d, epilogue=epi)
+    done()
+    assert torch.equal(d.double(), want)
+
+
+@pytest.mark.parametrize("n", [1, 2, 3, 4])
+@pytest.mark.parametrize("ta,tb", [(False, False), (True, False), (False, True), (True, True)])
+@pytest.mark.parametrize("m,k", [(1, 1), (7, 9), (65, 1023), (200, 257), (129, 2055), (64, 300)])
+def test_few_columns_of_any_size_and_order(m, k, n, ta, tb):
+    g = gen(m + k + n)
+    a, b, r = ints(g, m, k), ints(g, k, n), ints(g, m, n, dtype=torch.float32)
+    bias = ints(g, m, dtype=torch.float32)
+    poison = torch.full((a.numel() + 40,), float("nan"), dtype=torch.float16, device="cuda")     # NaN around A
+    aw = cm(a.T) if ta else a
+    view = poison[11: 11 + a.numel()].view(aw.shape[1], aw.shape[0]).T
+    view.copy_(aw)
+    for src in (aw, view):
+        d = torch.full_like(r, -9.0)
+        cf = conf(m, n, k, torch.float16, torch.float32, ta, tb, True)
+        epi = Epilogue.BiasActivationResidual(bias, activation=ACT["relu"])
+        assert GK.query(cf, src, cm(b.T) if tb else b, r, d, epilogue=epi).kernel == 6
+        GK.matmul(cf, src, cm(b.T) if tb else b, r, d, epilogue=epi)
+        done()
+        assert torch.equal(d.double(), (a.double() @ b.double() + bias.double()[:, None]).clamp(min=0) + r.double())
 
 
 # ------------------------------------------------------------------------------------------------
@@ -311,6 +352,26 @@ def test_grouped_product_of_integers_is_exact(counts, m, k, ta, tb):
     dt = torch.bfloat16 if m == 264 else torch.float16
     run_grouped(counts, m, k, dt, ta, tb)
     run_grouped(counts, m, k, dt, ta, tb, first=3, tail=13, offdt=torch.int64)
+
+
+@pytest.mark.parametrize("ta,tb", [(False, False), (True, True)])
+@pytest.mark.parametrize("counts", [[40, 0, 300, 1], [2, 0, 3, 1]])
+def test_grouped_unaligned_with_and_without_room(counts, ta, tb):
+    g = gen(51)
+    m, k, G = 77, 45, 4
+    offsets, o = offsets_of(counts, first=1)
+    total = o[-1] + 2
+    w, x = ints(g, m, k, G), ints(g, k, total)
+    want = cm(torch.full((m, total), -9.0, device="cuda")).double()
+    for i in range(G):
+        want[:, o[i]:o[i + 1]] = w[:, :, i].double() @ x[:, o[i]:o[i + 1]].double()
+    aw, xw = cm(w.permute(1, 0, 2)) if ta else w, cm(x.T) if tb else x
+    cf = conf(m, total, k, torch.float16, torch.float32, ta, tb)
+    for room in (None, 256):
+        d = cm(torch.full((m, total), -9.0, device="cuda"))
+        GK.matmul_grouped(cf, aw, xw, None, d, offsets, workspace=None if room is None else torch.zeros(room, dtype=torch.uint8, device="cuda"))
+        done()
+        assert torch.equal(d.double(), want)
 
 
 @pytest.mark.parametrize("tile_n,cg", [(32, 1), (64, 1), (128, 1), (256, 1), (128, 2), (256, 2)])
