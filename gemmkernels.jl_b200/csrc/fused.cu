@@ -169,13 +169,15 @@ static bool skinny_plan(gk_handle h, const gk_gemm_desc& d, const gk_group_desc*
   auto al = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
   p.any = !al(a) || !al(b) || d.lda % 8 || d.ldb % 8 || d.k % 8 || (!d.trans_a && d.m % 8) || d.trans_b ||
           (gr && groups > 1 && gr->stride_a % 8);
-  p.nt = d.n <= 1 ? 1 : (d.n <= 2 * active ? 2 : 4);
+  // Columns at a time: the average of the groups that can have any, rounded up (a group with more is streamed again, from L2).
+  p.nt = d.n <= active ? 1 : (d.n <= 2 * active ? 2 : 4);
   p.items = static_cast<int>(std::min<int64_t>(d.n, d.n / p.nt + active));
   if (groups == 1) p.items = static_cast<int>((d.n + p.nt - 1) / p.nt);
   p.rows = static_cast<int>((d.m + kSkinnyRows - 1) / kSkinnyRows);
-  const int64_t want = 2 * static_cast<int64_t>(h->sm_count);      // two CTAs per SM
+  // K is cut as far as the CTAs still run in one round.
+  const int64_t slots = static_cast<int64_t>(p.any ? 2 : skinny_ctas(p.nt)) * h->sm_count;
   const int64_t steps = (d.k + kSkinnyStep - 1) / kSkinnyStep;
-  while (p.ranks < 8 && 2 * p.ranks <= steps && static_cast<int64_t>(p.rows) * p.items * p.ranks < want) p.ranks *= 2;
+  while (p.ranks < 8 && 2 * p.ranks <= steps && 2 * static_cast<int64_t>(p.rows) * p.items * p.ranks <= slots) p.ranks *= 2;
   p.k_per_rank = static_cast<int>((steps + p.ranks - 1) / p.ranks * kSkinnyStep);
   *out = p;
   return true;

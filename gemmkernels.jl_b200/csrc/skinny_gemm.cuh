@@ -6,7 +6,7 @@
 // the whole stream of a 4096 x 4096 layer (5.1 us at 6.57 TB/s), so plain 16-byte loads feed FMAs directly.
 //
 // A cluster of S CTAs owns 64 rows of D; its CTA r takes the r-th run of K, so that a layer with few rows still has
-// loads in flight on every SM (S is chosen on the host: two CTAs per SM).  The CTAs' partial sums meet in
+// loads in flight on every SM (S is chosen on the host: one round of resident CTAs).  The CTAs' partial sums meet in
 // distributed shared memory, where each CTA adds one slice of the 64 x NT outputs in the order of the ranks (the
 // result does not depend on timing) and applies the epilogue.
 //   K_MAJOR  (A stored with consecutive k): a warp owns 8 rows, its lanes 8 consecutive k each
@@ -26,6 +26,9 @@ namespace gk {
 constexpr int kSkinnyThreads = 256;
 constexpr int kSkinnyRows = 64;        // rows of D per cluster
 constexpr int kSkinnyStep = 256;       // K consumed per step of a CTA (K runs are multiples of it)
+// CTAs per SM, which the registers are limited to: the loads in flight are what hides the latency of HBM (4096 x 4096,
+// one column: 12.3 us with two, 8.3 us with four).
+__host__ __device__ constexpr int skinny_ctas(int nt) { return nt == 1 ? 4 : (nt == 2 ? 3 : 2); }
 
 struct SkinnyParams {
   const void* A; const void* B; const void* C; void* D;
@@ -98,7 +101,7 @@ __device__ __forceinline__ int skinny_reduce(float (&v)[V], int lane) {
 }
 
 template <typename T, bool K_MAJOR, int NT, bool ANY>
-__global__ void __launch_bounds__(kSkinnyThreads, 2) skinny_gemm_kernel(const SkinnyParams p) {
+__global__ void __launch_bounds__(kSkinnyThreads, ANY ? 2 : skinny_ctas(NT)) skinny_gemm_kernel(const SkinnyParams p) {
   constexpr int kOut = kSkinnyRows * NT;
   __shared__ float part[K_MAJOR ? 1 : 8][kOut];   // M_MAJOR: sums of each warp
   __shared__ float sum[kOut];                     // sums of this CTA's K run, [column][row]
