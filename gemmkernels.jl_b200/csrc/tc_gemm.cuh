@@ -192,6 +192,16 @@ __device__ __forceinline__ void tc_build_table(const TcParams& p, int* tab, int 
   if (lane == 0) tab[G] = FORM == kTcRaggedCols ? tiles : p.tiles_m * p.tiles_n * G;
 }
 
+// kTcRaggedCols: first column of the group's tile tn, and how many columns the tile multiplies: what the group still
+// has, in steps of 32 (the last tile of a group is as narrow as that; its copies and MMAs shrink with it).
+__device__ __forceinline__ int tc_group_col0(const TcParams& p, const int* tab, int g, int tn) {
+  const int lo = tab[p.f.groups + 1 + g];
+  return lo - lo % p.col_align + tn * p.bn;
+}
+__device__ __forceinline__ int tc_group_cols(const TcParams& p, const int* tab, int g, int col0) {
+  return min(p.bn, (tab[2 * p.f.groups + 1 + g] - col0 + 31) & ~31);
+}
+
 // kTcRaggedCols: unit t of the list -> group (the cursor g only moves forward) and tile of it.
 __device__ __forceinline__ void tc_group_tile(const TcParams& p, const int* tab, int t, int& g, int& tm, int& tn) {
   while (t >= tab[g + 1]) ++g;
@@ -872,13 +882,15 @@ __global__ void __launch_bounds__(FORM == kTcPlain ? tc_threads(PLANES) : 128 + 
           (RANK5 ? sb * (is_a ? p.a_sub_bytes : p.b_sub_bytes) : 0) + kj * kblock_bytes;
       const void* tmap = is_a ? static_cast<const void*>(&p.tm_a) : static_cast<const void*>(&p.tm_b);
       [[maybe_unused]] int grp = 0, map_of = -1;      // ragged forms: the unit's group, the group `tmap` belongs to
-      const int mn_add = (mn_major ? bx * (is_a ? p.a_box_mn : p.b_box_mn) : sb * sub_step) + nb * p.bn;
+      // (ragged columns load a K-major B in boxes too, so that a narrow tile loads only some of them)
+      const int mn_add = (mn_major || (FORM == kTcRaggedCols && !is_a) ? bx * (is_a ? p.a_box_mn : p.b_box_mn) : sb * sub_step) + nb * p.bn;
       [[maybe_unused]] const int k_add = mn_major ? sb * sub_step : 0;
       [[maybe_unused]] const int perm = is_a ? p.a_perm : p.b_perm;
       [[maybe_unused]] const int mn_div = is_a ? p.a_mn_div : p.b_mn_div;   // RANK5 only
       [[maybe_unused]] const int k_div = is_a ? p.a_k_div : p.b_k_div;
       const uint32_t full0_signal = (CG == 2) ? map_to_cta(bar_full, 0) : bar_full;
-      const uint32_t tx_bytes = stage_bytes * CG;
+      uint32_t tx_bytes = stage_bytes * CG;
+      bool loads = active;               // this lane's box is part of the unit
       int s = 0;
       uint32_t ph = 0;
       uint32_t it = 0;        // pipeline stages passed so far (both warps count all of them)
@@ -900,8 +912,12 @@ __global__ void __launch_bounds__(FORM == kTcPlain ? tc_threads(PLANES) : 128 + 
         int n_cta = tn * bn_tile + static_cast<int>(rank) * bn_cta;
         [[maybe_unused]] int k_first = 0;
         if constexpr (FORM == kTcRaggedCols) {
-          const int lo = tab[p.f.groups + 1 + grp];
-          n_cta += lo - lo % p.col_align;
+          const int col0 = tc_group_col0(p, tab, grp, tn);
+          const int cols_cta = tc_group_cols(p, tab, grp, col0) / CG;     // this CTA's share of the tile's columns
+          n_cta = col0 + static_cast<int>(rank) * cols_cta;
+          const int boxes = (cols_cta + p.b_box_mn - 1) / p.b_box_mn;
+          loads = active && (is_a || bx < boxes);
+          tx_bytes = CG * p.kps * (p.a_plane_bytes + boxes * p.b_box_bytes);
         }
         if constexpr (FORM == kTcRaggedDepth) {
           k_first = tab[p.f.groups + 1 + bt];
@@ -935,7 +951,7 @@ __global__ void __launch_bounds__(FORM == kTcPlain ? tc_threads(PLANES) : 128 + 
             if (armed == 0 && lane == 0) tc_mark(p.status, dbg, 2 + which, 1);   // about to issue first copies
             if (dbg & 1) {
               if (lane == 0 && leader) mbar_arrive(bar_full + 8u * s);
-            } else if (active) {
+            } else if (loads) {
               // Bytes may be counted on the barrier before they are expected: the phase cannot
               // complete until the arrival that announces them.
               if (lane == 0 && leader) mbar_arrive_expect_tx(bar_full + 8u * s, tx_bytes);
@@ -1043,6 +1059,7 @@ __global__ void __launch_bounds__(FORM == kTcPlain ? tc_threads(PLANES) : 128 + 
       uint32_t ph = 0;
       uint32_t acc_it = 0;
       bool ok = true;
+      [[maybe_unused]] int grp = 0;
       const bool prof = (dbg & 8) != 0;
       long long mw = 0, mi = 0, mt = 0, t0 = 0, t1 = 0;
       const long long k_start = clock64();
@@ -1132,6 +1149,12 @@ __global__ void __launch_bounds__(FORM == kTcPlain ? tc_threads(PLANES) : 128 + 
         if constexpr (FORM == kTcRaggedDepth) {
           const int bt = t / units_per_product;
           kb1 = (tab[2 * p.f.groups + 1 + bt] - tab[p.f.groups + 1 + bt] + p.bk - 1) / p.bk;
+        }
+        if constexpr (FORM == kTcRaggedCols) {
+          int tm, tn;
+          tc_group_tile(p, tab, t, grp, tm, tn);
+          const int cols = tc_group_cols(p, tab, grp, tc_group_col0(p, tab, grp, tn));
+          t_id[0] = (p.idesc & ~(0x3fu << 17)) | (static_cast<uint32_t>(cols >> 3) << 17);
         }
         bool first_kb = true;   // the first k-block of a tile (or K-run) overwrites the accumulators
         for (int kb = kb0; kb < kb1; kb += p.kps) {
@@ -1230,14 +1253,14 @@ __global__ void __launch_bounds__(FORM == kTcPlain ? tc_threads(PLANES) : 128 + 
       if constexpr (FORM == kTcRaggedDepth) nothing = tab[p.f.groups + 1 + bt] == tab[2 * p.f.groups + 1 + bt];
       const uint32_t as = two_acc ? (acc_it & 1u) : 0u;
       const uint32_t aph = (two_acc ? (acc_it >> 1) : acc_it) & 1u;
-      if (prefetch_c) {
+      if (FORM == kTcPlain && prefetch_c) {
         // While the main loop of this tile runs, pull the tile's part of C into L2: one request per
         // 128-byte line (this warp's 32 rows of one column), columns dealt out to the lanes.
         const int m0 = m - lane;
         if (m0 < p.M) {
           const size_t es_c = p.dtype_c == TC_F32 ? 4 : 2;
           const char* c_line = static_cast<const char*>(p.C) + (static_cast<size_t>(m0) + static_cast<size_t>(bt) * p.c_batch) * es_c;
-          for (int c = lane + chunk_first; c < bn_tile && n0 + c < (FORM == kTcRaggedCols ? n_hi : p.N); c += chunk_step) {
+          for (int c = lane + chunk_first; c < bn_tile && n0 + c < p.N; c += chunk_step) {
 #pragma unroll
             for (int pl = 0; pl < PLANES; ++pl)
               prefetch_l2(c_line + (static_cast<size_t>(pl) * p.c_plane + static_cast<size_t>(n0 + c) * p.c_sn0) * es_c);
@@ -1245,11 +1268,17 @@ __global__ void __launch_bounds__(FORM == kTcPlain ? tc_threads(PLANES) : 128 + 
         }
       }
       if constexpr (FORM != kTcPlain) {
-        if (p.f.form == FUSED_GRADIENT && m - lane < p.M) {      // the same for the tile's part of Z
-          const size_t es = p.dtype_d == TC_F32 ? 4 : 2;
-          const char* z_line = static_cast<const char*>(p.f.Z) + static_cast<size_t>(m - lane) * es;
-          for (int c = lane + chunk_first; c < bn_tile && n0 + c < (FORM == kTcRaggedCols ? n_hi : p.N); c += chunk_step)
-            prefetch_l2(z_line + static_cast<size_t>(n0 + c) * p.f.z_sn * es);
+        // (A tile further ahead is slower: 1 GB of accumulated weight gradients 245 against 203 us.)
+        // While the main loop of this tile runs, pull its part of C (and of the Z that the gradient form reads) into L2.
+        const bool reads_z = p.f.form == FUSED_GRADIENT;
+        if ((has_c || reads_z) && m - lane < p.M) {
+          const int64_t es = p.dtype_d == TC_F32 ? 4 : 2;
+          const char* c_line = static_cast<const char*>(p.C) + (m - lane + bt * p.c_batch) * es;
+          const char* z_line = static_cast<const char*>(p.f.Z) + (m - lane) * es;
+          for (int c = lane + chunk_first; c < bn_tile && n0 + c < n_hi; c += chunk_step) {
+            if (has_c) prefetch_l2(c_line + (n0 + c) * p.c_sn0 * es);
+            if (reads_z) prefetch_l2(z_line + (n0 + c) * p.f.z_sn * es);
+          }
         }
       }
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + as * acc_cols;
