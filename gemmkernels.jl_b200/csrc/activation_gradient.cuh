@@ -77,17 +77,24 @@ __global__ void __launch_bounds__(kActGradThreads, 3) activation_gradient_kernel
     const T* dd = static_cast<const T*>(p.dD) + row + static_cast<int64_t>(c0) * p.ldd;
     const T* z = static_cast<const T*>(p.Z) + row + static_cast<int64_t>(c0) * p.ldz;
     T* dz = static_cast<T*>(p.dZ) + row + static_cast<int64_t>(c0) * p.lddz;
-    constexpr int U = 2;                                  // columns per thread whose loads are in flight together
-    for (int c = slot; c < n; c += U * kSlots) {
-      V dv[U], zv[U];
+    // The loads of the next U columns are in flight while these are computed (8192 x 16384, GELU: 163 us without).
+    constexpr int U = 2;
+    V dv[U], zv[U], dn[U], zn[U];
+    auto load = [&](int c, V (&d)[U], V (&w)[U]) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int col = c + u * kSlots;
         if (col < n) {
-          dv[u] = *reinterpret_cast<const V*>(dd + col * p.ldd);
-          if (ACT != FUSED_ACT_NONE) zv[u] = *reinterpret_cast<const V*>(z + col * p.ldz);
+          d[u] = *reinterpret_cast<const V*>(dd + col * p.ldd);
+          if (ACT != FUSED_ACT_NONE) w[u] = *reinterpret_cast<const V*>(z + col * p.ldz);
         }
       }
+    };
+    load(slot, dn, zn);
+    for (int c = slot; c < n; c += U * kSlots) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) { dv[u] = dn[u]; zv[u] = zn[u]; }
+      load(c + U * kSlots, dn, zn);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int col = c + u * kSlots;

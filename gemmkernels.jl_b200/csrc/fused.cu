@@ -260,7 +260,7 @@ static ActGradPlan actgrad_plan(int sm_count, const gk_activation_gradient_desc&
   p.rows = static_cast<int>((d.m + kActGradRows - 1) / kActGradRows);
   // Strips long enough to amortise their reduction, short enough for eight CTAs per SM.
   const int64_t want = (d.n * p.rows + 8 * sm_count - 1) / (8 * sm_count);
-  int64_t strip = std::max<int64_t>(128, std::min<int64_t>(512, (want + 127) / 128 * 128));
+  int64_t strip = std::max<int64_t>(128, std::min<int64_t>(2048, (want + 127) / 128 * 128));
   // A short matrix is summed by one CTA per group and 64 rows: a second launch costs more than it spreads.
   p.per_group = sums && d.n <= 512 ? 1 : 0;
   const int64_t active = std::min<int64_t>(d.groups, d.n);
