@@ -114,8 +114,8 @@ __global__ void __launch_bounds__(kActGradThreads, 3) activation_gradient_kernel
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
               float v = actgrad_float(de[i]);
-              if (ACT != FUSED_ACT_NONE) v *= fused_act_gradient(actgrad_float(ze[i]), ACT);
-              acc[i] += v;
+              if (ACT != FUSED_ACT_NONE) v = __fmul_rn(v, fused_act_gradient(actgrad_float(ze[i]), ACT));
+              acc[i] = __fadd_rn(acc[i], v);    // never contracted: the same sums whether dZ is stored or not
               de[i] = actgrad_round<T>(v);
             }
           }

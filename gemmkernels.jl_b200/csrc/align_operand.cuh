@@ -2,8 +2,8 @@
 // before a fused or ragged product: dst[g][c][r] = src[g * group + c * ld + r], columns of ld_dst (a multiple of 8)
 // elements, zeros behind the rows.  A copy at the rate of HBM against feeding the tensor cores by bounds-checked loads
 // of two warps: 1000 x 777 x 1111, B unaligned, 140 us without it.
-// A warp takes a column; its lanes take 8 rows each, whose 16 source bytes lie in two granules: the second one is the
-// next lane's first.
+// A warp takes 256 rows of a column; its lanes take 8 each, whose 16 source bytes lie in two granules: the second one is
+// the next lane's first.
 #pragma once
 #include "any_load.cuh"
 #include "fused_epilogue.cuh"
@@ -38,21 +38,21 @@ static __global__ void __launch_bounds__(kAlignThreads) align_operand_kernel(con
   const uint16_t* src = p.src + g * p.group;
   const uint16_t* end = src + static_cast<int64_t>(p.cols - 1) * p.ld + p.rows;
   uint16_t* dst = p.dst + g * p.group_dst;
-  const int pieces = static_cast<int>(p.ld_dst / 8);
-  for (int c = static_cast<int>(blockIdx.x) * (kAlignThreads / 32) + warp; c < p.cols; c += static_cast<int>(gridDim.x) * (kAlignThreads / 32)) {
+  const int pieces = static_cast<int>(p.ld_dst / 8), segments = (pieces + 31) / 32;
+  const int64_t units = static_cast<int64_t>(segments) * p.cols, step = static_cast<int64_t>(gridDim.x) * (kAlignThreads / 32);
+  for (int64_t u = static_cast<int64_t>(blockIdx.x) * (kAlignThreads / 32) + warp; u < units; u += step) {
+    const int64_t c = u / segments;
     const uint16_t* col = src + c * p.ld;
     const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(col) & 15);
     const uint16_t* granules = reinterpret_cast<const uint16_t*>(reinterpret_cast<uintptr_t>(col) & ~static_cast<uintptr_t>(15));
-    for (int q0 = 0; q0 < pieces; q0 += 32) {
-      const int q = q0 + lane;
-      const uint4 lo = any_granule(granules + 8 * q, src, end);
-      uint4 hi;
-      hi.x = __shfl_down_sync(0xffffffffu, lo.x, 1); hi.y = __shfl_down_sync(0xffffffffu, lo.y, 1);
-      hi.z = __shfl_down_sync(0xffffffffu, lo.z, 1); hi.w = __shfl_down_sync(0xffffffffu, lo.w, 1);
-      if (lane == 31) hi = any_granule(granules + 8 * q + 8, src, end);
-      if (q < pieces)
-        *reinterpret_cast<uint4*>(dst + c * p.ld_dst + 8 * q) = any_keep(any_shift(lo, hi, shift), min(8, p.rows - 8 * q));
-    }
+    const int q = static_cast<int>(u - c * segments) * 32 + lane;
+    const uint4 lo = any_granule(granules + 8 * q, src, end);
+    uint4 hi;
+    hi.x = __shfl_down_sync(0xffffffffu, lo.x, 1); hi.y = __shfl_down_sync(0xffffffffu, lo.y, 1);
+    hi.z = __shfl_down_sync(0xffffffffu, lo.z, 1); hi.w = __shfl_down_sync(0xffffffffu, lo.w, 1);
+    if (lane == 31) hi = any_granule(granules + 8 * q + 8, src, end);
+    if (q < pieces)
+      *reinterpret_cast<uint4*>(dst + c * p.ld_dst + 8 * q) = any_keep(any_shift(lo, hi, shift), min(8, p.rows - 8 * q));
   }
 }
 

@@ -148,7 +148,8 @@ static gk_status launch_copy(gk_handle h, const OperandCopy& c, const void* src,
   p.f = f;
   const int per_block = kAlignThreads / 32;
   const int64_t want = std::max<int64_t>(1, 16 * static_cast<int64_t>(h->sm_count) / c.groups);
-  const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((c.cols + per_block - 1) / per_block, want));
+  const int64_t units = (c.ld / 8 + 31) / 32 * c.cols;      // a warp's share: 256 rows of a column
+  const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((units + per_block - 1) / per_block, want));
   GK_CUDA_CHECK(launch_dependent(&align_operand_kernel, dim3(blocks, static_cast<unsigned>(c.groups)), dim3(kAlignThreads), 0, stream, p));
   return GK_OK;
 }
@@ -164,7 +165,8 @@ static bool skinny_plan(gk_handle h, const gk_gemm_desc& d, const gk_group_desc*
   if (d.k < 1 || d.alpha == 0.0 || d.n < 1 || d.m < 1) return false;
   const int64_t groups = gr ? gr->groups : 1;
   const int64_t active = std::min<int64_t>(groups, d.n);
-  // One product: up to four columns (4096 x 4096: 11.8 us here, 15.3 on the tensor cores; eight columns 17 against 16).
+  // One product: up to four columns (4096 x 4096: 11.8 us here, 15.3 on the tensor cores; eight columns 16.4
+  // in one pass of eight - one CTA per SM for the registers - against 16.1; 8192 x 8192: 51 against 33).
   // Groups: while the average is one column (64 experts of 2048 x 2048: 16 tokens 25 against 34 us, 64 tokens 76 against
   // 72, 90 tokens 100 against 84 - a group with several columns streams its matrix several times).
   if (d.n > (groups > 1 ? 1 : 4) * active || d.n > 4096) return false;
@@ -218,11 +220,11 @@ static gk_status launch_skinny(const SkinnyPlan& sp, const gk_gemm_desc& d, cons
   cfg.blockDim = dim3(kSkinnyThreads);
   cfg.stream = stream;
   cudaLaunchAttribute at[2]{};
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = static_cast<unsigned>(sp.ranks); at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
-  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at; cfg.numAttrs = 2;
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = static_cast<unsigned>(sp.ranks); at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
+  cfg.attrs = at; cfg.numAttrs = sp.ranks > 1 ? 2 : 1;
   void* args[1] = {&p};
   const void* kernel = d.dtype_a == GK_F16 ? skinny_kernel<__half>(d.trans_a != 0, sp.any, sp.nt)
                                             : skinny_kernel<__nv_bfloat16>(d.trans_a != 0, sp.any, sp.nt);

@@ -61,9 +61,9 @@ enum TcBias : int32_t { TC_BIAS_NONE = 0, TC_BIAS_ROW = 1, TC_BIAS_COL = 2 };
 //                through shared memory by asynchronous copies, a chunk ahead
 //   kTcElements  everything else, element by element
 enum TcEpi : int { kTcElements = 0, kTcWords = 1, kTcFloats = 2 };
-__host__ __device__ constexpr int tc_fused_warps(int epi) { return 8; }
 
 enum TcForm : int { kTcPlain = 0, kTcFused = 1, kTcRaggedCols = 2, kTcRaggedDepth = 3 };
+__host__ __device__ constexpr int tc_fused_warps(int form, int epi) { return 8; }
 
 // status word values (0 = ok)
 enum TcStatus : int32_t {
@@ -698,12 +698,12 @@ __device__ __forceinline__ void tc_issue_kblock(uint32_t lo, bool first, uint32_
 // instance every such branch is compiled out, which shortens the per-stage loops of the producer and
 // MMA warps (their cost per pipeline stage is instruction latency, not bandwidth).
 template <int CG, int PLANES, bool TF32, bool RANK5, bool GENERIC = false, bool DBG = false, int FORM = kTcPlain, int EPI = kTcElements>
-__global__ void __launch_bounds__(FORM == kTcPlain ? tc_threads(PLANES) : 128 + 32 * tc_fused_warps(EPI), 1)
+__global__ void __launch_bounds__(FORM == kTcPlain ? tc_threads(PLANES) : 128 + 32 * tc_fused_warps(FORM, EPI), 1)
     tc_gemm_kernel(const __grid_constant__ TcParams p) {
   const int dbg = DBG ? p.debug : 0;
   static_assert(!GENERIC || (CG == 1 && PLANES == 1 && !TF32 && !RANK5), "generic loads: one CTA, one plane, 16-bit types");
   static_assert(FORM == kTcPlain || (PLANES == 1 && !TF32 && !RANK5 && !DBG), "fused forms: one plane, 16-bit types");
-  constexpr int kEpiWarps = FORM == kTcPlain ? tc_epilogue_warps(PLANES) : tc_fused_warps(EPI);
+  constexpr int kEpiWarps = FORM == kTcPlain ? tc_epilogue_warps(PLANES) : tc_fused_warps(FORM, EPI);
   extern __shared__ uint8_t smem_raw[];
   // 128-byte swizzle atoms are 1024 bytes and the pattern is a function of the address.
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;

@@ -552,7 +552,7 @@ gk_status tc_plan(gk_handle h, const TcProblem& pr_in, bool encode, TcLaunch* ou
                (!reads_c || (p.M % 4 == 0 && wide(pr.C, pr.c_sn[0], pr.batch_c, 4)))) {
       out->epi = kTcFloats;
     }
-    table_bytes = (pr.form >= kTcRaggedCols ? tc_table_bytes(pr.f.groups) : 0) + 16 + tc_fused_warps(out->epi) * tc_staging_bytes(out->epi);
+    table_bytes = (pr.form >= kTcRaggedCols ? tc_table_bytes(pr.f.groups) : 0) + 16 + tc_fused_warps(pr.form, out->epi) * tc_staging_bytes(out->epi);
   }
   const int kSmemBudget = kSmemMax - table_bytes;
   const int kblock_bytes = stage_bytes_for(cg, bn, n_sub, planes, planes);
