@@ -810,3 +810,139 @@ def test_ragged_depth_refuses_a_missing_workspace():
     for i in range(2):
         c = slice(o[i], o[i + 1])
         assert torch.equal(d[:, :, i].double(), dy[:, c].double() @ x[:, c].double().T)
+
+
+# ------------------------------------------------------------------------------------------------
+# combinations: types, leading dimensions, group strides, in-place C, epilogues - small integers, exact
+# ------------------------------------------------------------------------------------------------
+def roomy(t, pad, gap=0):
+    """The same (rows, cols[, groups]) array with `pad` elements between columns and `gap` more between groups, NaN there."""
+    rows, cols, groups = (*t.shape, 1)[:3]
+    ld = rows + pad
+    size = groups * (ld * cols + gap) + 8
+    buf = torch.full((size,), float("nan"), dtype=t.dtype, device=t.device)
+    view = buf.as_strided((rows, cols, groups), (1, ld, ld * cols + gap))
+    view.copy_(t if t.dim() == 3 else t[:, :, None])
+    return view if t.dim() == 3 else view[:, :, 0]
+
+
+@pytest.mark.parametrize("seed", range(60))
+def test_randomised_fused_and_grouped_combinations(seed):
+    import random
+    r = random.Random(seed)
+    g = gen(1000 + seed)
+    dt = r.choice([torch.float16, torch.bfloat16])
+    out = r.choice([torch.float32, dt])
+    step = r.choice([1, 8, 8, 16])
+    size = lambda lo, hi: max(step, r.randint(lo, hi) // step * step)
+    m, k, G = size(1, 600), size(1, 400), r.choice([1, 2, 5, 33])
+    counts = [r.choice([0, 0, 1, 3, 20, 70, 150]) for _ in range(G)]
+    grouped = r.random() < 0.6
+    n = sum(counts) + r.choice([0, 7]) if grouped else r.choice([1, 3, 9, 64, 130, 333])
+    ta, tb = r.random() < 0.5, r.random() < 0.3
+    pad, gap = r.choice([0, 8, 3]), r.choice([0, 16, 5])
+    form = r.choice(["standard", "residual", "gradient"])
+    act = r.choice([None, "relu"])
+    bits16 = out != torch.float32
+    lim = 1 if bits16 else 2
+    w = ints(g, m, k, G, dtype=dt, lo=-lim, hi=lim)
+    x = ints(g, k, n, dtype=dt, lo=0, hi=1)
+    if bits16:                       # at most 60 products of -1 .. 1 and small addends: every value is exact in 8 bits
+        x[:, :] = 0
+        x[: min(k, 60)] = ints(g, min(k, 60), n, dtype=dt, lo=0, hi=1)
+    has_c, keep = r.random() < 0.6, r.random() < 0.5
+    beta = r.choice([1.0, -2.0]) if has_c else 0.0
+    c, z0 = ints(g, m, n, dtype=out, lo=-9, hi=9), ints(g, m, n, dtype=out, lo=-2, hi=2)
+    bias = ints(g, m, G, dtype=torch.float32, lo=-5, hi=5)
+    owner = torch.full((n,), -1, device="cuda")
+    offsets, o = offsets_of(counts, dtype=r.choice([torch.int32, torch.int64]))
+    prod = torch.zeros(m, n, device="cuda", dtype=torch.float64)
+    if grouped:
+        for i in range(G):
+            prod[:, o[i]:o[i + 1]] = w[:, :, i].double() @ x[:, o[i]:o[i + 1]].double()
+            owner[o[i]:o[i + 1]] = i
+    else:
+        prod, owner[:] = w[:, :, 0].double() @ x.double(), 0
+    live = owner >= 0
+    add = bias.double()[:, owner.clamp(min=0)] if form != "gradient" else 0.0
+    pre = prod + add + (beta * c.double() if form != "residual" else 0.0)
+    f = (lambda t: t.clamp(min=0)) if act else (lambda t: t)
+    want = pre * (grad64(z0.double(), act)) if form == "gradient" else f(pre) + (beta * c.double() if form == "residual" else 0.0)
+    wd = roomy(torch.full((m, n), -77.0, dtype=out, device="cuda"), pad)
+    wz = roomy(z0, pad)
+    aw = roomy(w.permute(1, 0, 2) if ta else w, pad, gap)
+    xw = roomy(x.T if tb else x, pad)
+    cw = roomy(c, pad) if has_c else None
+    inplace = has_c and r.random() < 0.4 and not grouped
+    d = cw if inplace else wd
+    if form == "standard":
+        epi, keep = Epilogue.Bias(bias if grouped else bias[:, 0].contiguous(), axis="row"), False
+    elif form == "residual":
+        epi = Epilogue.BiasActivationResidual(bias if grouped else bias[:, 0].contiguous(), activation=ACT[act], preactivation=wz if keep else None)
+    else:
+        epi = Epilogue.ActivationGradient(wz, ACT[act])
+    kw = {}
+    if beta != 1.0 and has_c:
+        kw["transform_shared_to_regs_c"] = Transform.Elementwise(Transform.Scale(beta))
+    if form == "standard" and act:
+        kw["transform_shared_to_global_d"] = Transform.Elementwise(ACT[act])
+    cf = conf(m, n, k, dt, out, ta, tb, has_c)
+    if grouped:
+        GK.matmul_grouped(cf, aw, xw, cw, d, offsets, epilogue=epi, **kw)
+    else:
+        GK.matmul(cf, aw[:, :, 0], xw, cw, d, epilogue=epi, **kw)
+    done()
+    assert torch.equal(d[:, live].double(), want[:, live])
+    assert (d[:, ~live] == -77).all()
+    if form == "residual" and keep:
+        assert torch.equal(wz[:, live].double(), pre[:, live]) and torch.equal(wz[:, ~live], z0[:, ~live])
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_randomised_outer_combinations(seed):
+    import random
+    r = random.Random(seed)
+    g = gen(2000 + seed)
+    dt = r.choice([torch.float16, torch.bfloat16])
+    out = r.choice([torch.float32, dt])
+    step = r.choice([1, 8, 8])
+    m, n, G = max(step, r.randint(1, 500) // step * step), max(step, r.randint(1, 500) // step * step), r.choice([1, 3, 20])
+    counts = [r.choice([0, 1, 5, 63, 64, 65, 130]) for _ in range(G)]
+    offsets, o = offsets_of(counts, first=r.choice([0, 5]))
+    total = o[-1] + r.choice([0, 9])
+    dy, x = ints(g, m, total, dtype=dt, lo=-1, hi=1), ints(g, n, total, dtype=dt, lo=0, hi=1)
+    dy[:, r.randrange(0, 2)::3] = 0                                   # |sums| stay below 256: exact in BF16
+    c = ints(g, m, n, G, dtype=out, lo=-20, hi=20)
+    pad, gap = r.choice([0, 8, 3]), r.choice([0, 16, 5])
+    has_c, inplace = r.random() < 0.6, r.random() < 0.5
+    alpha = r.choice([1.0, 0.0, -1.0])
+    cw = roomy(c, pad, gap) if has_c else None
+    d = cw if has_c and inplace else roomy(torch.full((m, n, G), -77.0, dtype=out, device="cuda"), pad, gap)
+    ta, tb = r.random() < 0.2, r.random() < 0.8
+    GK.matmul_grouped_outer(conf(m, n, total, dt, out, ta, tb, has_c), roomy(dy.T if ta else dy, pad), roomy(x if tb else x.T, pad), cw, d, offsets,
+                            transform_shared_to_regs_a=Transform.Elementwise(Transform.Scale(alpha)))
+    done()
+    for i in range(G):
+        want = alpha * (dy[:, o[i]:o[i + 1]].double() @ x[:, o[i]:o[i + 1]].double().T) + (c[:, :, i].double() if has_c else 0.0)
+        assert torch.equal(d[:, :, i].double(), want), i
+
+
+def test_grouped_with_nothing_to_multiply():
+    g = gen(61)
+    m, counts = 136, [30, 0, 5]
+    offsets, o = offsets_of(counts, first=2)
+    total = o[-1] + 3
+    bias, c = ints(g, m, 3, dtype=torch.float32), ints(g, m, total, dtype=torch.float32)
+    nan = lambda *s: cm(torch.full(s, float("nan"), dtype=torch.float16, device="cuda"))
+    for k, alpha in ((64, 0.0), (0, 1.0)):
+        d = cm(torch.full((m, total), -9.0, device="cuda"))
+        w = nan(m, max(k, 1), 3)[:, :k]
+        GK.matmul_grouped(conf(m, total, k, torch.float16, torch.float32, residual=True), w, nan(max(k, 1), total)[:k], c, d, offsets,
+                          epilogue=Epilogue.BiasActivationResidual(bias), transform_shared_to_regs_a=Transform.Elementwise(Transform.Scale(alpha)))
+        done()
+        for i in range(3):
+            assert torch.equal(d[:, o[i]:o[i + 1]], bias[:, i:i + 1] + c[:, o[i]:o[i + 1]])
+        assert (d[:, : o[0]] == -9).all() and (d[:, o[-1]:] == -9).all()
+    with pytest.raises(GK.ConfigError, match="per row"):
+        GK.matmul_grouped(conf(m, total, 64, torch.float16, torch.float32), nan(m, 64, 3), nan(64, total), None, d, offsets,
+                          epilogue=Epilogue.Bias(torch.zeros(total, device="cuda"), axis="col"))
