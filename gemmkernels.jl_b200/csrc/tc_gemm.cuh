@@ -57,8 +57,8 @@ enum TcBias : int32_t { TC_BIAS_NONE = 0, TC_BIAS_ROW = 1, TC_BIAS_COL = 2 };
 // How the epilogue of a layer-level form moves C, D and Z (chosen on the host from types, alignment and epilogue):
 //   kTcWords     16-bit D, C and Z, M and all leading dimensions multiples of 8, addresses of 16 bytes: 8 rows of a
 //                column per access, blocks of 32 x 32 turned in shared memory.  Long per chunk (activations): 16 warps.
-//   kTcFloats    FP32 D without activation and Z; C (M and its leading dimension multiples of 4, 16-byte aligned) comes
-//                through shared memory by asynchronous copies, a chunk ahead
+//   kTcFloats    FP32 D without activation and Z; C (where M and its leading dimension are multiples of 4 and it is
+//                16-byte aligned) comes through shared memory by asynchronous copies, a chunk ahead
 //   kTcElements  everything else, element by element
 enum TcEpi : int { kTcElements = 0, kTcWords = 1, kTcFloats = 2 };
 
@@ -159,6 +159,11 @@ struct TcParams {
   int32_t col_align;          // kTcRaggedCols: a group's first tile starts at a multiple of this many columns (8
                               // where TMA needs it: B with consecutive columns; columns before the group are not stored)
   const CUtensorMap* maps;    // kTcRaggedDepth: maps of A and B for group g at maps[2g], maps[2g + 1]
+  // kTcRaggedDepth with FP32 results: k-blocks that are added up in tensor memory; longer runs are added to D in parts of
+  // this many, in FP32 registers.  The tensor cores cut every addition off towards zero (against 64 bits: 1.1e-9 of the
+  // sum per element of K, 2.1e-6 after 2048 and 1.9e-5 after 16384; a library product errs the same).
+  int32_t part_blocks;
+  int32_t copy_c;             // kTcFloats: 1 = C (and, in parts, D) can be copied 16 bytes at a time; 0 = element loads
 };
 
 // Group table of the ragged forms, behind the control block: first tile of each group (groups + 1 values), then
@@ -416,13 +421,19 @@ __device__ __forceinline__ void tc_elements_chunk(const TcParams& p, const uint3
 // FP32 results without activation and Z - weight gradients: D = alpha * AB + bias (+ beta * C, from shared memory).
 // Every warp-uniform decision costs a branch and, behind it, an instruction fetch (about 40 cycles); taken once per
 // chunk instead of once per eight columns they made the stores of 537 MB of weight gradients 266 -> 131 us.
-__device__ __forceinline__ void tc_floats_chunk(const TcParams& p, const uint32_t (&v)[32], float* d, float bias_row, uint32_t live,
-                                               uint32_t c_row_shared) {
+__device__ __forceinline__ void tc_floats_chunk(const TcParams& p, const uint32_t (&v)[32], float* d, float beta, float bias_row,
+                                                uint32_t live, uint32_t c_row_shared, const float* c, int64_t c_step) {
   const int64_t step = p.d_sn0;
   float x[32];
+  if (c != nullptr) {                        // C that cannot be copied 16 bytes at a time
+#pragma unroll
+    for (int j = 0; j < 32; ++j) { x[j] = (live >> j) & 1u ? *c : 0.0f; c += c_step; }
+#pragma unroll
+    for (int j = 0; j < 32; ++j) x[j] = fmaf(beta, x[j], fmaf(p.alpha, __uint_as_float(v[j]), bias_row));
+  } else
   if (c_row_shared != 0) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) x[j] = fmaf(p.beta, shared_load_f32(c_row_shared + j * 128), fmaf(p.alpha, __uint_as_float(v[j]), bias_row));
+    for (int j = 0; j < 32; ++j) x[j] = fmaf(beta, shared_load_f32(c_row_shared + j * 128), fmaf(p.alpha, __uint_as_float(v[j]), bias_row));
   } else {
 #pragma unroll
     for (int j = 0; j < 32; ++j) x[j] = fmaf(p.alpha, __uint_as_float(v[j]), bias_row);
@@ -468,7 +479,7 @@ __device__ __forceinline__ void tc_copy_block(const TcParams& p, uint32_t buf, c
   for (int i = 0; i < 8; ++i) {
     const int piece = lane + 32 * i, col = piece >> 3, part = piece & 7;
     const bool ok = ((live >> col) & 1u) && m0 + 4 * part < p.M;
-    async_copy_16(buf + piece * 16, ok ? c_col0 + 4 * part + col * c_step : static_cast<const float*>(p.C), ok ? 16u : 0u);
+    async_copy_16(buf + piece * 16, ok ? c_col0 + 4 * part + col * c_step : static_cast<const float*>(p.D), ok ? 16u : 0u);
   }
 }
 
@@ -1065,7 +1076,7 @@ __global__ void __launch_bounds__(FORM == kTcPlain ? tc_threads(PLANES) : 128 + 
       const long long k_start = clock64();
       const uint64_t g_start = global_timer_ns();
       for (int t = cluster_id; t < num_tiles && ok; t += num_clusters, ++acc_it) {
-        const uint32_t as = two_acc ? (acc_it & 1u) : 0u;
+        uint32_t as = two_acc ? (acc_it & 1u) : 0u;
         const uint32_t aph = (two_acc ? (acc_it >> 1) : acc_it) & 1u;
         if constexpr (PLANES == 1 && !GENERIC && !DBG) {
           if (skew) {
@@ -1143,7 +1154,7 @@ __global__ void __launch_bounds__(FORM == kTcPlain ? tc_threads(PLANES) : 128 + 
           break;
         }
         tc_fence_after_sync();
-        const uint32_t d_base = tmem_base + as * acc_cols;
+        uint32_t d_base = tmem_base + as * acc_cols;
         const int kb0 = FORM == kTcPlain ? (t % p.k_split) * p.kb_per_split : 0;
         int kb1 = FORM == kTcPlain ? min(kb0 + p.kb_per_split, p.k_blocks) : p.k_blocks;
         if constexpr (FORM == kTcRaggedDepth) {
@@ -1158,6 +1169,22 @@ __global__ void __launch_bounds__(FORM == kTcPlain ? tc_threads(PLANES) : 128 + 
         }
         bool first_kb = true;   // the first k-block of a tile (or K-run) overwrites the accumulators
         for (int kb = kb0; kb < kb1; kb += p.kps) {
+          if constexpr (FORM == kTcRaggedDepth && EPI == kTcFloats) {
+            if (kb != kb0 && (kb - kb0) % p.part_blocks == 0) {     // hand this part over, go on in the other accumulators
+              if (elected) umma_commit<CG>(bar_tfull + 8u * as);
+              ++acc_it;
+              as = two_acc ? (acc_it & 1u) : 0u;
+              d_base = tmem_base + as * acc_cols;
+              const bool pgot = mbar_wait(bar_tempty + 8u * as, ((two_acc ? (acc_it >> 1) : acc_it) & 1u) ^ 1u, abort_flag, kTcWaitLimitNs);
+              if (!__all_sync(0xffffffffu, pgot)) {
+                if (reporter) tc_report(p.status, TC_ST_TIMEOUT_MMA);
+                ok = false;
+                break;
+              }
+              tc_fence_after_sync();
+              first_kb = true;
+            }
+          }
           if (prof) t0 = clock64();
           const bool fgot = mbar_wait(bar_full + 8u * s, ph, abort_flag, kTcWaitLimitNs);
           if (prof) { t1 = clock64(); mw += t1 - t0; }
@@ -1250,9 +1277,12 @@ __global__ void __launch_bounds__(FORM == kTcPlain ? tc_threads(PLANES) : 128 + 
         n_lo = tab[p.f.groups + 1 + grp]; n_hi = tab[2 * p.f.groups + 1 + grp];
         n0 += n_lo - n_lo % p.col_align;
       }
-      if constexpr (FORM == kTcRaggedDepth) nothing = tab[p.f.groups + 1 + bt] == tab[2 * p.f.groups + 1 + bt];
-      const uint32_t as = two_acc ? (acc_it & 1u) : 0u;
-      const uint32_t aph = (two_acc ? (acc_it >> 1) : acc_it) & 1u;
+      int parts = 1;                                          // sums handed over by the MMA issuer for this unit
+      if constexpr (FORM == kTcRaggedDepth) {
+        const int depth = tab[2 * p.f.groups + 1 + bt] - tab[p.f.groups + 1 + bt];
+        nothing = depth == 0;
+        if constexpr (EPI == kTcFloats) parts = max(1, ((depth + p.bk - 1) / p.bk + p.part_blocks - 1) / p.part_blocks);
+      }
       if (FORM == kTcPlain && prefetch_c) {
         // While the main loop of this tile runs, pull the tile's part of C into L2: one request per
         // 128-byte line (this warp's 32 rows of one column), columns dealt out to the lanes.
@@ -1281,16 +1311,24 @@ __global__ void __launch_bounds__(FORM == kTcPlain ? tc_threads(PLANES) : 128 + 
           }
         }
       }
-      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + as * acc_cols;
       const bool m_ok = m < p.M;
       float bias_row = 0.0f;
       if (p.bias_axis == TC_BIAS_ROW && m_ok) bias_row = p.bias[m + (FORM == kTcRaggedCols ? grp * p.f.bias_group : 0)];
       const int m_in = m % p.m_div, m_out = m / p.m_div;
       const int64_t d_row = m_in * p.d_sm0 + m_out * p.d_sm1 + bt * p.d_batch + split_off;
       const int64_t c_row = m_in * p.c_sm0 + m_out * p.c_sm1 + bt * p.c_batch;
+      long long e0 = 0, e1 = 0;
+      for (int part = 0; part < parts && ok; ++part) {
+      if (part != 0) ++acc_it;
+      const uint32_t as = two_acc ? (acc_it & 1u) : 0u;
+      const uint32_t aph = (two_acc ? (acc_it >> 1) : acc_it) & 1u;
+      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + as * acc_cols;
+      // kTcFloats: what is added to this part - C, or what the parts before have left in D
+      [[maybe_unused]] const bool adds = has_c || part != 0;
+      [[maybe_unused]] const float* add_row = part != 0 ? static_cast<const float*>(p.D) + d_row : static_cast<const float*>(p.C) + c_row;
+      [[maybe_unused]] const int64_t add_step = part != 0 ? p.d_sn0 : p.c_sn0;
       // One pass over the accumulator stage - or, with the skewed schedule of 512-column tiles, one pass per
       // column block, each behind its own barrier (slot = block).
-      long long e0 = 0, e1 = 0;
       for (int half = 0; half < (skew ? 2 : 1); ++half) {
       const uint32_t hb = skew ? static_cast<uint32_t>(half) : as;
       [[maybe_unused]] const int c_lo = chunk_first + (skew ? half * p.bn : 0), c_hi = skew ? (half + 1) * p.bn : bn_tile;
@@ -1310,8 +1348,7 @@ __global__ void __launch_bounds__(FORM == kTcPlain ? tc_threads(PLANES) : 128 + 
       [[maybe_unused]] auto fetch = [&](int c, uint32_t into, uint4 (&w)[4]) {
         const uint32_t live = live_of(c);
         if constexpr (EPI == kTcFloats) {
-          if (has_c) tc_copy_block(p, stage.base + into, static_cast<const float*>(p.C) + c_row - lane + static_cast<int64_t>(n0 + c) * p.c_sn0, m0,
-                        p.c_sn0, live, lane);
+          if (adds && p.copy_c) tc_copy_block(p, stage.base + into, add_row - lane + (n0 + c) * add_step, m0, add_step, live, lane);
         } else if constexpr (EPI == kTcWords) {
           const uint32_t live_lane = m0 + r8 < p.M ? live >> lc : 0u;
           const int64_t corner = n0 + c + lc;
@@ -1364,7 +1401,9 @@ __global__ void __launch_bounds__(FORM == kTcPlain ? tc_threads(PLANES) : 128 + 
             } else if constexpr (EPI == kTcFloats) {
               async_copy_wait<1>();
               __syncwarp();
-              if (m_ok) tc_floats_chunk(p, v, static_cast<float*>(p.D) + di, bias_row, live, has_c ? stage.base + buf + 4 * lane : 0u);
+              if (m_ok) tc_floats_chunk(p, v, static_cast<float*>(p.D) + di, part != 0 ? 1.0f : p.beta, bias_row, live,
+                                        adds && p.copy_c ? stage.base + buf + 4 * lane : 0u,
+                                        adds && !p.copy_c ? add_row + col0 * add_step : nullptr, add_step);
             } else if (m_ok) {
               const int64_t ci = c_row + static_cast<int64_t>(col0) * p.c_sn0, zi = m + static_cast<int64_t>(col0) * p.f.z_sn;
               if (p.dtype_d == TC_F32)
@@ -1488,6 +1527,7 @@ __global__ void __launch_bounds__(FORM == kTcPlain ? tc_threads(PLANES) : 128 + 
         if constexpr (CG == 2 && FORM != kTcPlain) mbar_arrive_cluster_relaxed(tempty_leader + 8u * hb);
         else if constexpr (CG == 2) mbar_arrive_cluster(tempty_leader + 8u * hb);
         else mbar_arrive(bar_tempty + 8u * hb);
+      }
       }
       }
       if (!ok) break;

@@ -946,3 +946,31 @@ def test_grouped_with_nothing_to_multiply():
     with pytest.raises(GK.ConfigError, match="per row"):
         GK.matmul_grouped(conf(m, total, 64, torch.float16, torch.float32), nan(m, 64, 3), nan(64, total), None, d, offsets,
                           epilogue=Epilogue.Bias(torch.zeros(total, device="cuda"), axis="col"))
+
+
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("counts", [[5000, 2048, 0, 2049], [4096, 100], [2047, 6145]])
+@pytest.mark.parametrize("m", [264, 131])
+def test_long_runs_are_added_up_in_parts(counts, accumulate, m):
+    """FP32 sums over more than 2048 columns: exact on integers, and the error does not grow with the length any more."""
+    g = gen(71)
+    offsets, o = offsets_of(counts, first=1)
+    n, G, total = 520, len(counts), o[-1] + 5
+    dy, x, c = ints(g, m, total), ints(g, n, total), ints(g, m, n, G, dtype=torch.float32, lo=-50, hi=50)
+    d = c.clone(memory_format=torch.preserve_format) if accumulate else cm(torch.full((m, n, G), float("nan"), device="cuda"))
+    call = GK.bind_grouped_outer(conf(m, n, total, torch.float16, torch.float32, tb=True, residual=accumulate), dy, x, d if accumulate else None, d,
+                                 offsets, transform_shared_to_regs_a=Transform.Elementwise(Transform.Scale(2.0)))
+    call()
+    done()
+    for i in range(G):
+        want = 2 * (dy[:, o[i]:o[i + 1]].double() @ x[:, o[i]:o[i + 1]].double().T) + (c[:, :, i].double() if accumulate else 0.0)
+        assert torch.equal(d[:, :, i].double(), want), i
+    dy, x = normal(g, m, total, dtype=torch.bfloat16), normal(g, n, total, dtype=torch.bfloat16)
+    d = cm(torch.zeros(m, n, G, device="cuda"))
+    GK.matmul_grouped_outer(conf(m, n, total, torch.bfloat16, torch.float32, tb=True), dy, x, None, d, offsets)
+    done()
+    for i, count in enumerate(counts):
+        want = dy[:, o[i]:o[i + 1]].double() @ x[:, o[i]:o[i + 1]].double().T
+        mag = dy[:, o[i]:o[i + 1]].double().abs() @ x[:, o[i]:o[i + 1]].double().abs().T
+        # within a part at most one ulp of the running sum per 16 products (128 additions of 2^-23), then one rounding a part
+        assert ((d[:, :, i].double() - want).abs() <= (128 + 4) * 2.0 ** -23 * mag + 1e-30).all(), i
