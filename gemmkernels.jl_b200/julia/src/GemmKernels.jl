@@ -7,8 +7,10 @@ include("vocabulary.jl")
 include("config.jl")
 include("matmul.jl")
 include("blas.jl")
+include("fused.jl")
 
 export Layout, Operator, Transform, Epilogue, Kernel, CTASwizzle
 export Config, ConfigError, get_config, matmul, matmatmul!, mul!, contract!
+export matmul_fused, matmul_grouped, matmul_grouped_outer, activation_gradient!
 
 end

@@ -62,6 +62,7 @@ module Transform
     struct Scale{T}; factor::T; end
     struct ReLU end
     struct GELU end
+    struct SiLU end                                                 # layer-level epilogues only
     struct Cast{T} end
     struct Elementwise{F}; func::F; end
     Elementwise() = Elementwise(identity)
@@ -75,6 +76,17 @@ module Epilogue
         axis::Symbol
     end
     Bias(ptr) = Bias(ptr, :col)
+    # layer-level epilogues (fused.jl); arrays, not pointers
+    Base.@kwdef struct BiasActivationResidual{B, F, Z}              # act(alpha*A*B + bias) + beta*C
+        bias::B = nothing
+        axis::Symbol = :row
+        activation::F = nothing
+        preactivation::Z = nothing
+    end
+    struct ActivationGradient{Z, F}                                 # (alpha*A*B + beta*C) .* act'(Z)
+        preactivation::Z
+        activation::F
+    end
 end
 
 module Kernel                                                       # tags only: one persistent TMA pipeline serves all three

@@ -30,7 +30,7 @@ extern "C" {
 #endif
 
 #define GK_VERSION_MAJOR 0
-#define GK_VERSION_MINOR 2
+#define GK_VERSION_MINOR 3
 
 typedef struct gk_handle_s* gk_handle;
 typedef void* gk_stream; /* a CUstream / cudaStream_t; NULL = the legacy default stream */
@@ -151,7 +151,7 @@ typedef struct gk_epilogue_desc {
 
 typedef struct gk_gemm_plan {
   int32_t kernel;       /* 1 = tcgen05, 2 = FPU (SIMT FFMA), 3 = generic SIMT, 4 = diagonal scale,
-                           5 = contraction gather kernel */
+                           5 = contraction gather kernel, 6 = streaming kernel for a few columns */
   int32_t grid, block, cluster;
   int32_t smem_bytes, tmem_columns;
   int32_t tile_m, tile_n, tile_k, stages; /* tile_k: K elements per pipeline stage */
@@ -345,7 +345,9 @@ GK_API gk_status gk_gemm_host(gk_handle h, const gk_gemm_desc* desc, const void*
  *                       there is), e.g. the weight gradient of expert g.  D_g = d + g * stride_d, C_g = c +
  *                       g * stride_c.  STANDARD form without bias, activation and Z.  A group without columns
  *                       gives beta * C_g.  Nothing outside a group's run is read into its product.
- *                       Fast for trans_a = 0, trans_b = 1 (K strided in both operands).
+ *                       Fast for trans_a = 0, trans_b = 1 (K strided in both operands).  FP32 results over more than
+ *                       2048 columns are added up in parts of 2048, in FP32 registers (the tensor cores cut each
+ *                       addition off towards zero: an error that would grow with the run).
  */
 typedef enum gk_fused_form { GK_FUSED_STANDARD = 0, GK_FUSED_RESIDUAL = 1, GK_FUSED_GRADIENT = 2 } gk_fused_form;
 
