@@ -165,22 +165,24 @@ static bool skinny_plan(gk_handle h, const gk_gemm_desc& d, const gk_group_desc*
   if (d.k < 1 || d.alpha == 0.0 || d.n < 1 || d.m < 1) return false;
   const int64_t groups = gr ? gr->groups : 1;
   const int64_t active = std::min<int64_t>(groups, d.n);
-  // One product: up to four columns (4096 x 4096: 11.8 us here, 15.3 on the tensor cores; eight columns 16.4
-  // in one pass of eight - one CTA per SM for the registers - against 16.1; 8192 x 8192: 51 against 33).
-  // Groups: while the average is one column (64 experts of 2048 x 2048: 16 tokens 25 against 34 us, 64 tokens 76 against
-  // 72, 90 tokens 100 against 84 - a group with several columns streams its matrix several times).
-  if (d.n > (groups > 1 ? 1 : 4) * active || d.n > 4096) return false;
+  if (d.n > 4096) return false;
   SkinnyPlan p;
   auto al = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
   p.any = !al(a) || !al(b) || d.lda % 8 || d.ldb % 8 || d.k % 8 || (!d.trans_a && d.m % 8) || d.trans_b ||
           (gr && groups > 1 && gr->stride_a % 8);
-  // Columns at a time: the average of the groups that can have any, rounded up (a group with more is streamed again, from L2).
-  p.nt = d.n <= active ? 1 : (d.n <= 2 * active ? 2 : 4);
+  // Groups: while the average is one column (64 experts of 2048 x 2048: 16 tokens 25 us, 34 on the tensor cores; 64 tokens
+  // 76 and 72, 90 tokens 100 and 84: a group with more columns is streamed again).  One product: up to 16 columns of a
+  // transposed A (4096 x 4096, 8 columns: 11.0 us, 16.1 on the tensor cores; 16: 13.0 and 16.2), else up to four (4
+  // columns: 11.6 and 15.3 us, 8: 17.1 and 16.3).
+  const bool mma = groups == 1 && d.trans_a && !p.any && d.n > 1;
+  if (d.n > (groups > 1 ? active : mma ? kSkinnyMmaCols : 4)) return false;
+  p.nt = d.n <= active ? 1 : mma ? kSkinnyMmaCols : (d.n <= 2 ? 2 : 4);
   p.items = static_cast<int>(std::min<int64_t>(d.n, d.n / p.nt + active));
   if (groups == 1) p.items = static_cast<int>((d.n + p.nt - 1) / p.nt);
   p.rows = static_cast<int>((d.m + kSkinnyRows - 1) / kSkinnyRows);
   // K is cut as far as the CTAs still run in one round.
-  const int64_t slots = static_cast<int64_t>(p.any ? 2 : skinny_ctas(p.nt)) * h->sm_count;
+  const int ctas = p.nt == kSkinnyMmaCols ? kSkinnyMmaCtas : skinny_ctas(p.nt, p.any);
+  const int64_t slots = static_cast<int64_t>(ctas) * h->sm_count;
   const int64_t steps = (d.k + kSkinnyStep - 1) / kSkinnyStep;
   while (p.ranks < 8 && 2 * p.ranks <= steps && 2 * static_cast<int64_t>(p.rows) * p.items * p.ranks <= slots) p.ranks *= 2;
   p.k_per_rank = static_cast<int>((steps + p.ranks - 1) / p.ranks * kSkinnyStep);
@@ -197,7 +199,8 @@ static const void* skinny_kernel_nt(int nt) {
 
 template <typename T>
 static const void* skinny_kernel(bool k_major, bool any, int nt) {
-  if (k_major) return any ? skinny_kernel_nt<T, true, true>(nt) : skinny_kernel_nt<T, true, false>(nt);
+  if (nt == kSkinnyMmaCols) return reinterpret_cast<const void*>(&skinny_mma_kernel<T>);
+  if (k_major) return any ? skinny_kernel_nt<T, true, true>(nt) : reinterpret_cast<const void*>(&skinny_gemm_kernel<T, true, 1, false>);
   return any ? skinny_kernel_nt<T, false, true>(nt) : skinny_kernel_nt<T, false, false>(nt);
 }
 

@@ -28,7 +28,7 @@ constexpr int kSkinnyRows = 64;        // rows of D per cluster
 constexpr int kSkinnyStep = 256;       // K consumed per step of a CTA (K runs are multiples of it)
 // CTAs per SM, which the registers are limited to: the loads in flight are what hides the latency of HBM (4096 x 4096,
 // one column: 12.3 us with two, 8.3 us with four).
-__host__ __device__ constexpr int skinny_ctas(int nt) { return nt == 1 ? 4 : (nt == 2 ? 3 : 2); }
+__host__ __device__ constexpr int skinny_ctas(int nt, bool any) { return any ? 2 : (nt == 1 ? 4 : (nt == 2 ? 3 : 2)); }
 
 struct SkinnyParams {
   const void* A; const void* B; const void* C; void* D;
@@ -100,8 +100,32 @@ __device__ __forceinline__ int skinny_reduce(float (&v)[V], int lane) {
   return first;
 }
 
+// The end of both kernels: the cluster's sums ([column][row], n columns) are added in rank order, each CTA taking a
+// slice of the outputs, and the epilogue is applied.
+__device__ __forceinline__ void skinny_finish(const SkinnyParams& p, const float* sum, int g, int c0, int n, int row0, uint32_t ranks, uint32_t rank) {
+  __syncthreads();
+  if (ranks > 1) cluster_sync_all();
+  const int outputs = n * kSkinnyRows, mine = (outputs + static_cast<int>(ranks) - 1) / static_cast<int>(ranks);
+  const int first = static_cast<int>(rank) * mine, last = min(first + mine, outputs);
+  const uint32_t sum_addr = smem_u32(sum);
+  for (int o = first + static_cast<int>(threadIdx.x); o < last; o += kSkinnyThreads) {
+    float s = 0.0f;
+    for (uint32_t r = 0; r < ranks; ++r) s += skinny_load_cluster(map_to_cta(sum_addr + 4u * o, r));
+    const int m = row0 + o % kSkinnyRows;
+    if (m >= p.M) continue;
+    const int64_t col = c0 + o / kSkinnyRows;
+    const float bias = p.bias_axis == 1 ? p.bias[m + g * p.f.bias_group] : (p.bias_axis == 2 ? p.bias[col] : 0.0f);
+    fused_put(p.D, m + col * p.ldd, p.dtype_d,
+              fused_finish(p.f, fmaf(p.alpha, s, bias), p.beta, p.C, m + col * p.ldc, p.dtype_d, p.act, m, col));
+  }
+  if (ranks > 1) cluster_sync_all();     // the peers have read this CTA's sums
+}
+
+template <typename T> struct SkinnyIsHalf { static constexpr bool value = false; };
+template <> struct SkinnyIsHalf<__half> { static constexpr bool value = true; };
+
 template <typename T, bool K_MAJOR, int NT, bool ANY>
-__global__ void __launch_bounds__(kSkinnyThreads, ANY ? 2 : skinny_ctas(NT)) skinny_gemm_kernel(const SkinnyParams p) {
+__global__ void __launch_bounds__(kSkinnyThreads, skinny_ctas(NT, ANY)) skinny_gemm_kernel(const SkinnyParams p) {
   constexpr int kOut = kSkinnyRows * NT;
   __shared__ float part[K_MAJOR ? 1 : 8][kOut];   // M_MAJOR: sums of each warp
   __shared__ float sum[kOut];                     // sums of this CTA's K run, [column][row]
@@ -202,21 +226,83 @@ __global__ void __launch_bounds__(kSkinnyThreads, ANY ? 2 : skinny_ctas(NT)) ski
       sum[o] = s;
     }
   }
-  __syncthreads();
-  if (ranks > 1) cluster_sync_all();
-  const int mine = kOut / static_cast<int>(ranks);
-  const uint32_t sum_addr = smem_u32(sum);
-  for (int o = static_cast<int>(rank) * mine + threadIdx.x; o < static_cast<int>(rank + 1) * mine; o += kSkinnyThreads) {
-    float s = 0.0f;
-    for (uint32_t r = 0; r < ranks; ++r) s += skinny_load_cluster(map_to_cta(sum_addr + 4u * o, r));
-    const int t = o / kSkinnyRows, m = row0 + o % kSkinnyRows;
-    if (t >= n || m >= p.M) continue;
-    const int64_t col = c0 + t;
-    const float bias = p.bias_axis == 1 ? p.bias[m + g * p.f.bias_group] : (p.bias_axis == 2 ? p.bias[col] : 0.0f);
-    fused_put(p.D, m + col * p.ldd, p.dtype_d,
-              fused_finish(p.f, fmaf(p.alpha, s, bias), p.beta, p.C, m + col * p.ldc, p.dtype_d, p.act, m, col));
+  skinny_finish(p, sum, g, c0, n, row0, ranks, rank);
+}
+
+// Several columns, up to 16, of A with consecutive k: the same stream with the warp-level matrix instructions (m16n8k16,
+// FP32 accumulators) in place of FMAs - the columns are its 16 rows, eight rows of A its 8 columns - so that the weights
+// need no unpacking and the accumulators of 16 columns fit four registers.  (tcgen05 would want its operands staged in
+// shared memory and tensor memory set up: the latency that this kernel avoids.  The rate is that of the loads: eight
+// columns of a 4096 x 4096 layer 11.0 us against 16.1 with tcgen05.)  Lane 4 * g + t holds k0 + 8 t .. + 7 of row g of the
+// warp's 8 rows and of columns g and g + 8: the instruction's K is permuted, in both operands alike, so that a lane's 16
+// bytes feed two instructions.  (With consecutive rows instead, pairs of k have to be put together by byte permutations
+// and 16 columns need 32 accumulators: 15.7 us, no better than the FMAs below five columns and tcgen05 above.)
+constexpr int kSkinnyMmaCols = 16;
+constexpr int kSkinnyMmaCtas = 4;      // per SM: 64 registers, eight loads of A in flight per thread (three: 13.0 us)
+
+template <typename T>
+__device__ __forceinline__ void skinny_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (SkinnyIsHalf<T>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kSkinnyThreads, kSkinnyMmaCtas) skinny_mma_kernel(const SkinnyParams p) {
+  __shared__ float sum[kSkinnyMmaCols * kSkinnyRows];                                    // [column][row]
+  __shared__ int item[3];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g4 = lane >> 2, t4 = lane & 3;
+  uint32_t ranks;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
+  const uint32_t rank = cluster_cta_rank();
+  const int row0 = static_cast<int>(blockIdx.x / ranks) * kSkinnyRows;
+
+  pdl_launch_dependents();
+  pdl_wait();
+  if (warp == 0) {
+    int g, c0, n;
+    fused_find_item(p.f, blockIdx.y, kSkinnyMmaCols, lane, g, c0, n);
+    if (lane == 0) { item[0] = g; item[1] = c0; item[2] = n; }
   }
-  if (ranks > 1) cluster_sync_all();     // the peers have read this CTA's sums
+  __syncthreads();
+  const int g = item[0], c0 = item[1], n = item[2];
+  if (n == 0) return;    // the list is shorter than the grid; the same for every CTA of the cluster
+
+  const T* A = static_cast<const T*>(p.A) + g * p.a_group;
+  const T* B = static_cast<const T*>(p.B) + c0 * p.b_sn;
+  const int k_begin = static_cast<int>(rank) * p.k_per_rank;
+  const int k_end = min(k_begin + p.k_per_rank, p.K);
+  const T* x0 = B + g4 * p.b_sn;                       // this lane's columns of B (read only if they exist)
+  const T* x1 = B + (g4 + 8) * p.b_sn;
+  const bool has0 = g4 < n, has1 = g4 + 8 < n;
+
+  constexpr int U = 8;                               // steps of 32 k whose loads are in flight together
+  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  const T* a_row = A + static_cast<int64_t>(min(row0 + warp * 8 + g4, p.M - 1)) * p.lda;
+  for (int k = k_begin + t4 * 8; k < k_end + t4 * 8; k += 32 * U) {      // the same count for all lanes
+    uint4 w[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      w[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (k + 32 * i < k_end) w[i] = skinny_load_stream(a_row + k + 32 * i);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {                    // B comes from L1, which the CTA's other warps have filled
+      uint4 u = make_uint4(0u, 0u, 0u, 0u), v = u;
+      if (has0 && k + 32 * i < k_end) u = *reinterpret_cast<const uint4*>(x0 + k + 32 * i);
+      if (has1 && k + 32 * i < k_end) v = *reinterpret_cast<const uint4*>(x1 + k + 32 * i);
+      skinny_mma<T>(acc, u.x, v.x, u.y, v.y, w[i].x, w[i].y);
+      skinny_mma<T>(acc, u.z, v.z, u.w, v.w, w[i].z, w[i].w);
+    }
+  }
+  // acc: columns g4 and g4 + 8, rows 2 * t4 and 2 * t4 + 1 of the warp's
+  const int r = warp * 8 + 2 * t4;
+  sum[g4 * kSkinnyRows + r] = acc[0]; sum[g4 * kSkinnyRows + r + 1] = acc[1];
+  sum[(g4 + 8) * kSkinnyRows + r] = acc[2]; sum[(g4 + 8) * kSkinnyRows + r + 1] = acc[3];
+  skinny_finish(p, sum, g, c0, n, row0, ranks, rank);
 }
 
 }  // namespace gk

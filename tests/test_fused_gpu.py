@@ -974,3 +974,28 @@ def test_long_runs_are_added_up_in_parts(counts, accumulate, m):
         mag = dy[:, o[i]:o[i + 1]].double().abs() @ x[:, o[i]:o[i + 1]].double().abs().T
         # within a part at most one ulp of the running sum per 16 products (128 additions of 2^-23), then one rounding a part
         assert ((d[:, :, i].double() - want).abs() <= (128 + 4) * 2.0 ** -23 * mag + 1e-30).all(), i
+
+
+@pytest.mark.parametrize("n", [2, 5, 8, 9, 15, 16])
+@pytest.mark.parametrize("ta", [False, True])
+@pytest.mark.parametrize("m,k", [(8, 8), (64, 64), (72, 136), (200, 2048), (1000, 520), (4096, 264)])
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+def test_several_columns_stream(m, k, n, ta, dt):
+    g = gen(m + n)
+    a, b, r = ints(g, m, k, dtype=dt), ints(g, k, n, dtype=dt), ints(g, m, n, dtype=torch.float32)
+    bias = ints(g, m, dtype=torch.float32)
+    aw, bw = roomy(cm(a.T) if ta else a, 8), roomy(b, 16)
+    d, z = torch.full_like(r, -9.0), torch.full_like(r, -9.0)
+    cf, epi = conf(m, n, k, dt, torch.float32, ta, residual=True), Epilogue.BiasActivationResidual(bias, activation=ACT["relu"], preactivation=z)
+    assert GK.query(cf, aw, bw, r, d, epilogue=epi).kernel == (6 if ta or n <= 4 else 1)
+    GK.matmul(cf, aw, bw, r, d, epilogue=epi)
+    done()
+    x = a.double() @ b.double() + bias.double()[:, None]
+    assert torch.equal(z.double(), x) and torch.equal(d.double(), x.clamp(min=0) + r.double())
+
+
+@pytest.mark.parametrize("counts", [[3, 0, 2, 7], [16, 1, 0, 15], [17, 0, 0, 0], [1, 33, 2, 0], [4] * 9])
+@pytest.mark.parametrize("ta", [False, True])
+def test_several_columns_per_group_stream(counts, ta):
+    run_grouped(counts, 136, 264, torch.bfloat16, ta, False, tail=1)
+    run_grouped(counts, 520, 1032, torch.float16, ta, False, first=2, tail=1)
