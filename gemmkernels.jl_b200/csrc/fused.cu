@@ -74,8 +74,10 @@ static gk_status validate_fused(const gk_gemm_desc* d, const gk_fused_desc* fu, 
   return GK_OK;
 }
 
-static gk_status check_fused_pointers(const gk_gemm_desc& d, const gk_fused_desc& fu, const void* a, const void* b, const void* c,
-                                      const void* dd) {
+static bool off_element(const void* p, int32_t dtype) { return reinterpret_cast<uintptr_t>(p) % dtype_size(dtype) != 0; }
+
+static gk_status check_fused_pointers(const gk_gemm_desc& d, const gk_fused_desc& fu, const gk_group_desc* gr, const void* a, const void* b,
+                                      const void* c, const void* dd) {
   if (d.m == 0 || d.n == 0) return GK_OK;
   if (!dd) return set_error(GK_ERR_INVALID_ARGUMENT, "D is NULL");
   if (d.k > 0 && d.alpha != 0.0 && (!a || !b)) return set_error(GK_ERR_INVALID_ARGUMENT, "%s is NULL", a ? "B" : "A");
@@ -85,6 +87,14 @@ static gk_status check_fused_pointers(const gk_gemm_desc& d, const gk_fused_desc
   if (fu.form == GK_FUSED_GRADIENT && !fu.z) return set_error(GK_ERR_INVALID_ARGUMENT, "the gradient form needs Z");
   if (fu.form != GK_FUSED_GRADIENT && fu.z && (fu.z == dd || fu.z == c))
     return set_error(GK_ERR_INVALID_ARGUMENT, "Z is kept beside D: it cannot share memory with D or C");
+  const bool has_c = d.layout_c == GK_LAYOUT_DENSE && d.beta != 0.0;
+  if (off_element(a, d.dtype_a) || off_element(b, d.dtype_b) || off_element(dd, d.dtype_d) || (has_c && off_element(c, d.dtype_c)) ||
+      off_element(fu.z, d.dtype_d) || (fu.bias_axis != GK_BIAS_NONE && off_element(fu.bias, GK_F32)))
+    return set_error(GK_ERR_INVALID_ARGUMENT, "an array is not aligned to its element type");
+  // In place, every element is read and written by one thread: the two must be laid out alike.
+  const bool depth = gr && gr->ragged == GK_RAGGED_DEPTH && gr->groups > 1;
+  if ((has_c && c == dd && (d.ldc != d.ldd || (depth && gr->stride_c != gr->stride_d))) || (fu.z == dd && fu.ldz != d.ldd))
+    return set_error(GK_ERR_INVALID_ARGUMENT, "C or Z in place of D must have D's leading dimension and strides");
   return GK_OK;
 }
 
@@ -330,7 +340,7 @@ gk_status gk_gemm_fused(gk_handle h, const gk_gemm_desc* desc, const gk_fused_de
   clear_error();
   gk_status s = validate_fused(desc, fused, groups);
   if (s != GK_OK) return s;
-  if ((s = check_fused_pointers(*desc, *fused, a, b, c, d)) != GK_OK) return s;
+  if ((s = check_fused_pointers(*desc, *fused, groups, a, b, c, d)) != GK_OK) return s;
   if (workspace_bytes < 0 || (workspace_bytes > 0 && !workspace))
     return set_error(GK_ERR_INVALID_ARGUMENT, "workspace_bytes = %lld with a %s workspace", (long long)workspace_bytes, workspace ? "non-NULL" : "NULL");
   if (!h) return set_error(GK_ERR_INVALID_ARGUMENT, "handle is NULL");
@@ -392,6 +402,10 @@ gk_status gk_activation_gradient(gk_handle h, const gk_activation_gradient_desc*
   if (!dz && !db) return set_error(GK_ERR_INVALID_ARGUMENT, "neither dZ nor the bias gradient is wanted");
   if (desc->n > 0 && desc->m > 0 && !dd) return set_error(GK_ERR_INVALID_ARGUMENT, "dD is NULL");
   if (desc->n > 0 && desc->m > 0 && desc->activation != GK_ACT_NONE && !z) return set_error(GK_ERR_INVALID_ARGUMENT, "Z is NULL");
+  if (off_element(dd, desc->dtype) || off_element(z, desc->dtype) || off_element(dz, desc->dtype) || off_element(db, GK_F32))
+    return set_error(GK_ERR_INVALID_ARGUMENT, "an array is not aligned to its element type");
+  if (dz && ((dz == dd && desc->ld_dz != desc->ld_dd) || (dz == z && desc->ld_dz != desc->ld_z)))
+    return set_error(GK_ERR_INVALID_ARGUMENT, "dZ in place of dD or Z must have its leading dimension");
   if (!h) return set_error(GK_ERR_INVALID_ARGUMENT, "handle is NULL");
   if (desc->m == 0 || (desc->n == 0 && !db)) return GK_OK;
   const ActGradPlan pl = actgrad_plan(h->sm_count, *desc, db != nullptr);

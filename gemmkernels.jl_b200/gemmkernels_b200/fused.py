@@ -17,7 +17,7 @@ from . import epilogue as Epilogue
 from . import kernel as Kernel
 from . import transform as Transform
 from .config import Config, ConfigError, DimensionMismatch
-from .matmul import GemmKernelsError, _raise, _workspace_bytes, handle, lend_workspace, lower
+from .matmul import GemmKernelsError, _fold_transforms, _raise, _workspace_bytes, handle, lend_workspace, lower
 
 _ACT = {Transform.Identity: L.GK_ACT_NONE, Transform.ReLU: L.GK_ACT_RELU, Transform.GELU: L.GK_ACT_GELU,
         Transform.SiLU: L.GK_ACT_SILU}
@@ -187,10 +187,12 @@ class BoundFused:
 # ------------------------------------------------------------------------------------------------
 # lowering
 # ------------------------------------------------------------------------------------------------
-def _lower_epilogue(epilogue, act_hook: int, d, m: int, n: int, groups: int):
+def _lower_epilogue(epilogue, hooks: dict, act_hook: int, d, m: int, n: int, groups: int):
     """-> (FusedDesc, bias group stride, arrays to keep alive).  groups == 0: a plain product."""
     import torch
     fu = L.FusedDesc()
+    if not isinstance(epilogue, Epilogue.Default):
+        _fold_transforms(hooks, True)      # refuses what would have to run between the product and the bias, or scale both
     if isinstance(epilogue, Epilogue.Fused) and act_hook != L.GK_ACT_NONE:
         raise Transform.UnsupportedFunctor("the fused epilogues carry their own activation: leave the activation hooks empty")
     bias, axis, z = None, "row", None
@@ -239,7 +241,7 @@ def lower_fused(conf: Config, a, b, c, d, hooks: dict, epilogue, kernel) -> _Cal
     desc, epi, ptrs = lower(conf, a, b, c, d, hooks, Epilogue.Default(), kernel)
     m, n = desc.m, desc.n
     _check_matrices(A=a, B=b, C=c, D=d)
-    fu, _, keep = _lower_epilogue(epilogue, epi.activation, d, m, n, 0)
+    fu, _, keep = _lower_epilogue(epilogue, hooks, epi.activation, d, m, n, 0)
     dev = _one_device(d, a, b, c, *keep)
     return _Call(desc, fu, None, ptrs, dev, (a, b, c, d, epilogue) + keep)
 
@@ -253,7 +255,7 @@ def lower_grouped(conf: Config, a, b, c, d, offsets, hooks: dict, epilogue, kern
     desc, epi, ptrs = lower(conf, a0, b, c, d, hooks, Epilogue.Default(), kernel)
     m, n = desc.m, desc.n
     _check_matrices(B=b, C=c, D=d)
-    fu, stride_bias, keep = _lower_epilogue(epilogue, epi.activation, d, m, n, groups)
+    fu, stride_bias, keep = _lower_epilogue(epilogue, hooks, epi.activation, d, m, n, groups)
     gr = L.GroupDesc(ragged=L.GK_RAGGED_COLUMNS, groups=groups, stride_a=stride_a, stride_bias=stride_bias)
     gr.offsets, gr.offsets_dtype = _offsets(offsets, groups)
     dev = _one_device(d, a, b, c, offsets, *keep)

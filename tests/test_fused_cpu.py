@@ -72,11 +72,22 @@ def test_fused_descriptor_refusals(kw, fu, gr, status, needle):
     (dict(), dict(form=L.GK_FUSED_GRADIENT), {}, "needs Z"),
     (dict(), dict(form=L.GK_FUSED_RESIDUAL, z=0x1000, ldz=64), {}, "share memory"),
     (dict(), {}, dict(ws_bytes=64), "workspace_bytes"),
+    (dict(), {}, dict(a=C.c_void_p(0x1001)), "aligned"),
+    (dict(), {}, dict(dd=C.c_void_p(0x1002)), "aligned"),
+    (dict(), dict(form=L.GK_FUSED_RESIDUAL, z=0x2002, ldz=64), {}, "aligned"),
+    (dict(), dict(bias_axis=L.GK_BIAS_ROW, bias=0x2002), {}, "aligned"),
+    (dict(beta=1.0, ldc=72), {}, dict(c=FAKE), "leading dimension"),
+    (dict(), dict(form=L.GK_FUSED_GRADIENT, z=0x1000, ldz=72), {}, "leading dimension"),
     (dict(), {}, {}, "handle is NULL"),
 ])
 def test_fused_pointer_refusals(kw, fu, ptrs, needle):
     assert call(desc(**kw), L.FusedDesc(**fu), **ptrs) == L.GK_ERR_INVALID_ARGUMENT
     assert needle in L.last_error(), L.last_error()
+
+
+def test_in_place_gradients_need_equal_strides():
+    gr = groups(ragged=L.GK_RAGGED_DEPTH, stride_d=4096, stride_c=8192)
+    assert call(desc(beta=1.0, trans_b=1), gr=gr, c=FAKE) == L.GK_ERR_INVALID_ARGUMENT and "strides" in L.last_error()
 
 
 def test_struct_sizes_are_checked():
@@ -100,6 +111,9 @@ def test_struct_sizes_are_checked():
     (dict(), dict(dz=None, db=None), L.GK_ERR_INVALID_ARGUMENT, "neither"),
     (dict(), dict(dd=None), L.GK_ERR_INVALID_ARGUMENT, "dD is NULL"),
     (dict(), dict(z=None), L.GK_ERR_INVALID_ARGUMENT, "Z is NULL"),
+    (dict(), dict(z=C.c_void_p(0x1001)), L.GK_ERR_INVALID_ARGUMENT, "aligned"),
+    (dict(), dict(db=C.c_void_p(0x1002)), L.GK_ERR_INVALID_ARGUMENT, "aligned"),
+    (dict(ld_dz=72), {}, L.GK_ERR_INVALID_ARGUMENT, "leading dimension"),
     (dict(), {}, L.GK_ERR_INVALID_ARGUMENT, "handle is NULL"),
 ])
 def test_activation_gradient_refusals(kw, ptrs, status, needle):
@@ -145,6 +159,9 @@ def test_fused_epilogue_arguments_are_checked():
     refused(Transform.UnsupportedFunctor, "activation hooks", run(R(), transform_shared_to_global_d=Transform.Elementwise(Transform.ReLU())))
     refused(Transform.UnsupportedFunctor, "Float32", run(R(torch.zeros(64, dtype=torch.float16))))
     refused(GK.DimensionMismatch, "bias", run(R(torch.zeros(63))))
+    scale = Transform.Elementwise(Transform.Scale(2.0))
+    refused(Transform.UnsupportedFunctor, "not fused", run(R(torch.zeros(64)), transform_shared_to_global_d=scale))
+    refused(Transform.UnsupportedFunctor, "before the bias", run(R(torch.zeros(64)), transform_regs_to_shared_d=Transform.Elementwise(Transform.ReLU())))
     refused(GK.DimensionMismatch, "bias", run(R(torch.zeros(64), axis="col")))
     refused(GK.GemmKernelsError, "consecutive", run(R(torch.zeros(128)[::2])))
     refused(GK.GemmKernelsError, "address", run(R(0x1000)))
@@ -171,6 +188,8 @@ def test_grouped_arguments_are_checked():
     refused(GK.ConfigError, "offsets", run(offsets=offsets.float()))
     refused(GK.DimensionMismatch, "bias", run(epilogue=Epilogue.Bias(torch.zeros(64), axis="row")))
     refused(GK.GemmKernelsError, "consecutive", run(epilogue=Epilogue.Bias(torch.zeros(64, 4), axis="row")))
+    refused(Transform.UnsupportedFunctor, "before the bias", run(epilogue=Epilogue.Bias(cm(64, 4, dtype=torch.float32), axis="row"),
+                                                                 transform_regs_to_shared_d=Transform.Elementwise(Transform.ReLU())))
     refused(GK.GemmKernelsError, "column-major", run(a=torch.zeros(64, 32, 4, dtype=torch.float16)))
     refused(GK.GemmKernelsError, "overlapping", run(b=cm(32, 40).as_strided((32, 40), (1, 16))))
     refused(GK.GemmKernelsError, "CUDA", run())

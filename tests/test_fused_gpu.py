@@ -999,3 +999,65 @@ def test_several_columns_stream(m, k, n, ta, dt):
 def test_several_columns_per_group_stream(counts, ta):
     run_grouped(counts, 136, 264, torch.bfloat16, ta, False, tail=1)
     run_grouped(counts, 520, 1032, torch.float16, ta, False, first=2, tail=1)
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("n", [3, 200])
+def test_gradient_epilogue_in_32_bits(n, act):
+    g = gen(81)
+    m, k = 200, 96
+    a, b, z = normal(g, m, k, scale=k ** -0.5), normal(g, k, n), normal(g, m, n, dtype=torch.float32, scale=2.0)
+    d = torch.zeros_like(z)
+    GK.matmul(conf(m, n, k, torch.float16, torch.float32), a, b, None, d, epilogue=Epilogue.ActivationGradient(z, ACT[act]))
+    done()
+    want = (a.double() @ b.double()) * grad64(z.double(), act)
+    mag = a.double().abs() @ b.double().abs()
+    close(d, want, err(k, mag, want) + 16 * 2.0 ** -23 * mag)
+
+
+def test_offsets_of_64_bits_far_outside():
+    g = gen(82)
+    w, x = ints(g, 136, 72, 3), ints(g, 72, 100)
+    offsets = torch.tensor([-2 ** 60, 40, 2 ** 33 + 50, 2 ** 62], device="cuda")      # 2^33 + 50 is 50 in its low 32 bits
+    d = cm(torch.full((136, 100), -9.0, device="cuda"))
+    GK.matmul_grouped(conf(136, 100, 72, torch.float16, torch.float32), w, x, None, d, offsets)
+    done()
+    assert torch.equal(d[:, :40].double(), w[:, :, 0].double() @ x[:, :40].double())
+    assert torch.equal(d[:, 40:].double(), w[:, :, 1].double() @ x[:, 40:].double())
+
+
+@pytest.mark.parametrize("m,n,k,ta", [(300, 257, 1111, False), (520, 1, 1032, True), (520, 7, 1032, True), (77, 2, 45, False), (256, 96, 8192, False)])
+def test_captured_single_products(m, n, k, ta):
+    """Every route of a single product - copies, both streaming kernels, split K - in a graph of its own workspace."""
+    g = gen(83)
+    side = torch.cuda.Stream()
+    made = []
+    for _ in range(2):
+        a, b, r = ints(g, m, k, lo=-1, hi=1), ints(g, k, n, lo=-1, hi=1), ints(g, m, n, dtype=torch.float32)
+        aw = cm(a.T) if ta else a
+        d = torch.zeros_like(r)
+        cf = conf(m, n, k, torch.float16, torch.float32, ta, residual=True)
+        epi = Epilogue.BiasActivationResidual(activation=ACT["relu"])
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            GK.matmul(cf, aw, b, r, d, epilogue=epi)
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            GK.matmul(cf, aw, b, r, d, epilogue=epi)
+        made.append((graph, aw, b, r, d))
+    for _ in range(3):
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        for graph, aw, b, r, d in made:
+            aw.copy_(ints(g, *aw.shape, lo=-1, hi=1))
+            b.copy_(ints(g, k, n, lo=-1, hi=1))
+            d.zero_()
+        torch.cuda.synchronize()
+        for s, (graph, *_) in zip(streams, made):
+            with torch.cuda.stream(s):
+                graph.replay()
+                graph.replay()
+        done()
+        for graph, aw, b, r, d in made:
+            a = aw.T if ta else aw
+            assert torch.equal(d.double(), (a.double() @ b.double()).clamp(min=0) + r.double())
