@@ -325,7 +325,7 @@ gk_status gk_gemm_fused_query(gk_handle h, const gk_gemm_desc* desc, const gk_fu
   TcLaunch L;
   if ((s = tc_plan(h, pr, false, &L)) != GK_OK) return s;
   if (plan->kernel == 0) {
-    plan->kernel = 1; plan->grid = L.grid; plan->block = tc_launch_threads(L); plan->cluster = L.cg;
+    plan->kernel = 1; plan->grid = L.grid; plan->block = tc_threads(1); plan->cluster = L.cg;
     plan->smem_bytes = L.smem_bytes; plan->tmem_columns = static_cast<int32_t>(L.params.tmem_cols);
     plan->tile_m = kTcTileM * L.cg; plan->tile_n = L.params.bn * L.params.n_sub; plan->tile_k = L.params.bk * L.params.kps;
     plan->stages = L.params.stages;

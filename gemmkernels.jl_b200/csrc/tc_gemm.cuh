@@ -56,14 +56,13 @@ enum TcBias : int32_t { TC_BIAS_NONE = 0, TC_BIAS_ROW = 1, TC_BIAS_COL = 2 };
 
 // How the epilogue of a layer-level form moves C, D and Z (chosen on the host from types, alignment and epilogue):
 //   kTcWords     16-bit D, C and Z, M and all leading dimensions multiples of 8, addresses of 16 bytes: 8 rows of a
-//                column per access, blocks of 32 x 32 turned in shared memory.  Long per chunk (activations): 16 warps.
+//                column per access, blocks of 32 x 32 turned in shared memory (12 and 16 epilogue warps were no faster)
 //   kTcFloats    FP32 D without activation and Z; C (where M and its leading dimension are multiples of 4 and it is
 //                16-byte aligned) comes through shared memory by asynchronous copies, a chunk ahead
 //   kTcElements  everything else, element by element
 enum TcEpi : int { kTcElements = 0, kTcWords = 1, kTcFloats = 2 };
 
 enum TcForm : int { kTcPlain = 0, kTcFused = 1, kTcRaggedCols = 2, kTcRaggedDepth = 3 };
-__host__ __device__ constexpr int tc_fused_warps(int form, int epi) { return 8; }
 
 // status word values (0 = ok)
 enum TcStatus : int32_t {
@@ -709,12 +708,10 @@ __device__ __forceinline__ void tc_issue_kblock(uint32_t lo, bool first, uint32_
 // instance every such branch is compiled out, which shortens the per-stage loops of the producer and
 // MMA warps (their cost per pipeline stage is instruction latency, not bandwidth).
 template <int CG, int PLANES, bool TF32, bool RANK5, bool GENERIC = false, bool DBG = false, int FORM = kTcPlain, int EPI = kTcElements>
-__global__ void __launch_bounds__(FORM == kTcPlain ? tc_threads(PLANES) : 128 + 32 * tc_fused_warps(FORM, EPI), 1)
-    tc_gemm_kernel(const __grid_constant__ TcParams p) {
+__global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __grid_constant__ TcParams p) {
   const int dbg = DBG ? p.debug : 0;
   static_assert(!GENERIC || (CG == 1 && PLANES == 1 && !TF32 && !RANK5), "generic loads: one CTA, one plane, 16-bit types");
   static_assert(FORM == kTcPlain || (PLANES == 1 && !TF32 && !RANK5 && !DBG), "fused forms: one plane, 16-bit types");
-  constexpr int kEpiWarps = FORM == kTcPlain ? tc_epilogue_warps(PLANES) : tc_fused_warps(FORM, EPI);
   extern __shared__ uint8_t smem_raw[];
   // 128-byte swizzle atoms are 1024 bytes and the pattern is a function of the address.
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -753,7 +750,7 @@ __global__ void __launch_bounds__(FORM == kTcPlain ? tc_threads(PLANES) : 128 + 
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(bar_tfull + 8u * a, 1);
-      mbar_init(bar_tempty + 8u * a, kEpiWarps * CG);  // one arrival per epilogue warp per CTA
+      mbar_init(bar_tempty + 8u * a, tc_epilogue_warps(PLANES) * CG);  // one arrival per epilogue warp per CTA
     }
     mbar_init(bar_drain, 1);
     *abort_flag = 0;
@@ -1246,7 +1243,7 @@ __global__ void __launch_bounds__(FORM == kTcPlain ? tc_threads(PLANES) : 128 + 
   } else if (warp >= 4) {
     // ------------------------------------------------------------------ epilogue
     const int q = warp & 3;                 // TMEM lane quarter this warp may read
-    const int chunk_step = 32 * (kEpiWarps / 4);
+    const int chunk_step = 32 * (tc_epilogue_warps(PLANES) / 4);
     const int chunk_first = 32 * ((warp - 4) >> 2);
     const uint32_t tempty_leader = (CG == 2) ? map_to_cta(bar_tempty, 0) : bar_tempty;
     uint32_t acc_it = 0;

@@ -65,8 +65,6 @@ struct TcLaunch {
   int smem_bytes = 0;
 };
 
-inline int tc_launch_threads(const TcLaunch& L) { return L.form == kTcPlain ? tc_threads(L.planes) : 128 + 32 * tc_fused_warps(L.form, L.epi); }
-
 // True when the descriptor (and, if given, the operand addresses) can go through TMA + tcgen05.
 bool tc_eligible(const gk_gemm_desc& d, const void* a, const void* b, std::string* why);
 // True when the only obstacle to tc_eligible is TMA's alignment rule (base address, leading dimension,
