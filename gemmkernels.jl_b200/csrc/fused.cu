@@ -182,16 +182,17 @@ static bool skinny_plan(gk_handle h, const gk_gemm_desc& d, const gk_group_desc*
           (gr && groups > 1 && gr->stride_a % 8);
   // Groups: while the average is one column (64 experts of 2048 x 2048: 16 tokens 25 us, 34 on the tensor cores; 64 tokens
   // 76 and 72, 90 tokens 100 and 84: a group with more columns is streamed again).  One product: up to 16 columns of a
-  // transposed A (4096 x 4096, 8 columns: 11.0 us, 16.1 on the tensor cores; 16: 13.0 and 16.2), else up to four (4
-  // columns: 11.6 and 15.3 us, 8: 17.1 and 16.3).
-  const bool mma = groups == 1 && d.trans_a && !p.any && d.n > 1;
-  if (d.n > (groups > 1 ? active : mma ? kSkinnyMmaCols : 4)) return false;
-  p.nt = d.n <= active ? 1 : mma ? kSkinnyMmaCols : (d.n <= 2 ? 2 : 4);
+  // transposed A (4096 x 4096, 8 columns: 11.0 us, 16.1 with tcgen05; 16: 13.0 and 16.2), else up to eight (12.4 and
+  // 16.3-17.2), of these with FMAs up to four (2048 x 2048, 4 columns: 6.0 us, 7.1 with warp-level matrix instructions; 4096 x
+  // 4096: 11.6 and 11.8) and up to four in all where 16-byte loads do not serve.
+  const int mma = groups != 1 || p.any ? 0 : d.trans_a ? (d.n > 1 ? kSkinnyMmaCols : 0) : (d.n > 4 ? kSkinnyMmaRowsCols : 0);
+  if (d.n > (groups > 1 ? active : mma ? mma : 4)) return false;
+  p.nt = d.n <= active ? 1 : mma ? mma : (d.n <= 2 ? 2 : 4);
   p.items = static_cast<int>(std::min<int64_t>(d.n, d.n / p.nt + active));
   if (groups == 1) p.items = static_cast<int>((d.n + p.nt - 1) / p.nt);
   p.rows = static_cast<int>((d.m + kSkinnyRows - 1) / kSkinnyRows);
   // K is cut as far as the CTAs still run in one round.
-  const int ctas = p.nt == kSkinnyMmaCols ? kSkinnyMmaCtas : skinny_ctas(p.nt, p.any);
+  const int ctas = p.nt == kSkinnyMmaCols ? kSkinnyMmaCtas : p.nt == kSkinnyMmaRowsCols ? kSkinnyMmaRowsCtas : skinny_ctas(p.nt, p.any);
   const int64_t slots = static_cast<int64_t>(ctas) * h->sm_count;
   const int64_t steps = (d.k + kSkinnyStep - 1) / kSkinnyStep;
   while (p.ranks < 8 && 2 * p.ranks <= steps && 2 * static_cast<int64_t>(p.rows) * p.items * p.ranks <= slots) p.ranks *= 2;
@@ -210,6 +211,7 @@ static const void* skinny_kernel_nt(int nt) {
 template <typename T>
 static const void* skinny_kernel(bool k_major, bool any, int nt) {
   if (nt == kSkinnyMmaCols) return reinterpret_cast<const void*>(&skinny_mma_kernel<T>);
+  if (nt == kSkinnyMmaRowsCols) return reinterpret_cast<const void*>(&skinny_mma_rows_kernel<T>);
   if (k_major) return any ? skinny_kernel_nt<T, true, true>(nt) : reinterpret_cast<const void*>(&skinny_gemm_kernel<T, true, 1, false>);
   return any ? skinny_kernel_nt<T, false, true>(nt) : skinny_kernel_nt<T, false, false>(nt);
 }

@@ -235,8 +235,7 @@ __global__ void __launch_bounds__(kSkinnyThreads, skinny_ctas(NT, ANY)) skinny_g
 // shared memory and tensor memory set up: the latency that this kernel avoids.  The rate is that of the loads: eight
 // columns of a 4096 x 4096 layer 11.0 us against 16.1 with tcgen05.)  Lane 4 * g + t holds k0 + 8 t .. + 7 of row g of the
 // warp's 8 rows and of columns g and g + 8: the instruction's K is permuted, in both operands alike, so that a lane's 16
-// bytes feed two instructions.  (With consecutive rows instead, pairs of k have to be put together by byte permutations
-// and 16 columns need 32 accumulators: 15.7 us, no better than the FMAs below five columns and tcgen05 above.)
+// bytes feed two instructions.
 constexpr int kSkinnyMmaCols = 16;
 constexpr int kSkinnyMmaCtas = 4;      // per SM: 64 registers, eight loads of A in flight per thread (three: 13.0 us)
 
@@ -302,6 +301,88 @@ __global__ void __launch_bounds__(kSkinnyThreads, kSkinnyMmaCtas) skinny_mma_ker
   const int r = warp * 8 + 2 * t4;
   sum[g4 * kSkinnyRows + r] = acc[0]; sum[g4 * kSkinnyRows + r + 1] = acc[1];
   sum[(g4 + 8) * kSkinnyRows + r] = acc[2]; sum[(g4 + 8) * kSkinnyRows + r + 1] = acc[3];
+  skinny_finish(p, sum, g, c0, n, row0, ranks, rank);
+}
+
+// The same for A with consecutive rows and 5 to 8 columns, which are the instruction's 8 columns here (8 columns of 4096 x
+// 4096: 12.4 us against 16.3-17.2 with tcgen05, of 2048 x 2048: 7.7 and 10.3; 8192 x 2048 and 8192 x 8192: even, within 0.7
+// us; 16 columns would need 32 accumulators: 15.7 us, no better than tcgen05).  Lane 4 * g + t holds
+// rows 8 g .. + 7 at k0 + 2 t, + 1, + 8, + 9; byte permutations put the pairs of k together, and instruction j takes rows
+// 8 g + 2 j and 8 g + 2 j + 1 of every g as its rows g and g + 8.  The warps of a CTA take turns along K.
+constexpr int kSkinnyMmaRowsCols = 8;
+constexpr int kSkinnyMmaRowsCtas = 2;  // per SM: K is cut less (three: 14.4 us at 8 columns of 4096 x 4096; one: 15.7)
+
+template <typename T>
+__global__ void __launch_bounds__(kSkinnyThreads, kSkinnyMmaRowsCtas) skinny_mma_rows_kernel(const SkinnyParams p) {
+  __shared__ float part[8][kSkinnyMmaRowsCols * kSkinnyRows];     // sums of each warp, [column][row]
+  __shared__ float sum[kSkinnyMmaRowsCols * kSkinnyRows];
+  __shared__ int item[3];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g4 = lane >> 2, t4 = lane & 3;
+  uint32_t ranks;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
+  const uint32_t rank = cluster_cta_rank();
+  const int row0 = static_cast<int>(blockIdx.x / ranks) * kSkinnyRows;
+
+  pdl_launch_dependents();
+  pdl_wait();
+  if (warp == 0) {
+    int g, c0, n;
+    fused_find_item(p.f, blockIdx.y, kSkinnyMmaRowsCols, lane, g, c0, n);
+    if (lane == 0) { item[0] = g; item[1] = c0; item[2] = n; }
+  }
+  __syncthreads();
+  const int g = item[0], c0 = item[1], n = item[2];
+  if (n == 0) return;    // the list is shorter than the grid; the same for every CTA of the cluster
+
+  const int k_begin = static_cast<int>(rank) * p.k_per_rank;
+  const int k_end = min(k_begin + p.k_per_rank, p.K);
+  const T* x = static_cast<const T*>(p.B) + (c0 + g4) * p.b_sn;      // this lane's column of B (read only if it exists)
+  const bool has = g4 < n;
+  const int row = row0 + g4 * 8;
+  const T* a_col = static_cast<const T*>(p.A) + g * p.a_group + (row < p.M ? row : 0);   // M is a multiple of 8; rows behind it are not stored
+  float acc[4][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) { acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f; }
+  constexpr int U = 2;                               // steps of 16 k whose loads are in flight together
+  for (int k = k_begin + warp * 16 * U; k < k_end; k += 8 * 16 * U) {
+    uint4 w[U][4];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {                  // k_end is a multiple of 8: pairs of k exist together
+        const int kk = k + 16 * i + 2 * t4 + (h & 1) + 8 * (h >> 1);
+        w[i][h] = make_uint4(0u, 0u, 0u, 0u);
+        if (kk < k_end) w[i][h] = skinny_load_stream(a_col + static_cast<int64_t>(kk) * p.lda);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int kk = k + 16 * i + 2 * t4;
+      uint32_t b0 = 0u, b1 = 0u;
+      if (has && kk < k_end) b0 = *reinterpret_cast<const uint32_t*>(x + kk);
+      if (has && kk + 8 < k_end) b1 = *reinterpret_cast<const uint32_t*>(x + kk + 8);
+      const uint32_t w0[4] = {w[i][0].x, w[i][0].y, w[i][0].z, w[i][0].w}, w1[4] = {w[i][1].x, w[i][1].y, w[i][1].z, w[i][1].w};
+      const uint32_t w2[4] = {w[i][2].x, w[i][2].y, w[i][2].z, w[i][2].w}, w3[4] = {w[i][3].x, w[i][3].y, w[i][3].z, w[i][3].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        skinny_mma<T>(acc[j], __byte_perm(w0[j], w1[j], 0x5410), __byte_perm(w0[j], w1[j], 0x7632), __byte_perm(w2[j], w3[j], 0x5410),
+                      __byte_perm(w2[j], w3[j], 0x7632), b0, b1);
+    }
+  }
+  // acc[j]: rows 8 * g4 + 2 * j and + 1, columns 2 * t4 and 2 * t4 + 1
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int r = 8 * g4 + 2 * j;
+    part[warp][2 * t4 * kSkinnyRows + r] = acc[j][0]; part[warp][(2 * t4 + 1) * kSkinnyRows + r] = acc[j][1];
+    part[warp][2 * t4 * kSkinnyRows + r + 1] = acc[j][2]; part[warp][(2 * t4 + 1) * kSkinnyRows + r + 1] = acc[j][3];
+  }
+  __syncthreads();
+  for (int o = threadIdx.x; o < n * kSkinnyRows; o += kSkinnyThreads) {
+    float s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) s += part[w][o];
+    sum[o] = s;
+  }
   skinny_finish(p, sum, g, c0, n, row0, ranks, rank);
 }
 

@@ -987,7 +987,7 @@ def test_several_columns_stream(m, k, n, ta, dt):
     aw, bw = roomy(cm(a.T) if ta else a, 8), roomy(b, 16)
     d, z = torch.full_like(r, -9.0), torch.full_like(r, -9.0)
     cf, epi = conf(m, n, k, dt, torch.float32, ta, residual=True), Epilogue.BiasActivationResidual(bias, activation=ACT["relu"], preactivation=z)
-    assert GK.query(cf, aw, bw, r, d, epilogue=epi).kernel == (6 if ta or n <= 4 else 1)
+    assert GK.query(cf, aw, bw, r, d, epilogue=epi).kernel == (6 if ta or n <= 8 else 1)
     GK.matmul(cf, aw, bw, r, d, epilogue=epi)
     done()
     x = a.double() @ b.double() + bias.double()[:, None]
