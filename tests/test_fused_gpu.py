@@ -1061,3 +1061,89 @@ def test_captured_single_products(m, n, k, ta):
         for graph, aw, b, r, d in made:
             a = aw.T if ta else aw
             assert torch.equal(d.double(), (a.double() @ b.double()).clamp(min=0) + r.double())
+
+
+@pytest.mark.parametrize("which", ["a", "b", "both"])
+@pytest.mark.parametrize("ta", [False, True])
+@pytest.mark.parametrize("n", [2, 6, 8, 16])
+def test_few_columns_that_start_off_16_bytes(n, ta, which):
+    """Aligned leading dimensions and a base one element off: the plan made without the pointers may not hold."""
+    g = gen(84)
+    m, k = 136, 264
+    a, b = ints(g, m, k), ints(g, k, n)
+
+    def off(t):
+        big = torch.zeros(t.numel() + 8, dtype=t.dtype, device="cuda")
+        view = big[1: 1 + t.numel()].view(t.shape[1], t.shape[0]).T
+        view.copy_(t)
+        return view
+
+    aw = cm(a.T) if ta else a
+    if which != "b":
+        aw = off(aw)
+    bw = off(b) if which != "a" else b
+    d, z = cm(torch.full((m, n), -9.0, device="cuda")), cm(torch.full((m, n), -9.0, device="cuda"))
+    GK.matmul(conf(m, n, k, torch.float16, torch.float32, ta), aw, bw, None, d,
+              epilogue=Epilogue.BiasActivationResidual(activation=ACT["relu"], preactivation=z))
+    done()
+    x = a.double() @ b.double()
+    assert torch.equal(z.double(), x) and torch.equal(d.double(), x.clamp(min=0))
+
+
+@pytest.mark.parametrize("ta", [False, True])
+@pytest.mark.parametrize("n", [5, 7, 8])
+def test_streamed_columns_do_not_mix(n, ta):
+    """A NaN in a column of B, an infinity in a row of A, NaN in the padding of both: each stays where it belongs."""
+    g = gen(85)
+    m, k = 200, 520
+    a, b = ints(g, m, k, lo=1, hi=2), ints(g, k, n, lo=1, hi=2)
+    a[77, 515] = math.inf
+    b[333, 3] = math.nan
+    want = a.double() @ b.double()
+    d = cm(torch.full((m, n), -9.0, device="cuda"))
+    GK.matmul(conf(m, n, k, torch.float16, torch.float32, ta), padded(cm(a.T) if ta else a, 8), padded(b, 16), None, d,
+              epilogue=Epilogue.BiasActivationResidual())
+    done()
+    assert want[77, 0] == math.inf and want[:, 3].isnan().all() and want.isnan().sum() == m
+    assert torch.equal(d.isnan(), want.isnan())
+    assert torch.equal(d.double().nan_to_num(nan=-1.0, posinf=-2.0), want.nan_to_num(nan=-1.0, posinf=-2.0))
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n", [5, 8])
+@pytest.mark.parametrize("form", ["gradient", "residual"])
+def test_streamed_columns_of_any_value(form, n, dt):
+    g = gen(86)
+    m, k = 264, 1032
+    a, b, r = normal(g, m, k, dtype=dt, scale=k ** -0.5), normal(g, k, n, dtype=dt), normal(g, m, n, dtype=dt)
+    d = torch.zeros_like(r)
+    x = a.double() @ b.double()
+    mag = a.double().abs() @ b.double().abs()
+    if form == "gradient":
+        GK.matmul(conf(m, n, k, dt, dt), a, b, None, d, epilogue=Epilogue.ActivationGradient(r, ACT["silu"]))
+        want, more = x * grad64(r.double(), "silu"), 16 * 2.0 ** -23 * mag
+    else:
+        GK.matmul(conf(m, n, k, dt, dt, residual=True), a, b, r, d, epilogue=Epilogue.BiasActivationResidual(activation=ACT["gelu"]))
+        want, more = act64(x, "gelu") + r.double(), 4 * 2.0 ** -23 * (x.abs() + r.double().abs())
+    done()
+    close(d, want, err(k, mag, x) + more)
+
+
+def test_captured_product_of_seven_columns():
+    g = gen(87)
+    m, n, k = 520, 7, 1032
+    a, b = ints(g, m, k), ints(g, k, n)
+    d = cm(torch.zeros(m, n, device="cuda"))
+    cf, epi = conf(m, n, k, torch.float16, torch.float32), Epilogue.BiasActivationResidual(activation=ACT["relu"])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        GK.matmul(cf, a, b, None, d, epilogue=epi)
+    for _ in range(2):
+        a.copy_(ints(g, m, k))
+        d.zero_()
+        graph.replay()
+        graph.replay()
+        done()
+        assert torch.equal(d.double(), (a.double() @ b.double()).clamp(min=0))
