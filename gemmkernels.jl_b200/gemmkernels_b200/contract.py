@@ -11,7 +11,7 @@ import ctypes as C
 
 from . import _lib as L
 from . import arrays
-from .matmul import _raise, handle
+from .matmul import _raise, handle, lent_workspace
 from .operator import TF32
 
 
@@ -73,18 +73,19 @@ def contract_(D, modes_d: str, A, modes_a: str, B, modes_b: str, alpha=1.0, beta
     with torch.cuda.device(dev):
         h = handle(dev)
         s = stream if stream is not None else torch.cuda.current_stream(dev).cuda_stream
+        need = 0
         if workspace is None:
             plan = L.GemmPlan()
             st = L.lib.gk_contract_query(h, C.byref(d), C.byref(plan))
             if st != L.GK_OK:
                 _raise(st)
-            if plan.workspace_bytes:
-                from .matmul import lend_workspace
-                workspace = lend_workspace(D.device, s, plan.workspace_bytes)
-        if workspace is not None:
-            ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-        st = L.lib.gk_contract(h, C.byref(d), A.data_ptr(), B.data_ptr(), C_in.data_ptr() if C_in is not None else None,
-                               D.data_ptr(), ws_ptr, ws_bytes, C.c_void_p(s))
+            need = plan.workspace_bytes
+        with lent_workspace(D.device, s, need) as lent:
+            ws = workspace if workspace is not None else lent
+            if ws is not None:
+                ws_ptr, ws_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
+            st = L.lib.gk_contract(h, C.byref(d), A.data_ptr(), B.data_ptr(), C_in.data_ptr() if C_in is not None else None,
+                                   D.data_ptr(), ws_ptr, ws_bytes, C.c_void_p(s))
     if st != L.GK_OK:
         _raise(st)
     return D

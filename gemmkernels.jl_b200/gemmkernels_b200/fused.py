@@ -9,6 +9,7 @@ neither computed nor written.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 
 from . import _lib as L
@@ -17,7 +18,7 @@ from . import epilogue as Epilogue
 from . import kernel as Kernel
 from . import transform as Transform
 from .config import Config, ConfigError, DimensionMismatch
-from .matmul import GemmKernelsError, _fold_transforms, _raise, _workspace_bytes, handle, lend_workspace, lower
+from .matmul import GemmKernelsError, _fold_transforms, _raise, _workspace_bytes, handle, lent_workspace, lower
 
 _ACT = {Transform.Identity: L.GK_ACT_NONE, Transform.ReLU: L.GK_ACT_RELU, Transform.GELU: L.GK_ACT_GELU,
         Transform.SiLU: L.GK_ACT_SILU}
@@ -124,15 +125,19 @@ class _GradientCall:
         return (h, C.byref(self.desc), *(C.c_void_p(p) for p in self.ptrs), ws, ws_bytes)
 
 
+@contextlib.contextmanager
 def _scratch(device, stream: int, nbytes: int):
     """Workspace of one call: the lent buffer of (device, stream) - or, while the stream is being captured into a
     graph, a buffer of the graph's own, so that two graphs never share one and none points into a buffer that a
     larger one replaces."""
     import torch
-    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device) if stream else torch.cuda.default_stream(device)):
-        if torch.cuda.is_current_stream_capturing():
-            return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    return lend_workspace(device, stream, nbytes)
+    if nbytes:
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device) if stream else torch.cuda.default_stream(device)):
+            if torch.cuda.is_current_stream_capturing():
+                yield torch.empty(nbytes, dtype=torch.uint8, device=device)
+                return
+    with lent_workspace(device, stream, nbytes) as ws:
+        yield ws
 
 
 def _run(call, stream, workspace=None):
@@ -141,12 +146,9 @@ def _run(call, stream, workspace=None):
     with torch.cuda.device(dev):
         h = handle(dev.index)
         s = stream if stream is not None else torch.cuda.current_stream(dev).cuda_stream
-        if workspace is None:
-            need = call.workspace_bytes(h)
-            if need:
-                workspace = _scratch(dev, s, need)
-        ws = workspace.data_ptr() if workspace is not None else None
-        st = call.function(*call.arguments(h, ws, _workspace_bytes(workspace)), s)
+        with _scratch(dev, s, call.workspace_bytes(h) if workspace is None else 0) as lent:
+            ws = workspace if workspace is not None else lent
+            st = call.function(*call.arguments(h, ws.data_ptr() if ws is not None else None, _workspace_bytes(ws)), s)
     if st != L.GK_OK:
         _raise(st)
 

@@ -7,6 +7,7 @@ does not import.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import threading
 
@@ -253,9 +254,17 @@ def _wants_workspace(desc) -> bool:
     return desc.m * desc.n <= (1 << 22) and desc.k >= 2048
 
 
-# Scratch buffers the package lends to gk_gemm when the caller passes none: one per (device, stream),
+# Scratch buffers the package lends to its calls when the caller passes none: one per (device, stream),
 # allocated on first need, replaced only by a larger one, never per call.  Kernels that use a buffer
-# are ordered by the stream it belongs to, so successive calls on that stream may share it.
+# are ordered by the stream it belongs to, so successive calls on that stream may share it - as long as
+# the launches of one call are not mixed with those of another: a call writes its scratch in one launch
+# and reads it in the next, and threads that share a stream (torch's default) would otherwise overwrite
+# each other's in between.  A buffer's lock is therefore held from lending until the call has enqueued.
+class _Scratch:
+    def __init__(self):
+        self.lock, self.buffer = threading.Lock(), None
+
+
 _workspaces: dict = {}
 _workspaces_lock = threading.Lock()
 
@@ -279,13 +288,19 @@ def _check_user_workspace(h, desc, epi, workspace):
         raise GemmKernelsError("workspace must be 256-byte aligned")
 
 
-def lend_workspace(device, stream: int, nbytes: int):
-    """The lent scratch buffer of (device, stream), at least `nbytes` long: allocated on first need,
-    replaced only by a larger one (never per call)."""
+@contextlib.contextmanager
+def lent_workspace(device, stream: int, nbytes: int):
+    """The lent scratch buffer of (device, stream), at least `nbytes` long (None for 0 bytes), for the calls
+    enqueued inside the `with` block; another thread's calls on that stream wait until the block is left."""
     import torch
+    if not nbytes:
+        yield None
+        return
     key = (device.index, int(stream))
     with _workspaces_lock:
-        ws = _workspaces.get(key)
+        scratch = _workspaces.setdefault(key, _Scratch())
+    with scratch.lock:
+        ws = scratch.buffer
         if ws is None or ws.numel() < nbytes:
             size = max(nbytes, 2 * (ws.numel() if ws is not None else 0))
             # allocate under the caller's stream so the caching allocator ties the block to it
@@ -294,19 +309,19 @@ def lend_workspace(device, stream: int, nbytes: int):
             else:
                 with torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=device)):
                     ws = torch.empty(size, dtype=torch.uint8, device=device)
-            _workspaces[key] = ws
-    return ws
+            scratch.buffer = ws
+        yield ws
 
 
-def _auto_workspace(h, desc, epi, like, stream: int):
-    """The lent workspace of (device, stream), grown to the size gk_gemm_query reports, or None."""
+def _auto_workspace_bytes(h, desc, epi) -> int:
+    """What gk_gemm_query reports for a product that can use a workspace, else 0."""
+    if not _wants_workspace(desc):
+        return 0
     plan = L.GemmPlan()
     st = L.lib.gk_gemm_query(h, C.byref(desc), C.byref(epi), C.byref(plan))
     if st != L.GK_OK:
         _raise(st)
-    if not plan.workspace_bytes:
-        return None
-    return lend_workspace(like.device, stream, plan.workspace_bytes)
+    return plan.workspace_bytes
 
 
 def matmul(conf: Config, a, b, c, d, *,
@@ -333,13 +348,16 @@ def matmul(conf: Config, a, b, c, d, *,
     dev = d.device.index if d.device.index is not None else torch.cuda.current_device()
     s = stream if stream is not None else torch.cuda.current_stream(dev).cuda_stream
     with torch.cuda.device(dev):
+        h = handle(dev)
+        need = 0
         if workspace is not None:
-            _check_user_workspace(handle(dev), desc, epi, workspace)
-        elif _wants_workspace(desc):
-            workspace = _auto_workspace(handle(dev), desc, epi, d, s)
-        ws = workspace.data_ptr() if workspace is not None else None
-        st = L.lib.gk_gemm(handle(dev), C.byref(desc), pa, pb, pc, pd, C.byref(epi), ws, _workspace_bytes(workspace),
-                           C.c_void_p(s))
+            _check_user_workspace(h, desc, epi, workspace)
+        else:
+            need = _auto_workspace_bytes(h, desc, epi)
+        with lent_workspace(d.device, s, need) as lent:
+            ws = workspace if workspace is not None else lent
+            st = L.lib.gk_gemm(h, C.byref(desc), pa, pb, pc, pd, C.byref(epi), ws.data_ptr() if ws is not None else None,
+                               _workspace_bytes(ws), C.c_void_p(s))
     if st != L.GK_OK:
         _raise(st)
     return None

@@ -1,0 +1,51 @@
+"""Layer-level operators on the GPU where they are used out of the ordinary: from two threads, on operands and results that
+start anywhere, at the ends of the activations' range.  Integers are exact, other tolerances stand beside their tests."""
+import math
+import threading
+
+import pytest
+import torch
+
+import gemmkernels_b200 as GK
+from gemmkernels_b200 import Epilogue, Transform
+from test_fused_gpu import ACT, cm, conf, done, gen, ints, normal, offsets_of
+
+pytestmark = pytest.mark.gpu
+
+
+def test_threads_that_share_a_stream():
+    """Both enqueue products of a ragged depth (tensor maps, then the product) and split products (partial sums, then their
+    addition) on the default stream, with scratch lent by the package."""
+    g = gen(301)
+    m, n, counts = 128, 256, [100, 0, 65, 3]
+    offsets, o = offsets_of(counts)
+    cf = conf(m, n, o[-1], torch.float16, torch.float32, False, True)
+    cs = conf(256, 64, 8192, torch.float16, torch.float32)
+    sets = []
+    for _ in range(2):
+        a, b = ints(g, m, o[-1]), ints(g, n, o[-1])
+        x, y = ints(g, 256, 8192, lo=-1, hi=1), ints(g, 8192, 64, lo=-1, hi=1)
+        sets.append((a, b, x, y, [(cm(torch.full((m, n, 4), -9.0, device="cuda")), cm(torch.full((256, 64), -9.0, device="cuda"))) for _ in range(40)]))
+    torch.cuda.synchronize()
+    errors = []
+
+    def work(a, b, x, y, outs):
+        try:
+            for d, p in outs:
+                GK.matmul_grouped_outer(cf, a, b, None, d, offsets)
+                GK.matmul(cs, x, y, None, p, epilogue=Epilogue.BiasActivationResidual())
+        except Exception as e:      # noqa: BLE001 - reported by the assertion below
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=s) for s in sets]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    done()
+    assert not errors, errors
+    for a, b, x, y, outs in sets:
+        want = torch.stack([a[:, o[i]:o[i + 1]].double() @ b[:, o[i]:o[i + 1]].double().T for i in range(4)], 2)
+        prod = x.double() @ y.double()
+        for d, p in outs:
+            assert torch.equal(d.double(), want) and torch.equal(p.double(), prod)

@@ -1,0 +1,136 @@
+"""Scratch memory that the package lends to its calls, without a GPU: the entry points run against stand-ins for the
+library's functions and for torch's streams, which record who enqueues when on what buffer."""
+import contextlib
+import ctypes as C
+import importlib
+import threading
+
+import pytest
+import torch
+
+import gemmkernels_b200 as GK
+from gemmkernels_b200 import _lib as L
+from gemmkernels_b200 import Layout, Operator
+
+# (the package's `matmul` is the function, not the module)
+matmul_mod, fused_mod, contract_mod = (importlib.import_module(f"gemmkernels_b200.{m}") for m in ("matmul", "fused", "contract"))
+F16, F32 = GK.Float16, GK.Float32
+
+
+class FakeStream:
+    def __init__(self, cuda_stream=0):
+        self.cuda_stream = cuda_stream
+
+
+@pytest.fixture
+def no_gpu(monkeypatch):
+    """torch's streams and devices as far as the entry points use them; buffers are host tensors."""
+    monkeypatch.setattr(torch.cuda, "device", lambda *a: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "stream", lambda *a: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "ExternalStream", lambda s, device=None: FakeStream(s))
+    monkeypatch.setattr(torch.cuda, "default_stream", lambda *a: FakeStream())
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: FakeStream())
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    for mod in (matmul_mod, fused_mod, contract_mod):
+        monkeypatch.setattr(mod, "handle", lambda *a: C.c_void_p(1))
+    monkeypatch.setattr(matmul_mod, "_workspaces", {})
+
+
+class Recorder:
+    """A library function that enqueues twice, as the calls with scratch do (its contents, then the product), and
+    gives another thread the time to come in between."""
+
+    def __init__(self):
+        self.log, self.met = [], threading.Barrier(2)
+
+    def __call__(self, ws):
+        me = threading.get_ident()
+        self.log.append((me, ws))
+        with contextlib.suppress(threading.BrokenBarrierError):
+            self.met.wait(timeout=0.3)
+        self.log.append((me, ws))
+        return L.GK_OK
+
+
+def two_threads(*calls):
+    errors = []
+
+    def guarded(f):
+        try:
+            f()
+        except Exception as e:      # noqa: BLE001 - reported by the assertion below
+            errors.append(e)
+
+    threads = [threading.Thread(target=guarded, args=(f,)) for f in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+
+
+def cm(*shape, dtype=torch.float16):
+    return torch.zeros(tuple(reversed(shape)), dtype=dtype).permute(*reversed(range(len(shape))))
+
+
+class FakeCall:
+    device = torch.device("cpu")
+
+    def __init__(self, recorder):
+        self.function = lambda ws, n, s: recorder(ws)
+
+    def workspace_bytes(self, h):
+        return 64
+
+    def arguments(self, h, ws, n):
+        return ws, n
+
+
+def entry_point(which, rec, monkeypatch):
+    """A callable (stream) -> None that goes through the entry point with `rec` as the library's function."""
+    def query(*args):
+        args[-1]._obj.workspace_bytes = 4096
+        return L.GK_OK
+
+    if which == "layer":
+        return lambda s: fused_mod._run(FakeCall(rec), s)
+    if which == "product":
+        monkeypatch.setattr(L.lib, "gk_gemm_query", query)
+        monkeypatch.setattr(L.lib, "gk_gemm", lambda h, desc, a, b, c, d, epi, ws, n, s: rec(ws))
+        cf = GK.get_config(gemm_shape=(64, 64, 4096), operator=Operator.TCGen05Operator[F16, F32], global_a_layout=Layout.ColMajor[F16],
+                           global_b_layout=Layout.ColMajor[F16], global_c_layout=Layout.Zero[F32], global_d_layout=Layout.ColMajor[F32])
+        return lambda s: GK.matmul(cf, cm(64, 4096), cm(4096, 64), None, cm(64, 64, dtype=torch.float32), stream=s)
+    monkeypatch.setattr(L.lib, "gk_contract_query", query)
+    monkeypatch.setattr(L.lib, "gk_contract", lambda h, desc, a, b, c, d, ws, n, s: rec(ws))
+    return lambda s: GK.contract_(cm(8, 8, dtype=torch.float32), "ab", cm(8, 8), "ac", cm(8, 8), "cb", stream=s)
+
+
+@pytest.mark.parametrize("which", ["layer", "product", "contraction"])
+def test_calls_of_two_threads_on_one_stream_do_not_mix(which, no_gpu, monkeypatch):
+    """Both write their scratch and read it in a later launch: the pairs must not interleave."""
+    rec = Recorder()
+    call = entry_point(which, rec, monkeypatch)
+    two_threads(lambda: call(5), lambda: call(5))
+    (a, wa), (b, wb), (c, wc), (d, wd) = rec.log
+    assert a == b and c == d and a != c
+    assert wa == wb == wc == wd and wa      # the same buffer: never one per call
+
+
+@pytest.mark.parametrize("which", ["layer", "product", "contraction"])
+def test_streams_have_buffers_of_their_own_and_do_not_wait(which, no_gpu, monkeypatch):
+    rec = Recorder()
+    call = entry_point(which, rec, monkeypatch)
+    two_threads(lambda: call(5), lambda: call(6))
+    assert len(rec.log) == 4 and len({t for t, _ in rec.log[:2]}) == 2 and len({w for _, w in rec.log}) == 2
+
+
+def test_a_call_that_fails_gives_the_buffer_back(no_gpu):
+    def fails(*_):
+        raise RuntimeError("refused")
+
+    call = FakeCall(Recorder())
+    call.function = fails
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="refused"):
+            fused_mod._run(call, 5)
