@@ -9,7 +9,6 @@ neither computed nor written.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 
 from . import _lib as L
@@ -125,28 +124,13 @@ class _GradientCall:
         return (h, C.byref(self.desc), *(C.c_void_p(p) for p in self.ptrs), ws, ws_bytes)
 
 
-@contextlib.contextmanager
-def _scratch(device, stream: int, nbytes: int):
-    """Workspace of one call: the lent buffer of (device, stream) - or, while the stream is being captured into a
-    graph, a buffer of the graph's own, so that two graphs never share one and none points into a buffer that a
-    larger one replaces."""
-    import torch
-    if nbytes:
-        with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device) if stream else torch.cuda.default_stream(device)):
-            if torch.cuda.is_current_stream_capturing():
-                yield torch.empty(nbytes, dtype=torch.uint8, device=device)
-                return
-    with lent_workspace(device, stream, nbytes) as ws:
-        yield ws
-
-
 def _run(call, stream, workspace=None):
     import torch
     dev = call.device
     with torch.cuda.device(dev):
         h = handle(dev.index)
         s = stream if stream is not None else torch.cuda.current_stream(dev).cuda_stream
-        with _scratch(dev, s, call.workspace_bytes(h) if workspace is None else 0) as lent:
+        with lent_workspace(dev, s, call.workspace_bytes(h) if workspace is None else 0) as lent:
             ws = workspace if workspace is not None else lent
             st = call.function(*call.arguments(h, ws.data_ptr() if ws is not None else None, _workspace_bytes(ws)), s)
     if st != L.GK_OK:

@@ -291,26 +291,28 @@ def _check_user_workspace(h, desc, epi, workspace):
 @contextlib.contextmanager
 def lent_workspace(device, stream: int, nbytes: int):
     """The lent scratch buffer of (device, stream), at least `nbytes` long (None for 0 bytes), for the calls
-    enqueued inside the `with` block; another thread's calls on that stream wait until the block is left."""
+    enqueued inside the `with` block; another thread's calls on that stream wait until the block is left.
+    While torch captures the stream into a graph, a buffer of the graph's own instead: two graphs never share one,
+    and none points into a buffer that a larger one replaces."""
     import torch
     if not nbytes:
         yield None
         return
-    key = (device.index, int(stream))
-    with _workspaces_lock:
-        scratch = _workspaces.setdefault(key, _Scratch())
-    with scratch.lock:
-        ws = scratch.buffer
-        if ws is None or ws.numel() < nbytes:
-            size = max(nbytes, 2 * (ws.numel() if ws is not None else 0))
-            # allocate under the caller's stream so the caching allocator ties the block to it
-            if int(stream) == torch.cuda.current_stream(device).cuda_stream:
-                ws = torch.empty(size, dtype=torch.uint8, device=device)
-            else:
-                with torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=device)):
-                    ws = torch.empty(size, dtype=torch.uint8, device=device)
-            scratch.buffer = ws
-        yield ws
+    stream = int(stream)
+    # allocate under the caller's stream so the caching allocator ties the block to it
+    with contextlib.nullcontext() if stream == torch.cuda.current_stream(device).cuda_stream else torch.cuda.stream(
+            torch.cuda.ExternalStream(stream, device=device) if stream else torch.cuda.default_stream(device)):
+        if torch.cuda.is_current_stream_capturing():
+            yield torch.empty(nbytes, dtype=torch.uint8, device=device)
+            return
+        with _workspaces_lock:
+            scratch = _workspaces.setdefault((device.index, stream), _Scratch())
+        with scratch.lock:
+            ws = scratch.buffer
+            if ws is None or ws.numel() < nbytes:
+                ws = torch.empty(max(nbytes, 2 * (ws.numel() if ws is not None else 0)), dtype=torch.uint8, device=device)
+                scratch.buffer = ws
+            yield ws
 
 
 def _auto_workspace_bytes(h, desc, epi) -> int:

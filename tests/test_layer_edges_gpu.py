@@ -49,3 +49,29 @@ def test_threads_that_share_a_stream():
         prod = x.double() @ y.double()
         for d, p in outs:
             assert torch.equal(d.double(), want) and torch.equal(p.double(), prod)
+
+
+def test_two_graphs_of_split_products_replayed_at_once():
+    """Plain products whose K is split, captured into two graphs on one stream and replayed on two."""
+    g = gen(302)
+    m, n, k = 256, 64, 16384
+    cf = conf(m, n, k, torch.float16, torch.float32)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    made = []
+    for _ in range(2):
+        a, b = ints(g, m, k, lo=-1, hi=1), ints(g, k, n, lo=-1, hi=1)
+        d = cm(torch.full((m, n), -9.0, device="cuda"))
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            for _ in range(20):
+                GK.matmul(cf, a, b, None, d)
+        made.append((graph, a, b, d))
+    other = torch.cuda.Stream()
+    for (graph, *_), s in zip(made, (side, other)):
+        with torch.cuda.stream(s):
+            graph.replay()
+    done()
+    for _, a, b, d in made:
+        assert torch.equal(d.double(), a.double() @ b.double())

@@ -134,3 +134,31 @@ def test_a_call_that_fails_gives_the_buffer_back(no_gpu):
     for _ in range(2):
         with pytest.raises(RuntimeError, match="refused"):
             fused_mod._run(call, 5)
+
+
+@pytest.mark.parametrize("which", ["layer", "product", "contraction"])
+def test_captured_calls_have_scratch_of_their_own(which, no_gpu, monkeypatch):
+    """A buffer that two graphs share would be written by both when they are replayed at the same time, and one that a graph's
+    memory pool holds must not be lent to calls outside the graph."""
+    capturing, seen, kept = [False], [], []
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    real_empty = torch.empty
+
+    def empty(*size, **kw):
+        t = real_empty(*size, **kw)
+        if kw.get("dtype") == torch.uint8:
+            kept.append(t)                   # alive, so that no two buffers can have one address
+        return t
+
+    monkeypatch.setattr(torch, "empty", empty)
+    call = entry_point(which, lambda ws: seen.append(ws) or L.GK_OK, monkeypatch)
+    for state in (False, True, True, False):
+        capturing[0] = state
+        call(5)
+    eager, first, second, again = seen
+    assert eager == again and len({eager, first, second}) == 3 and all(seen)
+    capturing[0] = True
+    call(7)                                  # the first call on a stream is a captured one
+    capturing[0] = False
+    call(7)
+    assert seen[-1] != seen[-2]
