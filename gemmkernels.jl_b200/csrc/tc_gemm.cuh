@@ -471,14 +471,15 @@ struct TcStage {
 };
 
 // kTcFloats: starts the copies of the 32 x 32 block of C at rows m0, columns col0 into `buf` (columns of 128 bytes),
-// eight 16-byte pieces per lane.
-__device__ __forceinline__ void tc_copy_block(const TcParams& p, uint32_t buf, const float* c_col0, int m0, int64_t c_step, uint32_t live,
-                                              int lane) {
+// eight 16-byte pieces per lane.  `base`: the matrix itself, 16-byte aligned; it stands in as the address of pieces that do
+// not exist (nothing is read there, but every address must be aligned, and D's need not be).
+__device__ __forceinline__ void tc_copy_block(const TcParams& p, uint32_t buf, const void* base, const float* c_col0, int m0, int64_t c_step,
+                                              uint32_t live, int lane) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int piece = lane + 32 * i, col = piece >> 3, part = piece & 7;
     const bool ok = ((live >> col) & 1u) && m0 + 4 * part < p.M;
-    async_copy_16(buf + piece * 16, ok ? c_col0 + 4 * part + col * c_step : static_cast<const float*>(p.D), ok ? 16u : 0u);
+    async_copy_16(buf + piece * 16, ok ? static_cast<const void*>(c_col0 + 4 * part + col * c_step) : base, ok ? 16u : 0u);
   }
 }
 
@@ -1345,7 +1346,7 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
       [[maybe_unused]] auto fetch = [&](int c, uint32_t into, uint4 (&w)[4]) {
         const uint32_t live = live_of(c);
         if constexpr (EPI == kTcFloats) {
-          if (adds && p.copy_c) tc_copy_block(p, stage.base + into, add_row - lane + (n0 + c) * add_step, m0, add_step, live, lane);
+          if (adds && p.copy_c) tc_copy_block(p, stage.base + into, part != 0 ? p.D : p.C, add_row - lane + (n0 + c) * add_step, m0, add_step, live, lane);
         } else if constexpr (EPI == kTcWords) {
           const uint32_t live_lane = m0 + r8 < p.M ? live >> lc : 0u;
           const int64_t corner = n0 + c + lc;

@@ -75,3 +75,32 @@ def test_two_graphs_of_split_products_replayed_at_once():
     done()
     for _, a, b, d in made:
         assert torch.equal(d.double(), a.double() @ b.double())
+
+
+def shifted(t, by=1, extra=0):
+    """The same matrix (rows, cols[, groups]) `by` elements behind a 16-byte boundary, `extra` elements between its columns."""
+    rows, cols, groups = (*t.shape, 1)[:3]
+    ld = rows + extra
+    buf = torch.full((groups * ld * cols + by + 8,), float("nan"), dtype=t.dtype, device="cuda")
+    view = buf[by:].as_strided((rows, cols, groups), (1, ld, ld * cols))
+    view.copy_(t if t.dim() == 3 else t[:, :, None])
+    return view if t.dim() == 3 else view[:, :, 0]
+
+
+@pytest.mark.parametrize("by", [1, 2, 3])
+@pytest.mark.parametrize("m,n", [(132, 40), (300, 129), (512, 257)])
+@pytest.mark.parametrize("kind", ["residual", "standard", "grouped"])
+def test_results_in_32_bits_that_start_off_16_bytes(kind, m, n, by):
+    """C aligned, D not: C is copied 16 bytes at a time, D is stored element by element."""
+    g = gen(303 + by)
+    k = 72
+    a, b, c = ints(g, m, k), ints(g, k, n), ints(g, m, n, dtype=torch.float32, hi=50)
+    d = shifted(torch.full((m, n), -9.0, device="cuda"), by)
+    cf = conf(m, n, k, torch.float16, torch.float32, residual=True)
+    if kind == "grouped":
+        offsets, _ = offsets_of([n])
+        GK.matmul_grouped(cf, a[:, :, None], b, c, d, offsets)
+    else:
+        GK.matmul(cf, a, b, c, d, epilogue=Epilogue.BiasActivationResidual() if kind == "residual" else Epilogue.Default())
+    done()
+    assert torch.equal(d.double(), a.double() @ b.double() + c.double())
