@@ -1346,7 +1346,8 @@ __global__ void __launch_bounds__(tc_threads(PLANES), 1) tc_gemm_kernel(const __
       [[maybe_unused]] auto fetch = [&](int c, uint32_t into, uint4 (&w)[4]) {
         const uint32_t live = live_of(c);
         if constexpr (EPI == kTcFloats) {
-          if (adds && p.copy_c) tc_copy_block(p, stage.base + into, part != 0 ? p.D : p.C, add_row - lane + (n0 + c) * add_step, m0, add_step, live, lane);
+          // (A chunk without columns has no copies: nothing would wait for their zeros before its buffer is filled again.)
+          if (adds && p.copy_c && live != 0u) tc_copy_block(p, stage.base + into, part != 0 ? p.D : p.C, add_row - lane + (n0 + c) * add_step, m0, add_step, live, lane);
         } else if constexpr (EPI == kTcWords) {
           const uint32_t live_lane = m0 + r8 < p.M ? live >> lc : 0u;
           const int64_t corner = n0 + c + lc;

@@ -104,3 +104,18 @@ def test_results_in_32_bits_that_start_off_16_bytes(kind, m, n, by):
         GK.matmul(cf, a, b, c, d, epilogue=Epilogue.BiasActivationResidual() if kind == "residual" else Epilogue.Default())
     done()
     assert torch.equal(d.double(), a.double() @ b.double() + c.double())
+
+
+@pytest.mark.parametrize("m,n", [(264, 72), (100, 40), (1032, 200)])
+def test_accumulation_in_tiles_that_end_early(m, n):
+    """Many tiles per CTA whose last chunks of 32 columns, and whose last warps, have nothing to add: each buffer of C is
+    filled again by the next tile."""
+    g = gen(310)
+    counts = [(7 * i) % 23 for i in range(300)]
+    offsets, o = offsets_of(counts)
+    a, b = ints(g, m, o[-1]), ints(g, n, o[-1])
+    c = ints(g, m, n, 300, dtype=torch.float32, lo=-50, hi=50)
+    want = c.double() + torch.stack([a[:, o[i]:o[i + 1]].double() @ b[:, o[i]:o[i + 1]].double().T for i in range(300)], 2)
+    GK.matmul_grouped_outer(conf(m, n, o[-1], torch.float16, torch.float32, False, True, True), a, b, c, c, offsets)
+    done()
+    assert torch.equal(c.double(), want)
