@@ -356,7 +356,9 @@ gk_status gk_gemm_fused(gk_handle h, const gk_gemm_desc* desc, const gk_fused_de
   if (skinny_plan(h, *desc, groups, a, b, &sp)) return launch_skinny(sp, *desc, *fused, groups, pr, a, b, c, d, st);
   const FusedFeed feed = fused_feed(*desc, groups, a, b);
   const int64_t copies = feed.bytes();
-  pr.generic = !feed.possible || (copies > 0 && (workspace_bytes < copies || (reinterpret_cast<uintptr_t>(workspace) & 255)));
+  // A ragged depth multiplies copies through tensor maps, which need their room behind them: decided before anything is enqueued.
+  const int64_t maps = pr.form == kTcRaggedDepth ? static_cast<int64_t>(groups->groups) * kTcDepthMapsBytes : 0;
+  pr.generic = !feed.possible || (copies > 0 && (workspace_bytes < copies + maps || (reinterpret_cast<uintptr_t>(workspace) & 255)));
   if (!pr.generic && copies > 0) {
     char* ws = static_cast<char*>(workspace);
     gk_gemm_desc e = *desc;

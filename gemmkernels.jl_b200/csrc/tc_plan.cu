@@ -743,7 +743,7 @@ int tc_choose_k_split(const TcProblem& pr, const TcLaunch& L, int sm_count) {
 
 int64_t tc_depth_maps_bytes(const TcLaunch& L) {
   if (L.form != kTcRaggedDepth || L.generic || L.params.k_blocks == 0) return 0;
-  return static_cast<int64_t>(L.params.f.groups) * 2 * sizeof(CUtensorMap);
+  return static_cast<int64_t>(L.params.f.groups) * kTcDepthMapsBytes;
 }
 
 gk_status tc_write_depth_maps(TcLaunch* L, void* workspace, cudaStream_t stream) {

@@ -78,6 +78,7 @@ gk_status tc_plan(gk_handle h, const TcProblem& pr, bool encode, TcLaunch* out);
 gk_status tc_launch(const TcLaunch& L, cudaStream_t stream);
 // kTcRaggedDepth: bytes of 256-byte aligned workspace for the groups' tensor maps (0: the plan needs none), and the
 // launch that writes them before tc_launch; sets L's map pointer.
+constexpr int64_t kTcDepthMapsBytes = 2 * sizeof(CUtensorMap);      // per group
 int64_t tc_depth_maps_bytes(const TcLaunch& L);
 gk_status tc_write_depth_maps(TcLaunch* L, void* workspace, cudaStream_t stream);
 // Runs the planned product `L` of `pr`.  Given a 256-byte aligned workspace, a product with few output

@@ -119,3 +119,27 @@ def test_accumulation_in_tiles_that_end_early(m, n):
     GK.matmul_grouped_outer(conf(m, n, o[-1], torch.float16, torch.float32, False, True, True), a, b, c, c, offsets)
     done()
     assert torch.equal(c.double(), want)
+
+
+@pytest.mark.parametrize("room", ["query", "copies - 256", "copies", "copies + 256", "copies + maps - 256", "copies + maps", "lent"])
+@pytest.mark.parametrize("which", ["a", "b", "both"])
+def test_ragged_depth_of_operands_off_16_bytes(which, room):
+    """Many groups of small matrices, whose tensor maps are larger than the padded copies: whatever room there is, the call
+    computes the product (the bounds-checked loads need none)."""
+    g = gen(311)
+    groups, m, n = 64, 64, 64
+    offsets, o = offsets_of([1] * groups)
+    a, b = ints(g, m, o[-1]), ints(g, n, o[-1])
+    want = torch.stack([torch.outer(a[:, i].double(), b[:, i].double()) for i in range(groups)], 2)
+    aw, bw = shifted(a) if which != "b" else a, shifted(b) if which != "a" else b
+    cf = conf(m, n, o[-1], torch.float16, torch.float32, False, True)
+    maps, copies = groups * 256, 64 * 64 * 2 * (2 if which == "both" else 1)
+    for out in (torch.float32, torch.float16):
+        cf = conf(m, n, o[-1], torch.float16, out, False, True)
+        d = cm(torch.full((m, n, groups), -9.0, device="cuda", dtype=out))
+        size = GK.grouped_query(cf, aw, bw, None, d, offsets).workspace_bytes if room == "query" else \
+            None if room == "lent" else eval(room, dict(copies=copies, maps=maps))
+        ws = None if size is None else torch.empty(size, dtype=torch.uint8, device="cuda")
+        GK.matmul_grouped_outer(cf, aw, bw, None, d, offsets, workspace=ws)
+        done()
+        assert torch.equal(d.double(), want)
