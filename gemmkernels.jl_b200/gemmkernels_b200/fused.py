@@ -81,9 +81,18 @@ class _Call:
     def _group_ref(self):
         return C.byref(self.groups) if self.groups is not None else None
 
+    def _off_16_bytes(self):
+        return (self.ptrs[0] or 0) % 16, (self.ptrs[1] or 0) % 16
+
     def query(self, h) -> L.GemmPlan:
+        # The query has no addresses and takes them to be 16-byte aligned.  An operand that is not is planned (and its copy
+        # sized) like one whose leading dimension is no multiple of 8.
+        desc = L.GemmDesc.from_buffer_copy(self.desc)
+        off_a, off_b = self._off_16_bytes()
+        desc.lda += off_a != 0 and desc.lda % 8 == 0
+        desc.ldb += off_b != 0 and desc.ldb % 8 == 0
         plan = L.GemmPlan()
-        st = L.lib.gk_gemm_fused_query(h, C.byref(self.desc), C.byref(self.fused), self._group_ref(), C.byref(plan))
+        st = L.lib.gk_gemm_fused_query(h, C.byref(desc), C.byref(self.fused), self._group_ref(), C.byref(plan))
         if st != L.GK_OK:
             _raise(st)
         return plan
@@ -91,7 +100,7 @@ class _Call:
     def workspace_bytes(self, h) -> int:
         d, gr = self.desc, self.groups
         ragged = gr.ragged if gr is not None else 0
-        aligned = d.lda % 8 == 0 and d.ldb % 8 == 0 and (gr is None or gr.stride_a % 8 == 0)
+        aligned = d.lda % 8 == 0 and d.ldb % 8 == 0 and (gr is None or gr.stride_a % 8 == 0) and self._off_16_bytes() == (0, 0)
         if aligned and ragged == L.GK_RAGGED_COLUMNS:
             return 0
         if aligned and ragged == 0 and not (d.m * d.n <= (1 << 22) and d.k >= 2048):

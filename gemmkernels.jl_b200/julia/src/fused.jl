@@ -52,11 +52,22 @@ function product_desc(conf::Config, a, b, c, d, alpha, beta)
                alpha, beta, conf.tile_n, conf.cta_group, conf.stages, conf.raster_group, 0, 0, 0, 0, 0, conf.k_blocks_per_stage, 0, 0, 0, 0)
 end
 
+# The query has no addresses and takes them to be 16-byte aligned: an operand that is not is asked for with a leading
+# dimension that is no multiple of 8.
+function query_desc(desc, a, b)
+    off(x) = x !== nothing && UInt(reinterpret(UInt, pointer(x))) % 16 != 0
+    odd(ld) = ld + (ld % 8 == 0)
+    fields = map(fieldnames(GkGemmDesc)) do f
+        f === :lda && off(a) ? odd(desc.lda) : f === :ldb && off(b) ? odd(desc.ldb) : getfield(desc, f)
+    end
+    GkGemmDesc(fields...)
+end
+
 function enqueue_fused(desc, fused, groups, a, b, c, d)
     g = groups === nothing ? Ptr{GkGroupDesc}(0) : groups
     plan = Ref(GkGemmPlan(0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0))
     gk_check(ccall((:gk_gemm_fused_query, libgk), Cint, (Ptr{Cvoid}, Ref{GkGemmDesc}, Ref{GkFusedDesc}, Ptr{GkGroupDesc}, Ref{GkGemmPlan}),
-                   gk_handle(), desc, fused, g, plan))
+                   gk_handle(), query_desc(desc, a, b), fused, g, plan))
     bytes = plan[].workspace_bytes
     ws = bytes > 0 ? reinterpret(CuPtr{Cvoid}, pointer(lent_workspace(bytes))) : CU_NONE
     gk_check(ccall((:gk_gemm_fused, libgk), Cint,

@@ -380,7 +380,9 @@ typedef struct gk_group_desc {
  * and the 256-byte aligned workspace it can use: REQUIRED for a ragged depth with K strided in both operands (the
  * groups' tensor maps); optional for operands whose columns are not 16-byte aligned (they are copied with padded
  * columns; without the room, bounds-checked loads read them, several times slower) and for a plain fused product
- * with few output tiles and a long K (cut along K); none otherwise. */
+ * with few output tiles and a long K (cut along K); none otherwise.  The query has no addresses and takes them to be
+ * 16-byte aligned; for an A or B that is not, ask with a leading dimension that is no multiple of 8 (one more): the
+ * copy's size does not depend on it. */
 GK_API gk_status gk_gemm_fused_query(gk_handle h, const gk_gemm_desc* desc, const gk_fused_desc* fused,
                                      const gk_group_desc* groups, gk_gemm_plan* plan);
 

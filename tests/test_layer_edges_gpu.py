@@ -143,3 +143,41 @@ def test_ragged_depth_of_operands_off_16_bytes(which, room):
         GK.matmul_grouped_outer(cf, aw, bw, None, d, offsets, workspace=ws)
         done()
         assert torch.equal(d.double(), want)
+
+
+@pytest.mark.parametrize("which", ["a", "b", "both"])
+@pytest.mark.parametrize("kind", ["fused", "grouped", "outer"])
+def test_operands_off_16_bytes_are_given_room_for_their_copies(kind, which):
+    """Views such as x[1:] whose columns are a multiple of 16 bytes apart."""
+    g = gen(312)
+    m, k, n = 136, 264, 96
+    a, b = ints(g, m, k), ints(g, k, n)
+    if kind == "outer":
+        b = ints(g, n, k)
+    aw, bw = shifted(a) if which != "b" else a, shifted(b) if which != "a" else b
+    room = (m * k * 2 + 255) // 256 * 256 * (which != "b") + (n * k * 2 + 255) // 256 * 256 * (which != "a")
+    if kind == "fused":
+        d = cm(torch.full((m, n), -9.0, device="cuda"))
+        cf, epi = conf(m, n, k, torch.float16, torch.float32), Epilogue.BiasActivationResidual()
+        assert GK.query(cf, aw, bw, None, d, epilogue=epi).workspace_bytes == room
+        for run in (lambda: GK.matmul(cf, aw, bw, None, d, epilogue=epi), GK.bind(cf, aw, bw, None, d, epilogue=epi)):
+            d.fill_(-9)
+            run()
+            done()
+            assert torch.equal(d.double(), a.double() @ b.double())
+    elif kind == "grouped":
+        d = cm(torch.full((m, n), -9.0, device="cuda"))
+        offsets, _ = offsets_of([n])
+        cf = conf(m, n, k, torch.float16, torch.float32)
+        assert GK.grouped_query(cf, aw[:, :, None], bw, None, d, offsets).workspace_bytes == room
+        GK.matmul_grouped(cf, aw[:, :, None], bw, None, d, offsets)
+        done()
+        assert torch.equal(d.double(), a.double() @ b.double())
+    else:
+        d = cm(torch.full((m, n, 2), -9.0, device="cuda"))
+        offsets, o = offsets_of([100, 164])
+        cf = conf(m, n, k, torch.float16, torch.float32, False, True)
+        assert GK.grouped_query(cf, aw, bw, None, d, offsets).workspace_bytes == room + 2 * 256
+        GK.matmul_grouped_outer(cf, aw, bw, None, d, offsets)
+        done()
+        assert torch.equal(d.double(), torch.stack([a[:, i:j].double() @ b[:, i:j].double().T for i, j in ((0, 100), (100, 264))], 2))

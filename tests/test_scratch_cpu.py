@@ -162,3 +162,28 @@ def test_captured_calls_have_scratch_of_their_own(which, no_gpu, monkeypatch):
     capturing[0] = False
     call(7)
     assert seen[-1] != seen[-2]
+
+
+@pytest.mark.parametrize("off_a,off_b", [(0, 0), (2, 0), (0, 14), (8, 6)])
+@pytest.mark.parametrize("bound", [False, True])
+def test_room_for_the_copies_of_operands_off_16_bytes(off_a, off_b, bound, no_gpu, monkeypatch):
+    """Aligned leading dimensions, a base between two 16-byte boundaries: the call asks for such a product, and gets the room."""
+    asked, got = [], []
+
+    def query(h, desc, fused, groups, plan):
+        d = desc._obj
+        asked.append((d.lda % 8 != 0, d.ldb % 8 != 0))
+        plan._obj.workspace_bytes = 512 * (d.lda % 8 != 0) + 1024 * (d.ldb % 8 != 0)
+        return L.GK_OK
+
+    monkeypatch.setattr(L.lib, "gk_gemm_fused_query", query)
+    desc = L.GemmDesc(m=64, n=64, k=64, lda=64, ldb=64, ldd=64, alpha=1.0)
+    call = fused_mod._Call(desc, L.FusedDesc(), None, (0x1000 + off_a, 0x2000 + off_b, None, 0x3000), torch.device("cpu"), ())
+    call.function = lambda h, desc, fu, gr, a, b, c, d, ws, n, s: got.append(n.value if bound else n) or L.GK_OK
+    if bound:
+        fused_mod.BoundFused(call)(5)
+    else:
+        fused_mod._run(call, 5)
+    want = 512 * (off_a != 0) + 1024 * (off_b != 0)
+    assert got == [want] and (not want or asked == [(off_a != 0, off_b != 0)])
+    assert (desc.lda, desc.ldb) == (64, 64)
