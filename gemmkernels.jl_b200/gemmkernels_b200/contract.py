@@ -11,7 +11,7 @@ import ctypes as C
 
 from . import _lib as L
 from . import arrays
-from .matmul import _raise, handle, lent_workspace
+from .matmul import BoundScratch, _raise, handle, lent_workspace
 from .operator import TF32
 
 
@@ -92,7 +92,7 @@ def contract_(D, modes_d: str, A, modes_a: str, B, modes_b: str, alpha=1.0, beta
 
 
 class BoundContraction:
-    """`contract_` with its descriptor built once (and its workspace allocated once): calling the
+    """`contract_` with its descriptor built once (and its workspace allocated once per stream): calling the
     object enqueues the same contraction again for the cost of one FFI call."""
 
     def __init__(self, D, modes_d, A, modes_a, B, modes_b, alpha=1.0, beta=0.0, C_in=None, *, compute=None,
@@ -102,6 +102,7 @@ class BoundContraction:
             C_in = D
         self.desc = _desc(D, modes_d, A, modes_a, B, modes_b, alpha, beta, C_in, compute, force_gather, tile_n, cta_group)
         self.device = D.device.index if D.device.index is not None else torch.cuda.current_device()
+        self._scratch = None
         with torch.cuda.device(self.device):
             self.handle = handle(self.device)
             if workspace is None:
@@ -110,7 +111,7 @@ class BoundContraction:
                 if st != L.GK_OK:
                     _raise(st)
                 if plan.workspace_bytes:
-                    workspace = torch.empty(plan.workspace_bytes // 8 + 1, dtype=torch.int64, device=D.device)
+                    self._scratch = BoundScratch(D.device, plan.workspace_bytes)
         self.ws = (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if workspace is not None else (None, 0)
         self.ptrs = (A.data_ptr(), B.data_ptr(), C_in.data_ptr() if C_in is not None else None, D.data_ptr())
         self._keep = (A, B, C_in, D, workspace)
@@ -118,7 +119,11 @@ class BoundContraction:
 
     def __call__(self, stream=None):
         s = stream if stream is not None else self._torch.cuda.current_stream(self.device).cuda_stream
-        st = L.lib.gk_contract(self.handle, C.byref(self.desc), *self.ptrs, *self.ws, C.c_void_p(s))
+        ws = self.ws
+        if self._scratch is not None:
+            buffer = self._scratch.on(s)
+            ws = (buffer.data_ptr(), buffer.numel())
+        st = L.lib.gk_contract(self.handle, C.byref(self.desc), *self.ptrs, *ws, C.c_void_p(s))
         if st != L.GK_OK:
             _raise(st)
 

@@ -17,7 +17,7 @@ from . import epilogue as Epilogue
 from . import kernel as Kernel
 from . import transform as Transform
 from .config import Config, ConfigError, DimensionMismatch
-from .matmul import GemmKernelsError, _fold_transforms, _raise, _workspace_bytes, handle, lent_workspace, lower
+from .matmul import BoundScratch, GemmKernelsError, _fold_transforms, _raise, _workspace_bytes, handle, lent_workspace, lower
 
 _ACT = {Transform.Identity: L.GK_ACT_NONE, Transform.ReLU: L.GK_ACT_RELU, Transform.GELU: L.GK_ACT_GELU,
         Transform.SiLU: L.GK_ACT_SILU}
@@ -148,18 +148,16 @@ def _run(call, stream, workspace=None):
 
 class BoundFused:
     """A layer-level operator with its arguments lowered once: calling the object enqueues it again on the same
-    arrays for the cost of one FFI call.  It keeps the arrays alive and owns its workspace, so calls of one
-    object must not overlap on the GPU."""
+    arrays for the cost of one FFI call.  It keeps the arrays alive and has a workspace on every stream it is
+    called on (unless one was given); calls of one object write the same results and must not overlap on the GPU."""
 
     def __init__(self, call, workspace=None):
         import torch
         self._call, self._torch, self.device = call, torch, call.device.index
         with torch.cuda.device(self.device):
             self.handle = handle(self.device)
-            if workspace is None:
-                need = call.workspace_bytes(self.handle)
-                if need:
-                    workspace = torch.empty(need, dtype=torch.uint8, device=call.device)
+            need = call.workspace_bytes(self.handle) if workspace is None else 0
+            self._scratch = BoundScratch(call.device, need) if need else None
         self._keep = workspace
         # converted once: ctypes would do it again for every argument of every call (8.8 -> 7 us of host time)
         self._arguments = call.arguments(self.handle, C.c_void_p(workspace.data_ptr() if workspace is not None else None),
@@ -170,11 +168,15 @@ class BoundFused:
         """Enqueues on `stream` (a raw CUDA stream handle) or on torch's current stream of the arrays' device."""
         cuda = self._torch.cuda
         s = stream if stream is not None else cuda.current_stream(self.device).cuda_stream
+        arguments = self._arguments
+        if self._scratch is not None:
+            buffer = self._scratch.on(s)
+            arguments = (*arguments[:-2], C.c_void_p(buffer.data_ptr()), C.c_int64(buffer.numel()))
         if cuda.current_device() == self.device:
-            st = self._function(*self._arguments, s)
+            st = self._function(*arguments, s)
         else:
             with cuda.device(self.device):
-                st = self._function(*self._arguments, s)
+                st = self._function(*arguments, s)
         if st != L.GK_OK:
             _raise(st)
 

@@ -288,6 +288,14 @@ def _check_user_workspace(h, desc, epi, workspace):
         raise GemmKernelsError("workspace must be 256-byte aligned")
 
 
+def _on_stream(device, stream: int):
+    """Makes `stream` (a raw handle) torch's current one, and its device the current device, so that the caching allocator ties new blocks to it."""
+    import torch
+    if device.index == torch.cuda.current_device() and stream == torch.cuda.current_stream(device).cuda_stream:
+        return contextlib.nullcontext()
+    return torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device) if stream else torch.cuda.default_stream(device))
+
+
 @contextlib.contextmanager
 def lent_workspace(device, stream: int, nbytes: int):
     """The lent scratch buffer of (device, stream), at least `nbytes` long (None for 0 bytes), for the calls
@@ -299,9 +307,7 @@ def lent_workspace(device, stream: int, nbytes: int):
         yield None
         return
     stream = int(stream)
-    # allocate under the caller's stream so the caching allocator ties the block to it
-    with contextlib.nullcontext() if stream == torch.cuda.current_stream(device).cuda_stream else torch.cuda.stream(
-            torch.cuda.ExternalStream(stream, device=device) if stream else torch.cuda.default_stream(device)):
+    with _on_stream(device, stream):
         if torch.cuda.is_current_stream_capturing():
             yield torch.empty(nbytes, dtype=torch.uint8, device=device)
             return
@@ -313,6 +319,28 @@ def lent_workspace(device, stream: int, nbytes: int):
                 ws = torch.empty(max(nbytes, 2 * (ws.numel() if ws is not None else 0)), dtype=torch.uint8, device=device)
                 scratch.buffer = ws
             yield ws
+
+
+class BoundScratch:
+    """The scratch of a bound call: a buffer for every stream the call is made on, allocated under that stream on first
+    need - so that no other stream's work can still be using its memory, nor get it while this stream's may (a buffer
+    dropped with the object goes back to the stream that used it).  Calls that torch captures into a graph take a buffer of
+    the graph's own, which lives as long as the graph."""
+
+    def __init__(self, device, nbytes: int):
+        import torch
+        self._torch, self._device, self.nbytes, self._buffers = torch, device, nbytes, {}
+        self.on(torch.cuda.current_stream(device).cuda_stream)
+
+    def on(self, stream: int):
+        torch = self._torch
+        with _on_stream(self._device, stream):
+            if torch.cuda.is_current_stream_capturing():
+                return torch.empty(self.nbytes, dtype=torch.uint8, device=self._device)
+            ws = self._buffers.get(stream)
+            if ws is None:
+                ws = self._buffers[stream] = torch.empty(self.nbytes, dtype=torch.uint8, device=self._device)
+            return ws
 
 
 def _auto_workspace_bytes(h, desc, epi) -> int:
@@ -409,21 +437,17 @@ class BoundMatmul:
     def __init__(self, conf, a, b, c, d, hooks, epilogue, kernel, workspace):
         import torch
         self._keep = (a, b, c, d, epilogue, workspace)
+        self._scratch = None
         self.desc, self.epi, self.ptrs = lower(conf, a, b, c, d, hooks, epilogue, kernel)
         self.device = d.device.index if d.device.index is not None else torch.cuda.current_device()
         with torch.cuda.device(self.device):
             self.handle = handle(self.device)
             if workspace is not None:
                 _check_user_workspace(self.handle, self.desc, self.epi, workspace)
-            elif _wants_workspace(self.desc):
-                # a bound product owns its scratch: it may be replayed on any stream
-                plan = L.GemmPlan()
-                st = L.lib.gk_gemm_query(self.handle, C.byref(self.desc), C.byref(self.epi), C.byref(plan))
-                if st != L.GK_OK:
-                    _raise(st)
-                if plan.workspace_bytes:
-                    workspace = torch.empty(plan.workspace_bytes, dtype=torch.uint8, device=d.device)
-                    self._keep += (workspace,)
+            else:
+                need = _auto_workspace_bytes(self.handle, self.desc, self.epi)
+                if need:
+                    self._scratch = BoundScratch(d.device, need)      # a bound product may be replayed on any stream
         self.ws = workspace.data_ptr() if workspace is not None else None
         self.ws_bytes = _workspace_bytes(workspace)
         self._torch = torch
@@ -433,8 +457,11 @@ class BoundMatmul:
         device that holds D; that device must be current."""
         s = stream if stream is not None else self._torch.cuda.current_stream(self.device).cuda_stream
         pa, pb, pc, pd = self.ptrs
-        st = L.lib.gk_gemm(self.handle, C.byref(self.desc), pa, pb, pc, pd, C.byref(self.epi), self.ws, self.ws_bytes,
-                           C.c_void_p(s))
+        ws, ws_bytes = self.ws, self.ws_bytes
+        if self._scratch is not None:
+            buffer = self._scratch.on(s)
+            ws, ws_bytes = buffer.data_ptr(), buffer.numel()
+        st = L.lib.gk_gemm(self.handle, C.byref(self.desc), pa, pb, pc, pd, C.byref(self.epi), ws, ws_bytes, C.c_void_p(s))
         if st != L.GK_OK:
             _raise(st)
 

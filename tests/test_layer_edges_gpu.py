@@ -181,3 +181,30 @@ def test_operands_off_16_bytes_are_given_room_for_their_copies(kind, which):
         GK.matmul_grouped_outer(cf, aw, bw, None, d, offsets)
         done()
         assert torch.equal(d.double(), torch.stack([a[:, i:j].double() @ b[:, i:j].double().T for i, j in ((0, 100), (100, 264))], 2))
+
+
+def test_bound_operators_on_another_stream_than_they_were_made_on():
+    """Called on a busy stream and dropped at once, while the stream they were made on allocates and writes memory."""
+    g = gen(313)
+    m, n, counts = 128, 256, [100, 0, 65, 3]
+    offsets, o = offsets_of(counts)
+    a, b = ints(g, m, o[-1]), ints(g, n, o[-1])
+    x, y = ints(g, 256, 8192, lo=-1, hi=1), ints(g, 8192, 64, lo=-1, hi=1)
+    want = torch.stack([a[:, o[i]:o[i + 1]].double() @ b[:, o[i]:o[i + 1]].double().T for i in range(4)], 2)
+    prod = x.double() @ y.double()
+    d, p, q = cm(torch.empty(m, n, 4, device="cuda")), cm(torch.empty(256, 64, device="cuda")), cm(torch.empty(256, 64, device="cuda"))
+    cf, cs = conf(m, n, o[-1], torch.float16, torch.float32, False, True), conf(256, 64, 8192, torch.float16, torch.float32)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        calls = [GK.bind_grouped_outer(cf, a, b, None, d, offsets), GK.bind(cs, x, y, None, p),
+                 GK.bind(cs, x, y, None, q, epilogue=Epilogue.BiasActivationResidual())]
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(200000)
+            for call in calls:
+                call()
+        del calls, call
+        for size in (1024, 1 << 16, 1 << 18, 1 << 20):
+            torch.empty(size, dtype=torch.uint8, device="cuda").fill_(255)
+    done()
+    assert torch.equal(d.double(), want) and torch.equal(p.double(), prod) and torch.equal(q.double(), prod)

@@ -187,3 +187,51 @@ def test_room_for_the_copies_of_operands_off_16_bytes(off_a, off_b, bound, no_gp
     want = 512 * (off_a != 0) + 1024 * (off_b != 0)
     assert got == [want] and (not want or asked == [(off_a != 0, off_b != 0)])
     assert (desc.lda, desc.ldb) == (64, 64)
+
+
+@pytest.mark.parametrize("which", ["layer", "product", "contraction"])
+def test_bound_calls_use_scratch_of_the_stream_they_are_on(which, no_gpu, monkeypatch):
+    """A buffer allocated under one stream and used on another may still be in use there, and goes back to the first
+    when the object is dropped: each buffer must be allocated under the stream that it is used on, once."""
+    on, made, used, capturing = [0], [], [], [False]
+
+    @contextlib.contextmanager
+    def stream(s):
+        before, on[0] = on[0], s.cuda_stream
+        yield
+        on[0] = before
+
+    real_empty = torch.empty
+
+    def empty(*size, **kw):
+        t = real_empty(*size, **kw)
+        if kw.get("dtype") in (torch.uint8, torch.int64):
+            made.append((t.data_ptr(), on[0], t))
+        return t
+
+    monkeypatch.setattr(torch.cuda, "stream", stream)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    monkeypatch.setattr(torch, "empty", empty)
+    address = lambda ws: ws if isinstance(ws, int) else ws.value
+    rec = lambda ws: used.append(address(ws)) or L.GK_OK
+    entry_point(which, rec, monkeypatch)
+    if which == "layer":
+        call = FakeCall(rec)
+        call.arguments = lambda h, ws, n: (ws, n)
+        bound = fused_mod.BoundFused(call)
+    elif which == "product":
+        cf = GK.get_config(gemm_shape=(64, 64, 4096), operator=Operator.TCGen05Operator[F16, F32], global_a_layout=Layout.ColMajor[F16],
+                           global_b_layout=Layout.ColMajor[F16], global_c_layout=Layout.Zero[F32], global_d_layout=Layout.ColMajor[F32])
+        bound = GK.bind(cf, cm(64, 4096), cm(4096, 64), None, cm(64, 64, dtype=torch.float32))
+    else:
+        bound = GK.bind_contract(cm(8, 8, dtype=torch.float32), "ab", cm(8, 8), "ac", cm(8, 8), "cb")
+    for s in (0, 5, 6, 5, 0):
+        bound(s)
+    owner = {p: s for p, s, _ in made}
+    assert [owner[p] for p in used] == [0, 5, 6, 5, 0] and len(made) == 3
+    capturing[0] = True
+    bound(5)
+    capturing[0] = False
+    assert used[-1] == made[-1][0] and len(made) == 4      # a graph's own
+    bound(5)
+    assert used[-1] == used[1] and len(made) == 4
