@@ -97,6 +97,12 @@ class _Call:
             _raise(st)
         return plan
 
+    def plan(self) -> L.GemmPlan:
+        """`query` for the arrays' device, made current: planning sets attributes of its kernels."""
+        import torch
+        with torch.cuda.device(self.device):
+            return self.query(handle(self.device.index))
+
     def workspace_bytes(self, h) -> int:
         d, gr = self.desc, self.groups
         ragged = gr.ragged if gr is not None else 0
@@ -325,7 +331,7 @@ def grouped_query(conf: Config, a, b, c, d, offsets, *, epilogue=None, kernel=Ke
     """What `matmul_grouped` (a 3-D `a`) or `matmul_grouped_outer` (a 3-D `d`) would launch; launches nothing."""
     call = lower_grouped_outer(conf, a, b, c, d, offsets, _hooks(transforms), kernel) if d.dim() == 3 else \
         lower_grouped(conf, a, b, c, d, offsets, _hooks(transforms), epilogue or Epilogue.Default(), kernel)
-    return call.query(handle(call.device.index))
+    return call.plan()
 
 
 # ------------------------------------------------------------------------------------------------

@@ -289,7 +289,8 @@ def _check_user_workspace(h, desc, epi, workspace):
 
 
 def _on_stream(device, stream: int):
-    """Makes `stream` (a raw handle) torch's current one, and its device the current device, so that the caching allocator ties new blocks to it."""
+    """Makes `stream` (a raw handle) torch's current one, and its device the current device, so that the caching
+    allocator ties new blocks to it."""
     import torch
     if device.index == torch.cuda.current_device() and stream == torch.cuda.current_stream(device).cuda_stream:
         return contextlib.nullcontext()
@@ -505,8 +506,7 @@ def query(conf: Config, a, b, c, d, *, epilogue=None, kernel=Kernel.matmul_singl
     hooks = {k.replace("transform_", ""): v for k, v in hooks.items()}
     if isinstance(epilogue, Epilogue.Fused):
         from .fused import lower_fused
-        call = lower_fused(conf, a, b, c, d, hooks, epilogue, kernel)
-        return call.query(handle(call.device.index))
+        return lower_fused(conf, a, b, c, d, hooks, epilogue, kernel).plan()
     desc, epi, _ = lower(conf, a, b, c, d, hooks, epilogue or Epilogue.Default(), kernel)
     plan = L.GemmPlan()
     st = L.lib.gk_gemm_query(handle(), C.byref(desc), C.byref(epi), C.byref(plan))

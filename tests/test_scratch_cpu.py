@@ -235,3 +235,24 @@ def test_bound_calls_use_scratch_of_the_stream_they_are_on(which, no_gpu, monkey
     assert used[-1] == made[-1][0] and len(made) == 4      # a graph's own
     bound(5)
     assert used[-1] == used[1] and len(made) == 4
+
+
+def test_plans_are_made_on_the_device_of_the_arrays(no_gpu, monkeypatch):
+    """Planning raises the shared-memory limits of the kernels it chooses, on the device that is current, and remembers that
+    it did in the handle of the arrays' device: on another one the later launch would fail."""
+    current, planned = [0], []
+
+    @contextlib.contextmanager
+    def device(d):
+        before, current[0] = current[0], getattr(d, "index", d)
+        yield
+        current[0] = before
+
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(L.lib, "gk_gemm_fused_query", lambda *a: planned.append(current[0]) or L.GK_OK)
+    monkeypatch.setattr(fused_mod, "_one_device", lambda *a: torch.device("cuda", 1))
+    cf = GK.get_config(gemm_shape=(64, 40, 32), operator=Operator.TCGen05Operator[F16, F32], global_a_layout=Layout.ColMajor[F16],
+                       global_b_layout=Layout.ColMajor[F16], global_c_layout=Layout.Zero[F32], global_d_layout=Layout.ColMajor[F32])
+    GK.query(cf, cm(64, 32), cm(32, 40), None, cm(64, 40, dtype=torch.float32), epilogue=GK.Epilogue.BiasActivationResidual())
+    GK.grouped_query(cf, cm(64, 32, 2), cm(32, 40), None, cm(64, 40, dtype=torch.float32), torch.zeros(3, dtype=torch.int32))
+    assert planned == [1, 1] and current[0] == 0
