@@ -208,3 +208,73 @@ def test_bound_operators_on_another_stream_than_they_were_made_on():
             torch.empty(size, dtype=torch.uint8, device="cuda").fill_(255)
     done()
     assert torch.equal(d.double(), want) and torch.equal(p.double(), prod) and torch.equal(q.double(), prod)
+
+
+# ------------------------------------------------------------------------------------------------
+# activations over their whole range
+# ------------------------------------------------------------------------------------------------
+ROUTES = {"words": (128, 96, 128), "elements": (130, 96, 128), "streamed": (128, 1, 128), "several": (128, 8, 128), "split": (128, 96, 16384)}
+
+
+def through_a_product(x, route, dt, out, act, z=None):
+    """act(x) - or with z x * act'(z) - as the fused epilogue computes it on one of its routes: x, exact in `dt`, behind a product
+    with the identity.  x and z have n columns of m values."""
+    m, n, k = ROUTES[route]
+    a = cm(torch.zeros(m, k, device="cuda", dtype=dt))
+    a[:, :min(m, k)] = torch.eye(m, min(m, k), device="cuda", dtype=dt)
+    b = cm(torch.zeros(k, n, device="cuda", dtype=dt))
+    b[: min(m, k)] = x[: min(m, k)].to(dt)
+    d = cm(torch.full((m, n), -9.0, device="cuda", dtype=out))
+    epi = Epilogue.ActivationGradient(z, ACT[act]) if z is not None else Epilogue.BiasActivationResidual(activation=ACT[act])
+    cf = conf(m, n, k, dt, out)
+    plan = GK.query(cf, a, b, None, d, epilogue=epi)
+    assert (plan.kernel == 6) == (route in ("streamed", "several")) and (plan.workspace_bytes > 0) == (route == "split")
+    GK.matmul(cf, a, b, None, d, epilogue=epi)
+    done()
+    return d
+
+
+def span(route, dt, lo=-12.0, hi=12.0):
+    m, n, k = ROUTES[route]
+    x = torch.linspace(lo, hi, m * n, device="cuda", dtype=torch.float64).reshape(n, m).T.to(dt)
+    x[min(m, k):] = 0                       # (rows that the identity does not reach)
+    return x
+
+
+def gelu64(x):
+    return 0.5 * x * torch.special.erfc(-x / math.sqrt(2))
+
+
+def within(got, want, rel, slack):
+    """One rounding to the type of `got`, behind a relative error `rel` and an absolute error `slack` before it."""
+    fi = torch.finfo(got.dtype)
+    tol = want.abs() * (fi.eps / 2 + rel * (1 + fi.eps)) + slack + fi.smallest_normal * fi.eps
+    off = (got.double() - want).abs() / tol
+    assert (off <= 1).all(), f"{int((~(off <= 1)).sum())} off, worst {float(off.max()):.2f} times the tolerance"
+
+
+# The tail's polynomial is off by 8.0e-7, the FP32 arithmetic around it rounds about 16 times (2^-24 each; two units of the last
+# place for the hardware's exponential and one for its reciprocal among them), and the exponent a^2 / 2 by three roundings of
+# 2^-24: a relative error of 8.0e-7 + (16 + 1.5 a^2) 2^-24 in Phi(-a); 1 - Phi(-a) and the sums with it round once more.
+def tail_error(x):
+    return 8.0e-7 + (16 + 1.5 * x * x) * 2.0 ** -24
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+def test_gelu_keeps_its_relative_accuracy_in_16_bits(dt):
+    x = span("words", dt)
+    want = gelu64(x.double())
+    got = through_a_product(x, "words", dt, dt, "gelu")
+    within(got, want, tail_error(x.double()), 0.0)
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+def test_gelu_gradient_keeps_its_accuracy_in_16_bits(dt):
+    z = cm(span("words", dt))
+    zd = z.double()
+    phi = zd.abs() * torch.exp(-zd * zd / 2) / math.sqrt(2 * math.pi)
+    tail = 0.5 * torch.special.erfc(zd.abs() / math.sqrt(2))
+    want = 0.5 * torch.special.erfc(-zd / math.sqrt(2)) + zd * torch.exp(-zd * zd / 2) / math.sqrt(2 * math.pi)
+    got = through_a_product(torch.ones_like(z), "words", dt, dt, "gelu", z)
+    slack = (tail + phi) * tail_error(zd) + 2.0 ** -23 * torch.maximum(phi, 0.5 * torch.special.erfc(-zd / math.sqrt(2)))
+    within(got, want, 0.0, slack * (1 + torch.finfo(dt).eps))
