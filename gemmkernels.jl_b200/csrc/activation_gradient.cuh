@@ -101,23 +101,21 @@ __global__ void __launch_bounds__(kActGradThreads, 3) activation_gradient_kernel
         if (col < n) {
           T* de = reinterpret_cast<T*>(&dv[u]);
           const T* ze = reinterpret_cast<const T*>(&zv[u]);
-          if constexpr (sizeof(T) == 2 && VEC > 1) {            // two elements at a time (fused_epilogue.cuh)
+          if constexpr (VEC > 1) {                              // two elements at a time (fused_epilogue.cuh)
 #pragma unroll
             for (int i = 0; i < VEC; i += 2) {
               float2 v = make_float2(actgrad_float(de[i]), actgrad_float(de[i + 1]));
               if (ACT != FUSED_ACT_NONE)
-                v = __fmul2_rn(v, fused_act_gradient2<ACT>(make_float2(actgrad_float(ze[i]), actgrad_float(ze[i + 1]))));
+                v = __fmul2_rn(v, fused_act_gradient2<ACT, sizeof(T) == 4>(make_float2(actgrad_float(ze[i]), actgrad_float(ze[i + 1]))));
               acc[i] += v.x; acc[i + 1] += v.y;
               de[i] = actgrad_round<T>(v.x); de[i + 1] = actgrad_round<T>(v.y);
             }
           } else {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-              float v = actgrad_float(de[i]);
-              if (ACT != FUSED_ACT_NONE) v = __fmul_rn(v, fused_act_gradient(actgrad_float(ze[i]), ACT));
-              acc[i] = __fadd_rn(acc[i], v);    // never contracted: the same sums whether dZ is stored or not
-              de[i] = actgrad_round<T>(v);
-            }
+            float v = actgrad_float(de[0]);
+            if (ACT == FUSED_ACT_GELU) v = __fmul_rn(v, fused_gelu_gradient2<sizeof(T) == 4>(fused_2(actgrad_float(ze[0]))).x);
+            else if (ACT != FUSED_ACT_NONE) v = __fmul_rn(v, fused_act_gradient(actgrad_float(ze[0]), ACT));
+            acc[0] = __fadd_rn(acc[0], v);      // never contracted: the same sums whether dZ is stored or not
+            de[0] = actgrad_round<T>(v);
           }
           if (p.dZ != nullptr) *reinterpret_cast<V*>(dz + col * p.lddz) = dv[u];
         }

@@ -32,7 +32,7 @@ struct FusedParams {
   int64_t bias_group;      // elements between the biases of consecutive groups
 };
 
-// Activations for results of 32 bits, one element.  A NaN passes through all of them.
+// A NaN passes through all activations.
 __device__ __forceinline__ float fused_max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -43,32 +43,6 @@ __device__ __forceinline__ float fused_min_nan(float a, float b) {
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-
-__device__ __forceinline__ float fused_act(float x, int32_t act) {
-  if (act == FUSED_ACT_RELU) return fused_max_nan(x, 0.0f);
-  if (act == FUSED_ACT_GELU) return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f));
-  if (act == FUSED_ACT_SILU) return x / (1.0f + expf(-x));
-  return x;
-}
-
-// act'(z), with ReLU'(0) = 0.  Where z multiplies something that has run out to zero it is clamped first, so
-// that an infinite z (a 16-bit pre-activation that overflowed) gives the limit, 0 or 1, instead of inf * 0.
-__device__ __forceinline__ float fused_act_gradient(float z, int32_t act) {
-  if (act == FUSED_ACT_RELU) return z > 0.0f ? 1.0f : (z <= 0.0f ? 0.0f : z);
-  if (act == FUSED_ACT_GELU) {   // Phi(z) + z phi(z)
-    const float c = fminf(fmaxf(z, -16.0f), 16.0f);
-    return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + c * (0.3989422804014327f * expf(-0.5f * c * c));
-  }
-  if (act == FUSED_ACT_SILU) {
-    const float c = fminf(fmaxf(z, -80.0f), 80.0f);
-    const float s = 1.0f / (1.0f + expf(-z));
-    return s * (1.0f + c * (1.0f - s));
-  }
-  return 1.0f;
-}
-
-// The same for results of 16 bits, whose half step (2^-12 relative at best) is far above the 2^-21 of the hardware
-// exponential and reciprocal: two elements at a time, so that the packed FP32 instructions do the arithmetic.
 __device__ __forceinline__ float fused_exp2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -82,14 +56,37 @@ __device__ __forceinline__ float fused_rcp(float x) {
 __device__ __forceinline__ float2 fused_2(float x) { return make_float2(x, x); }
 
 // The normal distribution's tail, Phi(-a) = e * R(a) with e = exp(-a^2 / 2), for a = min(|x|, 16) (beyond it both are zero
-// in FP32); returns S * R(a).  R is a polynomial of degree 7 without constant term in t = 1 / (1 + 0.363 a) - the form of
-// Hastings' approximations of the error function, but fitted here (least squares with Lawson's weights, over
-// 0 <= a <= 14.5) for the relative error: 8.0e-7, and in FP32, where a^2 / 2 is rounded before the exponential, 1.7e-6 up
-// to a = 5 and 6.9e-6 up to 13 - far below half a step of 16 bits (2.4e-4).  GELU' needs the exponential as well.
-template <int S>
+// in FP32); returns S * R(a).  (1 + erf(x / sqrt(2)) instead would cancel for x below -1.)  R is a polynomial without constant
+// term in t = 1 / (1 + c a) - the form of Hastings' approximations of the error function, but fitted here (least squares
+// with Lawson's weights, over 0 <= a <= 14.5) for the relative error.  Two elements at a time, for the packed FP32
+// instructions; GELU' needs the exponential as well.
+//   results of 16 bits   degree 7, 8.0e-7; in FP32, where a^2 / 2 is rounded before the exponential, 1.7e-6 up to a = 5 and
+//                        6.9e-6 up to 13 - far below half a step of 16 bits (2.4e-4)
+//   WIDE, of 32 bits     degree 9, 1.4e-8; the exponent's roundings are carried along, so that the FP32 arithmetic leaves
+//                        4.2e-7 everywhere (4096 x 2048 x 2048 with GELU: 46.5 us with erff, 54.4 with erfcf)
+template <bool WIDE, int S>
 __device__ __forceinline__ float2 fused_tail(float2 a, float2& e) {
-  const float2 s = __fmul2_rn(__fmul2_rn(a, a), fused_2(-0.72134752044448170f));        // log2(e) / 2
+  const float kLog = -0.72134752044448170f;                // -log2(e) / 2
+  const float2 a2 = __fmul2_rn(a, a), s = __fmul2_rn(a2, fused_2(kLog));
   e = make_float2(fused_exp2(s.x), fused_exp2(s.y));
+  if constexpr (WIDE) {
+    const float2 lo = __ffma2_rn(a, a, make_float2(-a2.x, -a2.y));      // what a^2 and the product with kLog, and kLog itself, lost
+    float2 d = __ffma2_rn(a2, fused_2(kLog), make_float2(-s.x, -s.y));
+    d = __ffma2_rn(lo, fused_2(kLog), d);
+    d = __ffma2_rn(a2, fused_2(static_cast<float>(-0.72134752044448170368 - static_cast<double>(kLog))), d);
+    e = __ffma2_rn(__fmul2_rn(e, fused_2(0.69314718055994531f)), d, e);
+    const float2 q = __ffma2_rn(a, fused_2(0.265f), fused_2(1.0f));
+    const float2 t = make_float2(fused_rcp(q.x), fused_rcp(q.y));
+    float2 r = __ffma2_rn(t, fused_2(S * 0.03062436632f), fused_2(S * -0.14330013024f));
+    r = __ffma2_rn(r, t, fused_2(S * 0.21594934599f));
+    r = __ffma2_rn(r, t, fused_2(S * -0.11428526510f));
+    r = __ffma2_rn(r, t, fused_2(S * 0.13655412860f));
+    r = __ffma2_rn(r, t, fused_2(S * 0.06089536025f));
+    r = __ffma2_rn(r, t, fused_2(S * 0.10255500375f));
+    r = __ffma2_rn(r, t, fused_2(S * 0.10526679036f));
+    r = __ffma2_rn(r, t, fused_2(S * 0.10574039670f));
+    return __fmul2_rn(r, t);
+  }
   const float2 d = __ffma2_rn(a, fused_2(0.363f), fused_2(1.0f));
   const float2 t = make_float2(fused_rcp(d.x), fused_rcp(d.y));
   float2 r = __ffma2_rn(t, fused_2(S * 0.04808691645f), fused_2(S * -0.17913879823f));
@@ -101,36 +98,67 @@ __device__ __forceinline__ float2 fused_tail(float2 a, float2& e) {
   return __fmul2_rn(r, t);
 }
 
+template <bool WIDE>
+__device__ __forceinline__ float2 fused_gelu2(float2 x) {      // x Phi(x) = max(x, 0) - |x| Phi(-|x|)
+  float2 e;
+  const float2 a = make_float2(fused_min_nan(fabsf(x.x), 16.0f), fused_min_nan(fabsf(x.y), 16.0f));
+  const float2 r = __fmul2_rn(a, fused_tail<WIDE, -1>(a, e));
+  return __ffma2_rn(r, e, make_float2(fmaxf(x.x, 0.0f), fmaxf(x.y, 0.0f)));
+}
+
+template <bool WIDE>
+__device__ __forceinline__ float2 fused_gelu_gradient2(float2 z) {
+  float2 e;
+  const float2 a = make_float2(fused_min_nan(fabsf(z.x), 16.0f), fused_min_nan(fabsf(z.y), 16.0f));
+  // w = Phi(-a) - a phi(a) is the derivative at -a, and 1 - w the one at a
+  const float2 w = __fmul2_rn(__ffma2_rn(a, fused_2(-0.3989422804014327f), fused_tail<WIDE, 1>(a, e)), e);
+  const float2 r = __ffma2_rn(w, fused_2(-1.0f), fused_2(1.0f));
+  return make_float2(z.x > 0.0f ? r.x : w.x, z.y > 0.0f ? r.y : w.y);
+}
+
+// Activations for results of 32 bits, one element.
+__device__ __forceinline__ float fused_act(float x, int32_t act) {
+  if (act == FUSED_ACT_RELU) return fused_max_nan(x, 0.0f);
+  if (act == FUSED_ACT_GELU) return fused_gelu2<true>(fused_2(x)).x;
+  if (act == FUSED_ACT_SILU) return x / (1.0f + expf(-x));
+  return x;
+}
+
+// act'(z), with ReLU'(0) = 0.  Where z multiplies something that has run out to zero it is clamped first, so
+// that an infinite z (a 16-bit pre-activation that overflowed) gives the limit, 0 or 1, instead of inf * 0.
+__device__ __forceinline__ float fused_act_gradient(float z, int32_t act) {
+  if (act == FUSED_ACT_RELU) return z > 0.0f ? 1.0f : (z <= 0.0f ? 0.0f : z);
+  if (act == FUSED_ACT_GELU) return fused_gelu_gradient2<true>(fused_2(z)).x;
+  if (act == FUSED_ACT_SILU) {
+    const float c = fminf(fmaxf(z, -80.0f), 80.0f);
+    const float s = 1.0f / (1.0f + expf(-z));
+    return s * (1.0f + c * (1.0f - s));
+  }
+  return 1.0f;
+}
+
+// Two elements at a time.  For results of 16 bits, whose half step (2^-12 relative at best) is far above the 2^-21 of the
+// hardware exponential and reciprocal, SiLU takes those too.
 __device__ __forceinline__ float2 fused_sigmoid2(float2 x) {
   const float2 s = __fmul2_rn(x, fused_2(-1.4426950408889634f));
   const float2 d = __fadd2_rn(make_float2(fused_exp2(s.x), fused_exp2(s.y)), fused_2(1.0f));
   return make_float2(fused_rcp(d.x), fused_rcp(d.y));
 }
 
-template <int ACT>
+template <int ACT, bool WIDE = false>
 __device__ __forceinline__ float2 fused_act2(float2 x) {
   if constexpr (ACT == FUSED_ACT_RELU) return make_float2(fused_max_nan(x.x, 0.0f), fused_max_nan(x.y, 0.0f));
-  if constexpr (ACT == FUSED_ACT_GELU) {      // x Phi(x) = max(x, 0) - |x| Phi(-|x|)
-    float2 e;
-    const float2 a = make_float2(fused_min_nan(fabsf(x.x), 16.0f), fused_min_nan(fabsf(x.y), 16.0f));
-    const float2 r = __fmul2_rn(a, fused_tail<-1>(a, e));
-    return __ffma2_rn(r, e, make_float2(fmaxf(x.x, 0.0f), fmaxf(x.y, 0.0f)));
-  }
+  if constexpr (ACT == FUSED_ACT_GELU) return fused_gelu2<WIDE>(x);
+  if constexpr (ACT == FUSED_ACT_SILU && WIDE) return make_float2(fused_act(x.x, ACT), fused_act(x.y, ACT));
   if constexpr (ACT == FUSED_ACT_SILU) return __fmul2_rn(x, fused_sigmoid2(x));
   return x;
 }
 
-template <int ACT>
+template <int ACT, bool WIDE = false>
 __device__ __forceinline__ float2 fused_act_gradient2(float2 z) {
-  if constexpr (ACT == FUSED_ACT_RELU) return make_float2(fused_act_gradient(z.x, FUSED_ACT_RELU), fused_act_gradient(z.y, FUSED_ACT_RELU));
-  if constexpr (ACT == FUSED_ACT_GELU) {
-    float2 e;
-    const float2 a = make_float2(fused_min_nan(fabsf(z.x), 16.0f), fused_min_nan(fabsf(z.y), 16.0f));
-    // w = Phi(-a) - a phi(a) is the derivative at -a, and 1 - w the one at a
-    const float2 w = __fmul2_rn(__ffma2_rn(a, fused_2(-0.3989422804014327f), fused_tail<1>(a, e)), e);
-    const float2 r = __ffma2_rn(w, fused_2(-1.0f), fused_2(1.0f));
-    return make_float2(z.x > 0.0f ? r.x : w.x, z.y > 0.0f ? r.y : w.y);
-  }
+  if constexpr (ACT == FUSED_ACT_RELU || (ACT == FUSED_ACT_SILU && WIDE))
+    return make_float2(fused_act_gradient(z.x, ACT), fused_act_gradient(z.y, ACT));
+  if constexpr (ACT == FUSED_ACT_GELU) return fused_gelu_gradient2<WIDE>(z);
   if constexpr (ACT == FUSED_ACT_SILU) {
     const float2 s = fused_sigmoid2(z);
     const float2 c = make_float2(fminf(fmaxf(z.x, -80.0f), 80.0f), fminf(fmaxf(z.y, -80.0f), 80.0f));

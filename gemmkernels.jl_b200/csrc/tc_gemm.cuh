@@ -370,7 +370,7 @@ __device__ __forceinline__ void tc_elements_chunk(const TcParams& p, const uint3
 #pragma unroll
   for (int h = 0; h < 32; h += W) {
     auto in = [&](int j) { return (live >> (h + j)) & 1u; };
-    T cv[W], zv[W];
+    T cv[W], zv[W] = {};
     if (has_c) {
 #pragma unroll
       for (int j = 0; j < W; ++j, advance(c, p.c_sn0))
@@ -397,7 +397,13 @@ __device__ __forceinline__ void tc_elements_chunk(const TcParams& p, const uint3
     if (gradient) {
 #define GK_EACH(expr) _Pragma("unroll") for (int j = 0; j < W; ++j) if (in(j)) { expr; }
       if (p.act == TC_ACT_RELU) { GK_EACH(x[j] *= fused_act_gradient(tc_get<T>(zv[j], f16), TC_ACT_RELU)) }
-      else if (p.act == TC_ACT_GELU) { GK_EACH(x[j] *= fused_act_gradient(tc_get<T>(zv[j], f16), TC_ACT_GELU)) }
+      else if (p.act == TC_ACT_GELU) {
+#pragma unroll
+        for (int j = 0; j < W; j += 2) {       // (columns that do not exist are not stored)
+          const float2 s = fused_gelu_gradient2<sizeof(T) == 4>(make_float2(tc_get<T>(zv[j], f16), tc_get<T>(zv[j + 1], f16)));
+          x[j] *= s.x; x[j + 1] *= s.y;
+        }
+      }
       else if (p.act == FUSED_ACT_SILU) { GK_EACH(x[j] *= fused_act_gradient(tc_get<T>(zv[j], f16), FUSED_ACT_SILU)) }
     } else {
       if (p.f.Z != nullptr) {
@@ -406,7 +412,13 @@ __device__ __forceinline__ void tc_elements_chunk(const TcParams& p, const uint3
           if (in(j)) *z = tc_put<T>(x[j], f16);
       }
       if (p.act == TC_ACT_RELU) { GK_EACH(x[j] = fused_act(x[j], TC_ACT_RELU)) }
-      else if (p.act == TC_ACT_GELU) { GK_EACH(x[j] = fused_act(x[j], TC_ACT_GELU)) }
+      else if (p.act == TC_ACT_GELU) {
+#pragma unroll
+        for (int j = 0; j < W; j += 2) {
+          const float2 y = fused_gelu2<sizeof(T) == 4>(make_float2(x[j], x[j + 1]));
+          x[j] = y.x; x[j + 1] = y.y;
+        }
+      }
       else if (p.act == FUSED_ACT_SILU) { GK_EACH(x[j] = fused_act(x[j], FUSED_ACT_SILU)) }
       if (has_c && residual) { GK_EACH(x[j] += p.beta * tc_get<T>(cv[j], f16)) }
     }

@@ -228,7 +228,7 @@ def through_a_product(x, route, dt, out, act, z=None):
     epi = Epilogue.ActivationGradient(z, ACT[act]) if z is not None else Epilogue.BiasActivationResidual(activation=ACT[act])
     cf = conf(m, n, k, dt, out)
     plan = GK.query(cf, a, b, None, d, epilogue=epi)
-    assert (plan.kernel == 6) == (route in ("streamed", "several")) and (plan.workspace_bytes > 0) == (route == "split")
+    assert (plan.kernel == 6) == (route in ("streamed", "several")) and (route != "split" or plan.workspace_bytes >= 2 * m * n * 4)
     GK.matmul(cf, a, b, None, d, epilogue=epi)
     done()
     return d
@@ -278,3 +278,47 @@ def test_gelu_gradient_keeps_its_accuracy_in_16_bits(dt):
     got = through_a_product(torch.ones_like(z), "words", dt, dt, "gelu", z)
     slack = (tail + phi) * tail_error(zd) + 2.0 ** -23 * torch.maximum(phi, 0.5 * torch.special.erfc(-zd / math.sqrt(2)))
     within(got, want, 0.0, slack * (1 + torch.finfo(dt).eps))
+
+
+# In 32 bits, what x / 2 * erfc(-x / sqrt(2)) costs when it is evaluated as it stands: the argument is off by two half steps
+# (2^-23), which its exponential exp(-x^2 / 2) multiplies by x^2; the function by 4 units of the last place (2^-21 at
+# most), the products around it by two half steps.  (The kernels carry the exponent's roundings along.)  The split sum,
+# alpha and the bias add zeros to x and leave it exact.
+def gelu32_error(x):
+    return (x * x + 4 + 2) * 2.0 ** -23
+
+
+@pytest.mark.parametrize("out", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("route", ["elements", "streamed", "several", "split"])
+def test_gelu_keeps_its_relative_accuracy_in_32_bits(route, out):
+    x = span(route, torch.float16)
+    got = through_a_product(x, route, torch.float16, out, "gelu")
+    within(got, gelu64(x.double()), gelu32_error(x.double()), 0.0)
+
+
+@pytest.mark.parametrize("out", [torch.float32, torch.float16])
+@pytest.mark.parametrize("route", ["elements", "streamed", "several", "split"])
+def test_gelu_gradient_keeps_its_accuracy_in_32_bits(route, out):
+    """Phi(z) and z phi(z), each to its own relative error (the exponential: its exponent rounded twice, two units of the last
+    place), and their sum's rounding."""
+    z = cm(span(route, out))
+    zd = z.double()
+    phi, tail = zd.abs() * torch.exp(-zd * zd / 2) / math.sqrt(2 * math.pi), 0.5 * torch.special.erfc(-zd / math.sqrt(2))
+    got = through_a_product(torch.ones_like(z), route, torch.float16, out, "gelu", z)
+    x = torch.zeros_like(zd)
+    x[: min(ROUTES[route][0], ROUTES[route][2])] = 1
+    slack = x * (tail * gelu32_error(zd) + phi * (zd * zd / 2 + 4 + 3) * 2.0 ** -23 + 2.0 ** -24 * (tail + phi))
+    within(got, x * (tail + zd * torch.exp(-zd * zd / 2) / math.sqrt(2 * math.pi)), 0.0, slack * (1 + torch.finfo(out).eps))
+
+
+@pytest.mark.parametrize("m,dt", [(128, torch.float32), (131, torch.float32), (131, torch.bfloat16)])
+def test_activation_gradient_of_gelu_keeps_its_accuracy(m, dt):
+    """The kernel of its own: in 32 bits, and element by element in 16."""
+    z = cm(torch.linspace(-12, 12, m * 200, device="cuda", dtype=torch.float64).reshape(200, m).T.to(dt))
+    zd = z.double()
+    phi, tail = zd.abs() * torch.exp(-zd * zd / 2) / math.sqrt(2 * math.pi), 0.5 * torch.special.erfc(-zd / math.sqrt(2))
+    dz = cm(torch.full((m, 200), -9.0, device="cuda", dtype=dt))
+    GK.activation_gradient_(dz, cm(torch.ones(m, 200, device="cuda", dtype=dt)), z, ACT["gelu"])
+    done()
+    slack = tail * gelu32_error(zd) + phi * (zd * zd / 2 + 4 + 3) * 2.0 ** -23 + 2.0 ** -24 * (tail + phi)
+    within(dz, tail + zd * torch.exp(-zd * zd / 2) / math.sqrt(2 * math.pi), 0.0, slack * (1 + torch.finfo(dt).eps))
