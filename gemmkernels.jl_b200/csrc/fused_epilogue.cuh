@@ -32,7 +32,8 @@ struct FusedParams {
   int64_t bias_group;      // elements between the biases of consecutive groups
 };
 
-// A NaN passes through all activations.
+// A NaN passes through all activations; at minus infinity GELU and SiLU have their limit 0 (the factor that multiplies what
+// has run out to zero is clamped), as their derivatives have 0 and 1.
 __device__ __forceinline__ float fused_max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -120,7 +121,7 @@ __device__ __forceinline__ float2 fused_gelu_gradient2(float2 z) {
 __device__ __forceinline__ float fused_act(float x, int32_t act) {
   if (act == FUSED_ACT_RELU) return fused_max_nan(x, 0.0f);
   if (act == FUSED_ACT_GELU) return fused_gelu2<true>(fused_2(x)).x;
-  if (act == FUSED_ACT_SILU) return x / (1.0f + expf(-x));
+  if (act == FUSED_ACT_SILU) return fused_max_nan(x, -128.0f) / (1.0f + expf(-x));
   return x;
 }
 
@@ -150,7 +151,8 @@ __device__ __forceinline__ float2 fused_act2(float2 x) {
   if constexpr (ACT == FUSED_ACT_RELU) return make_float2(fused_max_nan(x.x, 0.0f), fused_max_nan(x.y, 0.0f));
   if constexpr (ACT == FUSED_ACT_GELU) return fused_gelu2<WIDE>(x);
   if constexpr (ACT == FUSED_ACT_SILU && WIDE) return make_float2(fused_act(x.x, ACT), fused_act(x.y, ACT));
-  if constexpr (ACT == FUSED_ACT_SILU) return __fmul2_rn(x, fused_sigmoid2(x));
+  if constexpr (ACT == FUSED_ACT_SILU)
+    return __fmul2_rn(make_float2(fused_max_nan(x.x, -128.0f), fused_max_nan(x.y, -128.0f)), fused_sigmoid2(x));
   return x;
 }
 

@@ -322,3 +322,22 @@ def test_activation_gradient_of_gelu_keeps_its_accuracy(m, dt):
     done()
     slack = tail * gelu32_error(zd) + phi * (zd * zd / 2 + 4 + 3) * 2.0 ** -23 + 2.0 ** -24 * (tail + phi)
     within(dz, tail + zd * torch.exp(-zd * zd / 2) / math.sqrt(2 * math.pi), 0.0, slack * (1 + torch.finfo(dt).eps))
+
+
+@pytest.mark.parametrize("act", [None, "relu", "gelu", "silu"])
+@pytest.mark.parametrize("out", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("route", list(ROUTES))
+def test_activations_of_infinities_are_their_limits(route, out, act):
+    """On every route alike: 0 and infinity (x itself without an activation), and a NaN stays one."""
+    m, n, k = ROUTES[route]
+    a, b = cm(torch.zeros(m, k, device="cuda", dtype=torch.float16)), cm(torch.zeros(k, n, device="cuda", dtype=torch.float16))
+    bias = torch.zeros(m, device="cuda")
+    bias[0], bias[3], bias[m - 1], bias[64] = -math.inf, math.inf, math.nan, -200.0
+    d = cm(torch.full((m, n), -9.0, device="cuda", dtype=out))
+    GK.matmul(conf(m, n, k, torch.float16, out), a, b, None, d, epilogue=Epilogue.BiasActivationResidual(bias, activation=ACT[act]))
+    done()
+    want = torch.zeros(m, n, device="cuda", dtype=torch.float64)
+    want[3], want[m - 1] = math.inf, math.nan
+    if act is None:
+        want[0], want[64] = -math.inf, -200.0
+    assert torch.equal(d.double().nan_to_num(nan=-1.0), want.nan_to_num(nan=-1.0))
