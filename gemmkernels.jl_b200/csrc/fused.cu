@@ -167,6 +167,15 @@ static gk_status launch_copy(gk_handle h, const OperandCopy& c, const void* src,
 // ------------------------------------------------------------------------------------------------
 // a few columns: the streaming kernel
 // ------------------------------------------------------------------------------------------------
+// How the columns fall on the groups is known on the device only.  At this size the streaming kernel and the tensor cores are even
+// when all columns fall on one group, whose weights the tensor cores read once, and streaming is ahead when they are spread
+// (us, streaming / tensor cores; transposed A of 2048 x 2048, 64 groups: 8 columns spread 11.8 / 16.0, on one group 10.1 /
+// 12.0; 16 columns 22.5 / 25.9 and 15.2 / 11.8; 32 columns 37.3 / 38.0 and 25.9 / 12.0; 64 columns 62.8 / 57.3 and 45.3 / 12.0.
+// 256 groups of 1024 x 1024, 64 columns: 25.9 / 38.6 and 16.8 / 15.8.  8 groups of 4096 x 4096, 4 columns: 24.7 / 26.5
+// and 15.5 / 16.1.  Operands off 16 bytes, 64 groups of 2047 x 2049, 16 columns: 87 / 143 and 59 / 66, 32 columns: 170 / 165
+// and 110 / 68).
+constexpr int64_t kSkinnyGroupBytes = 1 << 27;
+
 struct SkinnyPlan { int nt = 0, ranks = 1, items = 0, rows = 0, k_per_rank = 0; bool any = false; };
 
 static bool skinny_plan(gk_handle h, const gk_gemm_desc& d, const gk_group_desc* gr, const void* a, const void* b, SkinnyPlan* out) {
@@ -180,13 +189,14 @@ static bool skinny_plan(gk_handle h, const gk_gemm_desc& d, const gk_group_desc*
   auto al = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
   p.any = !al(a) || !al(b) || d.lda % 8 || d.ldb % 8 || d.k % 8 || (!d.trans_a && d.m % 8) || d.trans_b ||
           (gr && groups > 1 && gr->stride_a % 8);
-  // Groups: while the average is one column (64 experts of 2048 x 2048: 16 tokens 25 us, 34 on the tensor cores; 64 tokens
-  // 76 and 72, 90 tokens 100 and 84: a group with more columns is streamed again).  One product: up to 16 columns of a
+  // Groups: one column at a time, while there are no more of them than groups and what they stream, counting a group's weights
+  // once for each of its columns, stays below kSkinnyGroupBytes.  One product: up to 16 columns of a
   // transposed A (4096 x 4096, 8 columns: 11.0 us, 16.1 with tcgen05; 16: 13.0 and 16.2), else up to eight (12.4 and
   // 16.3-17.2), of these with FMAs up to four (2048 x 2048, 4 columns: 6.0 us, 7.1 with warp-level matrix instructions; 4096 x
   // 4096: 11.6 and 11.8) and up to four in all where 16-byte loads do not serve.
   const int mma = groups != 1 || p.any ? 0 : d.trans_a ? (d.n > 1 ? kSkinnyMmaCols : 0) : (d.n > 4 ? kSkinnyMmaRowsCols : 0);
   if (d.n > (groups > 1 ? active : mma ? mma : 4)) return false;
+  if (groups > 1 && d.n > 1 && 2 * d.m * d.k > kSkinnyGroupBytes / d.n) return false;
   p.nt = d.n <= active ? 1 : mma ? mma : (d.n <= 2 ? 2 : 4);
   p.items = static_cast<int>(std::min<int64_t>(d.n, d.n / p.nt + active));
   if (groups == 1) p.items = static_cast<int>((d.n + p.nt - 1) / p.nt);

@@ -341,3 +341,24 @@ def test_activations_of_infinities_are_their_limits(route, out, act):
     if act is None:
         want[0], want[64] = -math.inf, -200.0
     assert torch.equal(d.double().nan_to_num(nan=-1.0), want.nan_to_num(nan=-1.0))
+
+
+@pytest.mark.parametrize("m,k,groups,n,streams", [(2048, 2048, 64, 8, True), (2048, 2048, 64, 64, False), (256, 128, 64, 64, True),
+                                                   (4096, 4096, 8, 8, False), (8192, 16384, 2, 1, True), (8192, 16384, 2, 2, False)])
+def test_grouped_columns_stream_while_the_worst_routing_allows(m, k, groups, n, streams):
+    """All tokens may fall on one group, whose weights the streaming kernel would read once for each of them; the choice is made
+    without knowing, and either kernel is right for any routing."""
+    g = gen(314)
+    w = ints(g, k, m, lo=-1, hi=1)
+    a = w[:, :, None].expand(k, m, groups)                 # one matrix for all groups (row-major weights)
+    b = cm(torch.zeros(k, n, device="cuda", dtype=torch.float16))
+    b[: 64] = ints(g, 64, n)
+    want = w.double().T @ b.double()
+    cf = conf(m, n, k, torch.float16, torch.float32, True)
+    for counts in ([1] * n + [0] * (groups - n), [0] * (groups - 1) + [n]):
+        offsets, _ = offsets_of(counts)
+        d = cm(torch.full((m, n), -9.0, device="cuda"))
+        assert (GK.grouped_query(cf, a, b, None, d, offsets).kernel == 6) == streams
+        GK.matmul_grouped(cf, a, b, None, d, offsets)
+        done()
+        assert torch.equal(d.double(), want)
