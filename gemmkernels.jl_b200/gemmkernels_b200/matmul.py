@@ -262,7 +262,7 @@ def _wants_workspace(desc) -> bool:
 # each other's in between.  A buffer's lock is therefore held from lending until the call has enqueued.
 class _Scratch:
     def __init__(self):
-        self.lock, self.buffer = threading.Lock(), None
+        self.lock, self.buffer = threading.RLock(), None      # (re-entrant: an allocation may run finalisers)
 
 
 _workspaces: dict = {}
@@ -297,17 +297,17 @@ def _on_stream(device, stream: int):
     return torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device) if stream else torch.cuda.default_stream(device))
 
 
-@contextlib.contextmanager
 def lent_workspace(device, stream: int, nbytes: int):
     """The lent scratch buffer of (device, stream), at least `nbytes` long (None for 0 bytes), for the calls
     enqueued inside the `with` block; another thread's calls on that stream wait until the block is left.
     While torch captures the stream into a graph, a buffer of the graph's own instead: two graphs never share one,
     and none points into a buffer that a larger one replaces."""
+    return _lend(device, int(stream), nbytes) if nbytes else contextlib.nullcontext()
+
+
+@contextlib.contextmanager
+def _lend(device, stream: int, nbytes: int):
     import torch
-    if not nbytes:
-        yield None
-        return
-    stream = int(stream)
     with _on_stream(device, stream):
         if torch.cuda.is_current_stream_capturing():
             yield torch.empty(nbytes, dtype=torch.uint8, device=device)
