@@ -121,8 +121,8 @@ class BoundContraction:
         s = stream if stream is not None else self._torch.cuda.current_stream(self.device).cuda_stream
         ws = self.ws
         if self._scratch is not None:
-            buffer = self._scratch.on(s)
-            ws = (buffer.data_ptr(), buffer.numel())
+            address, buffer = self._scratch.on(s, stream is None)
+            ws = (address, self._scratch.nbytes)
         st = L.lib.gk_contract(self.handle, C.byref(self.desc), *self.ptrs, *ws, C.c_void_p(s))
         if st != L.GK_OK:
             _raise(st)

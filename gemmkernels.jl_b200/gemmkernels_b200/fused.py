@@ -159,7 +159,8 @@ class BoundFused:
 
     def __init__(self, call, workspace=None):
         import torch
-        self._call, self._torch, self.device = call, torch, call.device.index
+        self._call, self._torch = call, torch
+        self.device = call.device.index if call.device.index is not None else torch.cuda.current_device()
         with torch.cuda.device(self.device):
             self.handle = handle(self.device)
             need = call.workspace_bytes(self.handle) if workspace is None else 0
@@ -168,21 +169,21 @@ class BoundFused:
         # converted once: ctypes would do it again for every argument of every call (8.8 -> 7 us of host time)
         self._arguments = call.arguments(self.handle, C.c_void_p(workspace.data_ptr() if workspace is not None else None),
                                          C.c_int64(_workspace_bytes(workspace)))
+        self._without_scratch = self._arguments[:-2]
         self._function = call.function
 
     def __call__(self, stream=None):
         """Enqueues on `stream` (a raw CUDA stream handle) or on torch's current stream of the arrays' device."""
         cuda = self._torch.cuda
-        s = stream if stream is not None else cuda.current_stream(self.device).cuda_stream
-        arguments = self._arguments
-        if self._scratch is not None:
-            buffer = self._scratch.on(s)
-            arguments = (*arguments[:-2], C.c_void_p(buffer.data_ptr()), C.c_int64(buffer.numel()))
-        if cuda.current_device() == self.device:
-            st = self._function(*arguments, s)
-        else:
+        if cuda.current_device() != self.device:
             with cuda.device(self.device):
-                st = self._function(*arguments, s)
+                return self(stream)
+        s = stream if stream is not None else cuda.current_stream(self.device).cuda_stream
+        if self._scratch is None:
+            st = self._function(*self._arguments, s)
+        else:
+            address, buffer = self._scratch.on(s, stream is None)
+            st = self._function(*self._without_scratch, address, self._scratch.nbytes, s)
         if st != L.GK_OK:
             _raise(st)
 

@@ -179,7 +179,7 @@ def test_room_for_the_copies_of_operands_off_16_bytes(off_a, off_b, bound, no_gp
     monkeypatch.setattr(L.lib, "gk_gemm_fused_query", query)
     desc = L.GemmDesc(m=64, n=64, k=64, lda=64, ldb=64, ldd=64, alpha=1.0)
     call = fused_mod._Call(desc, L.FusedDesc(), None, (0x1000 + off_a, 0x2000 + off_b, None, 0x3000), torch.device("cpu"), ())
-    call.function = lambda h, desc, fu, gr, a, b, c, d, ws, n, s: got.append(n.value if bound else n) or L.GK_OK
+    call.function = lambda h, desc, fu, gr, a, b, c, d, ws, n, s: got.append(getattr(n, "value", n)) or L.GK_OK
     if bound:
         fused_mod.BoundFused(call)(5)
     else:
