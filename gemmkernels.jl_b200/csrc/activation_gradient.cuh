@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(kActGradThreads, 3) activation_gradient_kernel
     const T* dd = static_cast<const T*>(p.dD) + row + static_cast<int64_t>(c0) * p.ldd;
     const T* z = static_cast<const T*>(p.Z) + row + static_cast<int64_t>(c0) * p.ldz;
     T* dz = static_cast<T*>(p.dZ) + row + static_cast<int64_t>(c0) * p.lddz;
-    // The loads of the next U columns are in flight while these are computed (8192 x 16384, GELU: 163 us without).
+    // The loads of the next U columns are in flight while these are computed (8192 x 16384, GELU, on one machine: 163 us without, 148 with).
     constexpr int U = 2;
     V dv[U], zv[U], dn[U], zn[U];
     auto load = [&](int c, V (&d)[U], V (&w)[U]) {

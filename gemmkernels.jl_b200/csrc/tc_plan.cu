@@ -172,8 +172,9 @@ static const void* tc_kernel_select(int cg, int planes, bool tf32, bool rank5, b
 static constexpr int kSmemMax = 232448;  // 227 KiB opt-in limit per CTA on sm_100
 static constexpr int kCtrlBytes = kTcCtrlBytes;
 // FP32 sums over a long ragged run of K are made in parts of this many (TcParams::part_blocks).  4096 x 2048 x 16 experts,
-// 16384 tokens accumulated in FP32: 346 us and an error of 2.1e-6 at most; parts of 1024: 379 us and 1.0e-6; of 512: 480 us
-// and 4.8e-7; no parts: 350 us and 1.1e-9 per token of the longest run.
+// 16384 tokens accumulated in FP32: 346 us and an error of 2.1e-6 at most (2.5e-6 for Float16 operands); parts of 1024: 379 us and
+// 1.0e-6; of 512: 480 us and 4.8e-7; no parts: 350 us and 1.1e-9 per token of the longest run.  (On another machine, equal
+// parts of at most 2048, 1280 and 1024: 378, 400 and 417 us.)
 static constexpr int kPartK = 2048;
 static constexpr double kWideEff = 1.08;   // measured gain of the single-stage 512-column tiles on large products
 
