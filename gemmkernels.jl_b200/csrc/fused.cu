@@ -178,7 +178,8 @@ constexpr int64_t kSkinnyGroupBytes = 1 << 27;
 
 struct SkinnyPlan { int nt = 0, ranks = 1, items = 0, rows = 0, k_per_rank = 0; bool any = false; };
 
-static bool skinny_plan(gk_handle h, const gk_gemm_desc& d, const gk_group_desc* gr, const void* a, const void* b, SkinnyPlan* out) {
+static bool skinny_plan(gk_handle h, const gk_gemm_desc& d, const gk_group_desc* gr, const void* a, const void* b, int64_t group_bytes,
+                        SkinnyPlan* out) {
   if (gr && gr->ragged != GK_RAGGED_COLUMNS) return false;
   if (d.tile_n || d.cta_group || d.stages || d.max_ctas) return false;      // a tensor-core tile was asked for
   if (d.k < 1 || d.alpha == 0.0 || d.n < 1 || d.m < 1) return false;
@@ -190,13 +191,13 @@ static bool skinny_plan(gk_handle h, const gk_gemm_desc& d, const gk_group_desc*
   p.any = !al(a) || !al(b) || d.lda % 8 || d.ldb % 8 || d.k % 8 || (!d.trans_a && d.m % 8) || d.trans_b ||
           (gr && groups > 1 && gr->stride_a % 8);
   // Groups: one column at a time, while there are no more of them than groups and what they stream, counting a group's weights
-  // once for each of its columns, stays below kSkinnyGroupBytes.  One product: up to 16 columns of a
+  // once for each of its columns, stays below `group_bytes`.  One product: up to 16 columns of a
   // transposed A (4096 x 4096, 8 columns: 11.0 us, 16.1 with tcgen05; 16: 13.0 and 16.2), else up to eight (12.4 and
   // 16.3-17.2), of these with FMAs up to four (2048 x 2048, 4 columns: 6.0 us, 7.1 with warp-level matrix instructions; 4096 x
   // 4096: 11.6 and 11.8) and up to four in all where 16-byte loads do not serve.
   const int mma = groups != 1 || p.any ? 0 : d.trans_a ? (d.n > 1 ? kSkinnyMmaCols : 0) : (d.n > 4 ? kSkinnyMmaRowsCols : 0);
   if (d.n > (groups > 1 ? active : mma ? mma : 4)) return false;
-  if (groups > 1 && d.n > 1 && 2 * d.m * d.k > kSkinnyGroupBytes / d.n) return false;
+  if (groups > 1 && d.n > 1 && 2 * d.m * d.k > group_bytes / d.n) return false;
   p.nt = d.n <= active ? 1 : mma ? mma : (d.n <= 2 ? 2 : 4);
   p.items = static_cast<int>(std::min<int64_t>(d.n, d.n / p.nt + active));
   if (groups == 1) p.items = static_cast<int>((d.n + p.nt - 1) / p.nt);
@@ -325,7 +326,7 @@ gk_status gk_gemm_fused_query(gk_handle h, const gk_gemm_desc* desc, const gk_fu
   std::memset(plan, 0, sizeof(*plan));
   if (desc->m == 0 || desc->n == 0) return GK_OK;
   SkinnyPlan sp;
-  if (skinny_plan(h, *desc, groups, nullptr, nullptr, &sp)) {
+  if (skinny_plan(h, *desc, groups, nullptr, nullptr, kSkinnyGroupBytes, &sp)) {
     plan->kernel = 6; plan->grid = sp.rows * sp.ranks * sp.items; plan->block = kSkinnyThreads; plan->cluster = sp.ranks;
     plan->tile_m = kSkinnyRows; plan->tile_n = sp.nt; plan->tile_k = kSkinnyStep; plan->stages = 1;
   }
@@ -363,12 +364,15 @@ gk_status gk_gemm_fused(gk_handle h, const gk_gemm_desc* desc, const gk_fused_de
   TcProblem pr;
   fused_problem(*desc, *fused, groups, &epi, a, b, desc->beta != 0.0 ? c : nullptr, d, &pr);
   SkinnyPlan sp;
-  if (skinny_plan(h, *desc, groups, a, b, &sp)) return launch_skinny(sp, *desc, *fused, groups, pr, a, b, c, d, st);
+  if (skinny_plan(h, *desc, groups, a, b, kSkinnyGroupBytes, &sp)) return launch_skinny(sp, *desc, *fused, groups, pr, a, b, c, d, st);
   const FusedFeed feed = fused_feed(*desc, groups, a, b);
   const int64_t copies = feed.bytes();
   // A ragged depth multiplies copies through tensor maps, which need their room behind them: decided before anything is enqueued.
   const int64_t maps = pr.form == kTcRaggedDepth ? static_cast<int64_t>(groups->groups) * kTcDepthMapsBytes : 0;
   pr.generic = !feed.possible || (copies > 0 && (workspace_bytes < copies + maps || (reinterpret_cast<uintptr_t>(workspace) & 255)));
+  // Few columns of unaligned operands without room for their copies stream whatever their number per group (64 groups of
+  // 2047 x 2049, 32 columns spread: 170 us, bounds-checked loads 2056; on one group 110 and 301).
+  if (pr.generic && skinny_plan(h, *desc, groups, a, b, INT64_MAX, &sp)) return launch_skinny(sp, *desc, *fused, groups, pr, a, b, c, d, st);
   if (!pr.generic && copies > 0) {
     char* ws = static_cast<char*>(workspace);
     gk_gemm_desc e = *desc;

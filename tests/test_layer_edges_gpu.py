@@ -362,3 +362,23 @@ def test_grouped_columns_stream_while_the_worst_routing_allows(m, k, groups, n, 
         GK.matmul_grouped(cf, a, b, None, d, offsets)
         done()
         assert torch.equal(d.double(), want)
+
+
+@pytest.mark.parametrize("ta", [False, True])
+def test_grouped_columns_of_unaligned_operands_without_room(ta):
+    """More columns than the routing rule lets stream, and no workspace for the copies that the tensor cores would need: the
+    streaming kernel takes them after all."""
+    g = gen(315)
+    m, k, groups, n = 1023, 2049, 64, 48
+    w = ints(g, *((k, m) if ta else (m, k)), lo=-1, hi=1)
+    a = w[:, :, None].expand(*w.shape, groups)
+    b = ints(g, k, n, lo=-1, hi=1)
+    cf = conf(m, n, k, torch.float16, torch.float32, ta)
+    want = (w.double().T if ta else w.double()) @ b.double()
+    for counts in ([1] * n + [0] * (groups - n), [0] * (groups - 1) + [n]):
+        offsets, _ = offsets_of(counts)
+        for room in (256, None):
+            d = cm(torch.full((m, n), -9.0, device="cuda"))
+            GK.matmul_grouped(cf, a, b, None, d, offsets, workspace=room and torch.empty(room, dtype=torch.uint8, device="cuda"))
+            done()
+            assert torch.equal(d.double(), want)
